@@ -194,6 +194,136 @@ mlipcpp_error_t mlipcpp_b200_domain_step(mlipcpp_b200_domain_t domain, const flo
  * rows sent, halo copies sent -> stats[0..12]. */
 mlipcpp_error_t mlipcpp_b200_domain_stats(mlipcpp_b200_domain_t domain, double stats[13]);
 
+/* ---- Transformer-block operators on device tensors -----------------------
+ * No counterpart in the reference, whose layers exist only inside its graph
+ * (src/models/pet/pet_layers.cpp:242-492).  The pieces of a pre-norm block
+ * with a gated feed-forward part, on the caller's own device memory, forward
+ * and backward: for models built or trained around the library's, and called
+ * by its own PET models of that form.
+ *
+ * Matrices are row-major; ld* is the distance between rows in elements, at
+ * least the row's length (any value where there is at most one row).  All
+ * tensors of a call have the type `dtype` and lie on the calling thread's
+ * current device, aligned to their elements; rows whose address and stride
+ * are multiples of 16 bytes are read where they lie, others cost a copy.  A
+ * call may have no rows (gradients of weights are then zeros); features are
+ * at least 1, and rows and features below 2^31.  Outputs must not overlap
+ * inputs, but for a residual that is also the output with the same stride.
+ *
+ * Products accumulate in fp32; activations, norms and sums run in fp32 and
+ * each output is rounded once.  f32 products have fp32 accuracy (22-bit
+ * split operands, one scale per 128 elements of a row of x or of a gradient,
+ * and one per weight matrix).  A backward call recomputes what it needs from
+ * the forward's inputs; gradients that enter a product are rounded to the
+ * call's type first.  Results do not depend on timing: no sum's order varies.
+ * In f32 an infinite element makes its row or column of a product NaN.
+ *
+ * `workspace`: device memory of at least the bytes that the matching
+ * *_workspace call gives for the same arguments, 256-byte aligned (NULL where
+ * that is 0), free for reuse once the work on `stream` is done; calls that
+ * may run at the same time need one each.  Work is ordered on `stream` (NULL:
+ * the legacy default stream); nothing is allocated and nothing waited for, so
+ * calls can be captured into a graph.  Errors found before the launch are
+ * returned; mlipcpp_b200_ops_status reports a tensor-core pipeline whose
+ * bounded wait ran out since. */
+typedef enum {
+  MLIPCPP_B200_DTYPE_F32 = 0,
+  MLIPCPP_B200_DTYPE_F16 = 1,
+  MLIPCPP_B200_DTYPE_BF16 = 2
+} mlipcpp_b200_dtype_t;
+
+typedef enum {
+  MLIPCPP_B200_ACT_IDENTITY = 0,
+  MLIPCPP_B200_ACT_SIGMOID = 1,
+  MLIPCPP_B200_ACT_SILU = 2,
+  MLIPCPP_B200_ACT_GELU = 3,      /* z Phi(z) */
+  MLIPCPP_B200_ACT_GELU_TANH = 4, /* its tanh approximation */
+  MLIPCPP_B200_ACT_RELU = 5
+} mlipcpp_b200_activation_t;
+
+typedef enum {
+  MLIPCPP_B200_NORM_NONE = 0,
+  MLIPCPP_B200_NORM_RMS = 1,  /* x / sqrt(mean(x^2) + eps) */
+  MLIPCPP_B200_NORM_LAYER = 2 /* (x - mean) / sqrt(var + eps) */
+} mlipcpp_b200_norm_t;
+
+/* h = act(x w_gate^T + b_gate) * (x w_value^T + b_value):
+ * x [rows, in_features], w_gate and w_value [hidden, in_features], h and dh
+ * [rows, hidden]; biases [hidden] or NULL.  Forward reads the inputs and
+ * writes h; backward reads them and dh and writes each of dx, dw_gate,
+ * dw_value, db_gate and db_value that is not NULL. */
+typedef struct {
+  int32_t dtype, activation;
+  int64_t rows, in_features, hidden;
+  const void *x, *w_gate, *w_value, *b_gate, *b_value;
+  int64_t ldx, ldw_gate, ldw_value;
+  void *h;
+  int64_t ldh;
+  const void *dh;
+  int64_t lddh;
+  void *dx, *dw_gate, *dw_value, *db_gate, *db_value;
+  int64_t lddx, lddw_gate, lddw_value;
+} mlipcpp_b200_gated_linear_t;
+int64_t mlipcpp_b200_gated_linear_workspace(const mlipcpp_b200_gated_linear_t *args, bool backward);
+mlipcpp_error_t mlipcpp_b200_gated_linear(const mlipcpp_b200_gated_linear_t *args, void *workspace,
+                                          int64_t workspace_bytes, void *stream);
+mlipcpp_error_t mlipcpp_b200_gated_linear_backward(const mlipcpp_b200_gated_linear_t *args, void *workspace,
+                                                   int64_t workspace_bytes, void *stream);
+
+/* y = residual + scale act(x w^T + b): x [rows, in_features], w
+ * [out_features, in_features], residual (or NULL), y and dy [rows,
+ * out_features], b [out_features] or NULL.  Backward writes each of dx, dw
+ * and db that is not NULL (the residual's gradient is dy). */
+typedef struct {
+  int32_t dtype, activation;
+  int64_t rows, in_features, out_features;
+  float scale;
+  const void *x, *w, *b, *residual;
+  int64_t ldx, ldw, ldresidual;
+  void *y;
+  int64_t ldy;
+  const void *dy;
+  int64_t lddy;
+  void *dx, *dw, *db;
+  int64_t lddx, lddw;
+} mlipcpp_b200_linear_t;
+int64_t mlipcpp_b200_linear_workspace(const mlipcpp_b200_linear_t *args, bool backward);
+mlipcpp_error_t mlipcpp_b200_linear(const mlipcpp_b200_linear_t *args, void *workspace, int64_t workspace_bytes,
+                                    void *stream);
+mlipcpp_error_t mlipcpp_b200_linear_backward(const mlipcpp_b200_linear_t *args, void *workspace,
+                                             int64_t workspace_bytes, void *stream);
+
+/* stream = scale residual + gate * post(y), out = norm(stream), on rows of
+ * `features` <= 16384 elements: post and norm are none, RMS or layer norms
+ * (eps > 0) with an optional weight and bias [features]; y NULL leaves
+ * scale * residual; gate NULL is 1, ldgate 0 is one row for all, else a gate
+ * for every row.  Forward writes each of stream and out that is not NULL.
+ * Backward reads residual, y and the gradients dstream and dout (NULL: zero)
+ * and writes each gradient that is not NULL (dgate: [features] where ldgate
+ * is 0, else rows of stride lddgate). */
+typedef struct {
+  int32_t dtype, norm, post_norm;
+  int64_t rows, features;
+  float scale, eps;
+  const void *residual, *y, *weight, *bias, *post_weight, *post_bias, *gate;
+  int64_t ldresidual, ldy, ldgate;
+  void *stream, *out;
+  int64_t ldstream, ldout;
+  const void *dstream, *dout;
+  int64_t lddstream, lddout;
+  void *dresidual, *dy, *dweight, *dbias, *dpost_weight, *dpost_bias, *dgate;
+  int64_t lddresidual, lddy, lddgate;
+} mlipcpp_b200_residual_norm_t;
+int64_t mlipcpp_b200_residual_norm_workspace(const mlipcpp_b200_residual_norm_t *args, bool backward);
+mlipcpp_error_t mlipcpp_b200_residual_norm(const mlipcpp_b200_residual_norm_t *args, void *workspace,
+                                           int64_t workspace_bytes, void *stream);
+mlipcpp_error_t mlipcpp_b200_residual_norm_backward(const mlipcpp_b200_residual_norm_t *args, void *workspace,
+                                                    int64_t workspace_bytes, void *stream);
+
+/* Waits for `stream`; MLIPCPP_ERROR_COMPUTATION (once) if an operator on the
+ * current device has given up a wait since the last call. */
+mlipcpp_error_t mlipcpp_b200_ops_status(void *stream);
+
 /* Number of CUDA kernels this library has launched in this process. */
 int64_t mlipcpp_b200_kernel_launches(void);
 

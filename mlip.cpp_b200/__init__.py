@@ -114,6 +114,16 @@ def lib() -> ctypes.CDLL:
         "mlipcpp_b200_domain_set_atoms": (ctypes.c_int, [vp, i32, vp]),
         "mlipcpp_b200_domain_step": (ctypes.c_int, [vp, vp, vp, b, vp, vp]),
         "mlipcpp_b200_domain_stats": (ctypes.c_int, [vp, vp]),
+        "mlipcpp_b200_gated_linear_workspace": (i64, [vp, b]),
+        "mlipcpp_b200_gated_linear": (ctypes.c_int, [vp, vp, i64, vp]),
+        "mlipcpp_b200_gated_linear_backward": (ctypes.c_int, [vp, vp, i64, vp]),
+        "mlipcpp_b200_linear_workspace": (i64, [vp, b]),
+        "mlipcpp_b200_linear": (ctypes.c_int, [vp, vp, i64, vp]),
+        "mlipcpp_b200_linear_backward": (ctypes.c_int, [vp, vp, i64, vp]),
+        "mlipcpp_b200_residual_norm_workspace": (i64, [vp, b]),
+        "mlipcpp_b200_residual_norm": (ctypes.c_int, [vp, vp, i64, vp]),
+        "mlipcpp_b200_residual_norm_backward": (ctypes.c_int, [vp, vp, i64, vp]),
+        "mlipcpp_b200_ops_status": (ctypes.c_int, [vp]),
         "mlipcpp_b200_set_kernel_profiling": (ctypes.c_int, [vp, b]),
         "mlipcpp_b200_kernel_stats": (ctypes.c_int, [vp, vp]),
     }

@@ -13,6 +13,7 @@
 
 #include "mlipcpp.h"
 #include "mlipcpp_b200.h"
+#include "block.h"
 #include "domain.h"
 #include "gemm_tc.cuh"
 #include "gguf.h"
@@ -116,6 +117,263 @@ void finish_options(pet::Result &r, const mlipcpp_predict_options_t &o) {
   if (!o.compute_stress) {
     r.stress.clear();
     r.has_stress = false;
+  }
+}
+
+// ---- transformer-block operators --------------------------------------------
+// Checks of one call's arguments; the first that fails sets the error.
+struct OpCheck {
+  mlipcpp_error_t code = MLIPCPP_OK;
+  size_t es = 4;
+  void fail(mlipcpp_error_t c, const std::string &m) {
+    if (code != MLIPCPP_OK) return;
+    set_error(m);
+    code = c;
+  }
+  void range(int64_t v, int64_t lo, int64_t hi, const char *what) {
+    if (v < lo || v > hi)
+      fail(MLIPCPP_ERROR_INVALID_PARAMETER, std::string(what) + " must be between " + std::to_string(lo) + " and " +
+                                                std::to_string(hi) + " (got " + std::to_string(v) + ")");
+  }
+  void vec(const void *p, const char *what) {
+    if (reinterpret_cast<uintptr_t>(p) % es)
+      fail(MLIPCPP_ERROR_INVALID_PARAMETER, std::string(what) + " is not aligned to its elements");
+  }
+  // a matrix; needed: it may not be NULL
+  void mat(const void *p, int64_t ld, int64_t rows, int64_t cols, const char *what, bool needed) {
+    if (!p && needed && rows > 0) fail(MLIPCPP_ERROR_NULL_POINTER, std::string("NULL ") + what);
+    vec(p, what);
+    if (p && rows > 1 && ld < cols)
+      fail(MLIPCPP_ERROR_INVALID_PARAMETER, std::string("the row stride of ") + what + " is shorter than its rows");
+    if (p && rows > 1 && ld > (int64_t(1) << 37))
+      fail(MLIPCPP_ERROR_INVALID_PARAMETER, std::string("the row stride of ") + what + " is too long");
+  }
+};
+// At most one row: its stride says nothing; one that keeps 16-byte rows.
+int64_t op_ld(int64_t ld, int64_t rows, int64_t cols) { return rows > 1 ? ld : (cols + 7) / 8 * 8; }
+
+constexpr int64_t kOpMax = 2147483647;
+
+mlipcpp_error_t op_args(const mlipcpp_b200_gated_linear_t *a, bool back, pet::GatedLinear &o) {
+  OpCheck c;
+  if (!a) {
+    c.fail(MLIPCPP_ERROR_NULL_POINTER, "NULL arguments");
+    return c.code;
+  }
+  c.range(a->dtype, 0, 2, "dtype");
+  c.range(a->activation, 0, pet::ACT_COUNT - 1, "activation");
+  c.range(a->rows, 0, kOpMax, "rows");
+  c.range(a->in_features, 1, kOpMax, "in_features");
+  c.range(a->hidden, 1, kOpMax, "hidden");
+  if (c.code != MLIPCPP_OK) return c.code;
+  c.es = pet::dtype_size(a->dtype);
+  const int64_t M = a->rows, K = a->in_features, F = a->hidden;
+  c.mat(a->x, a->ldx, M, K, "x", true);
+  c.mat(a->w_gate, a->ldw_gate, F, K, "w_gate", M > 0);
+  c.mat(a->w_value, a->ldw_value, F, K, "w_value", M > 0);
+  c.vec(a->b_gate, "b_gate");
+  c.vec(a->b_value, "b_value");
+  if (!back) {
+    c.mat(a->h, a->ldh, M, F, "h", true);
+  } else {
+    c.mat(a->dh, a->lddh, M, F, "dh", true);
+    c.mat(a->dx, a->lddx, M, K, "dx", false);
+    c.mat(a->dw_gate, a->lddw_gate, F, K, "dw_gate", false);
+    c.mat(a->dw_value, a->lddw_value, F, K, "dw_value", false);
+    c.vec(a->db_gate, "db_gate");
+    c.vec(a->db_value, "db_value");
+  }
+  o.dtype = a->dtype;
+  o.act = a->activation;
+  o.M = M;
+  o.K = K;
+  o.F = F;
+  o.x = {a->x, op_ld(a->ldx, M, K)};
+  o.wg = {a->w_gate, op_ld(a->ldw_gate, F, K)};
+  o.wv = {a->w_value, op_ld(a->ldw_value, F, K)};
+  o.bg = a->b_gate;
+  o.bv = a->b_value;
+  o.h = {a->h, op_ld(a->ldh, M, F)};
+  o.dh = {a->dh, op_ld(a->lddh, M, F)};
+  o.dx = {a->dx, op_ld(a->lddx, M, K)};
+  o.dwg = {a->dw_gate, op_ld(a->lddw_gate, F, K)};
+  o.dwv = {a->dw_value, op_ld(a->lddw_value, F, K)};
+  o.dbg = a->db_gate;
+  o.dbv = a->db_value;
+  return c.code;
+}
+
+mlipcpp_error_t op_args(const mlipcpp_b200_linear_t *a, bool back, pet::Linear &o) {
+  OpCheck c;
+  if (!a) {
+    c.fail(MLIPCPP_ERROR_NULL_POINTER, "NULL arguments");
+    return c.code;
+  }
+  c.range(a->dtype, 0, 2, "dtype");
+  c.range(a->activation, 0, pet::ACT_COUNT - 1, "activation");
+  c.range(a->rows, 0, kOpMax, "rows");
+  c.range(a->in_features, 1, kOpMax, "in_features");
+  c.range(a->out_features, 1, kOpMax, "out_features");
+  if (!std::isfinite(a->scale)) c.fail(MLIPCPP_ERROR_INVALID_PARAMETER, "scale must be finite");
+  if (c.code != MLIPCPP_OK) return c.code;
+  c.es = pet::dtype_size(a->dtype);
+  const int64_t M = a->rows, K = a->in_features, N = a->out_features;
+  c.mat(a->x, a->ldx, M, K, "x", true);
+  c.mat(a->w, a->ldw, N, K, "w", M > 0);
+  c.vec(a->b, "b");
+  if (!back) {
+    c.mat(a->residual, a->ldresidual, M, N, "residual", false);
+    c.mat(a->y, a->ldy, M, N, "y", true);
+  } else {
+    c.mat(a->dy, a->lddy, M, N, "dy", true);
+    c.mat(a->dx, a->lddx, M, K, "dx", false);
+    c.mat(a->dw, a->lddw, N, K, "dw", false);
+    c.vec(a->db, "db");
+  }
+  o.dtype = a->dtype;
+  o.act = a->activation;
+  o.M = M;
+  o.K = K;
+  o.N = N;
+  o.scale = a->scale;
+  o.x = {a->x, op_ld(a->ldx, M, K)};
+  o.w = {a->w, op_ld(a->ldw, N, K)};
+  o.residual = {a->residual, op_ld(a->ldresidual, M, N)};
+  o.b = a->b;
+  o.y = {a->y, op_ld(a->ldy, M, N)};
+  o.dy = {a->dy, op_ld(a->lddy, M, N)};
+  o.dx = {a->dx, op_ld(a->lddx, M, K)};
+  o.dw = {a->dw, op_ld(a->lddw, N, K)};
+  o.db = a->db;
+  return c.code;
+}
+
+mlipcpp_error_t op_args(const mlipcpp_b200_residual_norm_t *a, bool back, pet::ResidualNorm &o) {
+  OpCheck c;
+  if (!a) {
+    c.fail(MLIPCPP_ERROR_NULL_POINTER, "NULL arguments");
+    return c.code;
+  }
+  c.range(a->dtype, 0, 2, "dtype");
+  c.range(a->norm, 0, pet::NORM_COUNT - 1, "norm");
+  c.range(a->post_norm, 0, pet::NORM_COUNT - 1, "post_norm");
+  c.range(a->rows, 0, kOpMax, "rows");
+  c.range(a->features, 1, pet::kMaxNormDim, "features");
+  if (!std::isfinite(a->scale)) c.fail(MLIPCPP_ERROR_INVALID_PARAMETER, "scale must be finite");
+  if (!std::isfinite(a->eps) || a->eps <= 0.f)
+    c.fail(MLIPCPP_ERROR_INVALID_PARAMETER, "eps must be finite and positive");
+  // (an empty tensor may have no address)
+  if (!a->y && a->rows > 0 && (a->post_norm != pet::NORM_NONE || a->gate || a->post_weight || a->post_bias))
+    c.fail(MLIPCPP_ERROR_INVALID_PARAMETER, "a post norm, its weight or bias, or a gate needs y");
+  if (a->post_norm == pet::NORM_NONE && (a->post_weight || a->post_bias))
+    c.fail(MLIPCPP_ERROR_INVALID_PARAMETER, "post_weight and post_bias need a post norm");
+  if (a->norm == pet::NORM_NONE && (a->weight || a->bias))
+    c.fail(MLIPCPP_ERROR_INVALID_PARAMETER, "weight and bias need a norm");
+  if (c.code != MLIPCPP_OK) return c.code;
+  c.es = pet::dtype_size(a->dtype);
+  const int64_t M = a->rows, d = a->features;
+  const bool each = a->ldgate != 0;  // a gate for every row
+  c.mat(a->residual, a->ldresidual, M, d, "residual", true);
+  c.mat(a->y, a->ldy, M, d, "y", false);
+  if (each) c.mat(a->gate, a->ldgate, M, d, "gate", false);
+  for (const void *v : {a->weight, a->bias, a->post_weight, a->post_bias, a->gate}) c.vec(v, "a weight, bias or gate");
+  if (!back) {
+    c.mat(a->stream, a->ldstream, M, d, "stream", false);
+    c.mat(a->out, a->ldout, M, d, "out", false);
+  } else {
+    c.mat(a->dstream, a->lddstream, M, d, "dstream", false);
+    c.mat(a->dout, a->lddout, M, d, "dout", false);
+    c.mat(a->dresidual, a->lddresidual, M, d, "dresidual", false);
+    c.mat(a->dy, a->lddy, M, d, "dy", false);
+    if (each) c.mat(a->dgate, a->lddgate, M, d, "dgate", false);
+    for (const void *v : {a->dweight, a->dbias, a->dpost_weight, a->dpost_bias, a->dgate})
+      c.vec(v, "a gradient of a weight, bias or gate");
+    if ((a->rows > 0 && a->dy && !a->y) || (a->rows > 0 && a->dgate && !a->gate) || (a->dpost_weight && !a->post_weight) ||
+        (a->dpost_bias && !a->post_bias) || (a->dweight && !a->weight) || (a->dbias && !a->bias))
+      c.fail(MLIPCPP_ERROR_INVALID_PARAMETER, "a gradient is wanted of an input that is not there");
+  }
+  o.dtype = a->dtype;
+  o.norm = a->norm;
+  o.post = a->post_norm;
+  o.M = M;
+  o.d = static_cast<int>(d);
+  o.scale = a->scale;
+  o.eps = a->eps;
+  o.residual = {a->residual, op_ld(a->ldresidual, M, d)};
+  o.y = {a->y, op_ld(a->ldy, M, d)};
+  o.gate = {a->gate, each ? op_ld(a->ldgate, M, d) : 0};
+  o.w = a->weight;
+  o.b = a->bias;
+  o.pw = a->post_weight;
+  o.pb = a->post_bias;
+  o.stream = {a->stream, op_ld(a->ldstream, M, d)};
+  o.out = {a->out, op_ld(a->ldout, M, d)};
+  o.dstream = {a->dstream, op_ld(a->lddstream, M, d)};
+  o.dout = {a->dout, op_ld(a->lddout, M, d)};
+  o.dresidual = {a->dresidual, op_ld(a->lddresidual, M, d)};
+  o.dy = {a->dy, op_ld(a->lddy, M, d)};
+  o.dgate = {a->dgate, each ? op_ld(a->lddgate, M, d) : 0};
+  o.dw = a->dweight;
+  o.db = a->dbias;
+  o.dpw = a->dpost_weight;
+  o.dpb = a->dpost_bias;
+  return c.code;
+}
+
+template <typename Op, typename Args, typename Fn>
+int64_t op_workspace(const Args *args, bool back, Fn run) {
+  Op o;
+  if (const mlipcpp_error_t e = op_args(args, back, o)) return -static_cast<int64_t>(e);
+  if (!have_cuda_device()) {
+    set_error("No CUDA device available (this backend has no CPU fallback)");
+    return -MLIPCPP_ERROR_BACKEND;
+  }
+  try {
+    pet::Workspace ws;
+    run(o, ws, nullptr);
+    clear_error();
+    return static_cast<int64_t>(ws.off);
+  } catch (const pet::Error &e) {
+    set_error(e.what());
+    return -static_cast<int64_t>(e.code);
+  } catch (const std::exception &e) {
+    set_error(e.what());
+    return -MLIPCPP_ERROR_COMPUTATION;
+  }
+}
+
+template <typename Op, typename Args, typename Fn>
+mlipcpp_error_t op_run(const Args *args, bool back, void *workspace, int64_t bytes, void *stream, Fn run) {
+  Op o;
+  if (const mlipcpp_error_t e = op_args(args, back, o)) return e;
+  if (bytes < 0 || (bytes > 0 && !workspace) || reinterpret_cast<uintptr_t>(workspace) % 256) {
+    set_error("The workspace must be 256-byte aligned device memory of the given size");
+    return MLIPCPP_ERROR_INVALID_PARAMETER;
+  }
+  if (!have_cuda_device()) {
+    set_error("No CUDA device available (this backend has no CPU fallback)");
+    return MLIPCPP_ERROR_BACKEND;
+  }
+  try {
+    pet::Workspace need;
+    run(o, need, nullptr);  // sizes only: nothing is launched with too little
+    if (static_cast<int64_t>(need.off) > bytes) {
+      set_error("The workspace is too small (" + std::to_string(bytes) + " of " + std::to_string(need.off) + " bytes)");
+      return MLIPCPP_ERROR_INVALID_PARAMETER;
+    }
+    pet::Workspace ws;
+    // a call without working memory still runs: any non-null base will do
+    ws.base = workspace ? static_cast<char *>(workspace) : reinterpret_cast<char *>(256);
+    ws.cap = static_cast<size_t>(bytes);
+    run(o, ws, static_cast<cudaStream_t>(stream));
+    clear_error();
+    return MLIPCPP_OK;
+  } catch (const pet::Error &e) {
+    set_error(e.what());
+    return static_cast<mlipcpp_error_t>(e.code);
+  } catch (const std::exception &e) {
+    set_error(e.what());
+    return MLIPCPP_ERROR_COMPUTATION;
   }
 }
 
@@ -970,6 +1228,61 @@ mlipcpp_error_t mlipcpp_b200_kernel_stats(mlipcpp_model_t model, double stats[24
     stats[4 * c + 1] = k[c].ms;
     stats[4 * c + 2] = k[c].flops;
     stats[4 * c + 3] = k[c].bytes;
+  }
+  clear_error();
+  return MLIPCPP_OK;
+}
+
+// ---- transformer-block operators --------------------------------------------
+int64_t mlipcpp_b200_gated_linear_workspace(const mlipcpp_b200_gated_linear_t *args, bool backward) {
+  return op_workspace<pet::GatedLinear>(args, backward, backward ? pet::gated_linear_bwd : pet::gated_linear_fwd);
+}
+mlipcpp_error_t mlipcpp_b200_gated_linear(const mlipcpp_b200_gated_linear_t *args, void *workspace,
+                                          int64_t workspace_bytes, void *stream) {
+  return op_run<pet::GatedLinear>(args, false, workspace, workspace_bytes, stream, pet::gated_linear_fwd);
+}
+mlipcpp_error_t mlipcpp_b200_gated_linear_backward(const mlipcpp_b200_gated_linear_t *args, void *workspace,
+                                                   int64_t workspace_bytes, void *stream) {
+  return op_run<pet::GatedLinear>(args, true, workspace, workspace_bytes, stream, pet::gated_linear_bwd);
+}
+
+int64_t mlipcpp_b200_linear_workspace(const mlipcpp_b200_linear_t *args, bool backward) {
+  return op_workspace<pet::Linear>(args, backward, backward ? pet::linear_bwd : pet::linear_fwd);
+}
+mlipcpp_error_t mlipcpp_b200_linear(const mlipcpp_b200_linear_t *args, void *workspace, int64_t workspace_bytes,
+                                    void *stream) {
+  return op_run<pet::Linear>(args, false, workspace, workspace_bytes, stream, pet::linear_fwd);
+}
+mlipcpp_error_t mlipcpp_b200_linear_backward(const mlipcpp_b200_linear_t *args, void *workspace,
+                                             int64_t workspace_bytes, void *stream) {
+  return op_run<pet::Linear>(args, true, workspace, workspace_bytes, stream, pet::linear_bwd);
+}
+
+int64_t mlipcpp_b200_residual_norm_workspace(const mlipcpp_b200_residual_norm_t *args, bool backward) {
+  return op_workspace<pet::ResidualNorm>(args, backward, backward ? pet::residual_norm_bwd : pet::residual_norm_fwd);
+}
+mlipcpp_error_t mlipcpp_b200_residual_norm(const mlipcpp_b200_residual_norm_t *args, void *workspace,
+                                           int64_t workspace_bytes, void *stream) {
+  return op_run<pet::ResidualNorm>(args, false, workspace, workspace_bytes, stream, pet::residual_norm_fwd);
+}
+mlipcpp_error_t mlipcpp_b200_residual_norm_backward(const mlipcpp_b200_residual_norm_t *args, void *workspace,
+                                                    int64_t workspace_bytes, void *stream) {
+  return op_run<pet::ResidualNorm>(args, true, workspace, workspace_bytes, stream, pet::residual_norm_bwd);
+}
+
+mlipcpp_error_t mlipcpp_b200_ops_status(void *stream) {
+  if (!have_cuda_device()) {
+    set_error("No CUDA device available (this backend has no CPU fallback)");
+    return MLIPCPP_ERROR_BACKEND;
+  }
+  try {
+    if (pet::block_status(static_cast<cudaStream_t>(stream))) {
+      set_error("A tensor-core pipeline of an operator timed out; its outputs are incomplete");
+      return MLIPCPP_ERROR_COMPUTATION;
+    }
+  } catch (const pet::Error &e) {
+    set_error(e.what());
+    return static_cast<mlipcpp_error_t>(e.code);
   }
   clear_error();
   return MLIPCPP_OK;

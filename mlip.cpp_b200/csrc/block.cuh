@@ -1,0 +1,150 @@
+// Device helpers of the transformer-block operators: element types,
+// activations with their derivatives, and the launchers shared between the
+// operators' files.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "block.h"
+#include "common.cuh"
+
+namespace pet {
+namespace blk {
+
+inline bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+// Rows of p can be read or written in 16-byte pieces.
+inline bool rows16(const void *p, int64_t ld, int dt) {
+  return aligned16(p) && (ld * static_cast<int64_t>(dtype_size(dt))) % 16 == 0;
+}
+// SMs of the current device.
+int sm_count();
+
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f(float x);
+template <>
+__device__ __forceinline__ float from_f<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// 16 bytes of T <-> floats
+template <typename T>
+struct Vec {
+  static constexpr int n = 16 / sizeof(T);
+};
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4 &u, float (&v)[16 / sizeof(T)]) {
+  const T *t = reinterpret_cast<const T *>(&u);
+#pragma unroll
+  for (int j = 0; j < Vec<T>::n; ++j) v[j] = to_f(t[j]);
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack(const float (&v)[16 / sizeof(T)]) {
+  uint4 u;
+  T *t = reinterpret_cast<T *>(&u);
+#pragma unroll
+  for (int j = 0; j < Vec<T>::n; ++j) t[j] = from_f<T>(v[j]);
+  return u;
+}
+
+// 1 / (1 + e^-z).  kFast (16-bit results): the intrinsics, a few ulp of fp32,
+// far below the result's half step.  The exponent's argument stops at -80,
+// where the result is below 2e-35, so that e^-z stays finite.
+template <bool kFast>
+__device__ __forceinline__ float logistic(float z) {
+  const float t = fmaxf(z, -80.f);
+  return kFast ? __fdividef(1.f, 1.f + __expf(-t)) : 1.f / (1.f + expf(-t));
+}
+
+// a = act(z), da = act'(z)
+template <int ACT, bool kFast>
+__device__ __forceinline__ void act_pair(float z, float &a, float &da) {
+  if (ACT == ACT_SIGMOID) {
+    a = logistic<kFast>(z);
+    da = a * (1.f - a);
+  } else if (ACT == ACT_SILU) {
+    const float p = logistic<kFast>(z);
+    a = z * p;
+    da = p * (1.f + z * (1.f - p));
+  } else if (ACT == ACT_GELU) {
+    const float c = normcdff(z);
+    a = z * c;
+    const float e = kFast ? __expf(-0.5f * z * z) : expf(-0.5f * z * z);
+    da = c + z * e * 0.3989422804014327f;
+  } else if (ACT == ACT_GELU_TANH) {
+    const float p = logistic<kFast>(1.5957691216057308f * (z + 0.044715f * z * z * z));
+    a = z * p;
+    da = p + z * p * (1.f - p) * 1.5957691216057308f * (1.f + 0.134145f * z * z);
+  } else if (ACT == ACT_RELU) {
+    a = z > 0.f ? z : (z == z ? 0.f : z);
+    da = z > 0.f ? 1.f : 0.f;
+  } else {
+    a = z;
+    da = 1.f;
+  }
+}
+template <int ACT, bool kFast>
+__device__ __forceinline__ float act_only(float z) {
+  float a, da;
+  act_pair<ACT, kFast>(z, a, da);
+  return a;
+}
+template <int V>
+struct Const {
+  static constexpr int value = V;
+};
+// f(Const<act>{}) for the run-time activation (one uniform branch)
+template <typename F>
+__device__ __forceinline__ void with_act(int act, F &&f) {
+  switch (act) {
+    case ACT_SIGMOID: f(Const<ACT_SIGMOID>{}); break;
+    case ACT_SILU: f(Const<ACT_SILU>{}); break;
+    case ACT_GELU: f(Const<ACT_GELU>{}); break;
+    case ACT_GELU_TANH: f(Const<ACT_GELU_TANH>{}); break;
+    case ACT_RELU: f(Const<ACT_RELU>{}); break;
+    default: f(Const<ACT_IDENTITY>{}); break;
+  }
+}
+// Element j of a vector of run-time type.
+__device__ __forceinline__ float load_dt(const void *p, int dt, int64_t j) {
+  if (dt == DT_F32) return static_cast<const float *>(p)[j];
+  if (dt == DT_F16) return __half2float(static_cast<const __half *>(p)[j]);
+  return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[j]);
+}
+__device__ __forceinline__ void store_dt(void *p, int dt, int64_t j, float v) {
+  if (dt == DT_F32) static_cast<float *>(p)[j] = v;
+  else if (dt == DT_F16) static_cast<__half *>(p)[j] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16 *>(p)[j] = __float2bfloat16_rn(v);
+}
+
+// ---- few rows (block_rows.cu) ---------------------------------------------
+// Forward of at most kFewRows rows: reads each weight once with plain loads.
+constexpr int kFewRows = 8;
+struct FewRows {
+  int dt, act, M;
+  int64_t K, N;
+  const void *x, *w0, *w1;  // w1 null: linear
+  int64_t ldx, ldw0, ldw1;
+  const void *b0, *b1, *res;
+  int64_t ldr;
+  float scale;
+  void *out;
+  int64_t ldo;
+};
+void few_rows(const FewRows &a, cudaStream_t s);
+
+// Column sums of a [M, N] matrix (fp32 sums in a fixed order), times scale,
+// into out [N]; `part`: column_sum_floats(M, N) floats.
+// out[c] = scale sum over p < P of part[p][c], in a fixed order.
+void column_join(const float *part, int P, int64_t N, float scale, void *out, int dt, cudaStream_t s);
+size_t column_sum_floats(int64_t M, int64_t N);
+void column_sum(const void *p, int dt_in, int64_t ld, int64_t M, int64_t N, float scale, void *out, int dt_out,
+                float *part, cudaStream_t s);
+
+}  // namespace blk
+}  // namespace pet

@@ -1,0 +1,239 @@
+// Transformer-block operators for a handful of rows (single tokens), and the
+// column sums of the bias gradients.
+//
+// With at most 8 rows the dense forward is the time it takes to read the
+// weights once: one to eight warps per output feature stream its weight rows
+// with 16-byte loads, several in flight per lane, and multiply them with every
+// row of x, which stays in L1.  The sums run in fp32 FMAs; the tensor cores
+// would idle behind the same loads, and a 128-row tile would leave most SMs
+// without work.
+#include <algorithm>
+
+#include "block.cuh"
+
+namespace pet {
+namespace blk {
+
+namespace {
+
+constexpr int kDepth = 4;  // 16-byte loads in flight per lane and weight
+
+template <typename T, int MR, bool DUAL, bool VEC>
+__global__ void __launch_bounds__(256) k_few_rows(const FewRows a, int wpr) {
+  constexpr int V = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
+  constexpr int NS = DUAL ? 2 * MR : MR;
+  __shared__ float part[8][NS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * (8 / wpr) + warp / wpr;
+  const int sub = warp % wpr;
+  float sum[NS];
+#pragma unroll
+  for (int i = 0; i < NS; ++i) sum[i] = 0.f;
+  if (n < a.N) {
+    const T *x = static_cast<const T *>(a.x);
+    const T *w0 = static_cast<const T *>(a.w0) + n * a.ldw0;
+    const T *w1 = DUAL ? static_cast<const T *>(a.w1) + n * a.ldw1 : nullptr;
+    const int64_t step = static_cast<int64_t>(wpr) * 32 * V;
+    for (int64_t k0 = (static_cast<int64_t>(sub) * 32 + lane) * V; k0 < a.K; k0 += kDepth * step) {
+      if (VEC) {
+        uint4 r0[kDepth], r1[kDepth];
+#pragma unroll
+        for (int u = 0; u < kDepth; ++u) {
+          const int64_t k = k0 + u * step;
+          r0[u] = r1[u] = make_uint4(0u, 0u, 0u, 0u);
+          if (k < a.K) {
+            r0[u] = __ldg(reinterpret_cast<const uint4 *>(w0 + k));
+            if (DUAL) r1[u] = __ldg(reinterpret_cast<const uint4 *>(w1 + k));
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kDepth; ++u) {
+          const int64_t k = k0 + u * step;
+          if (k >= a.K) break;
+          float f0[16 / sizeof(T)], f1[16 / sizeof(T)];
+          unpack<T>(r0[u], f0);
+          if (DUAL) unpack<T>(r1[u], f1);
+#pragma unroll
+          for (int m = 0; m < MR; ++m) {
+            if (m >= a.M) break;
+            float xv[16 / sizeof(T)];
+            unpack<T>(__ldg(reinterpret_cast<const uint4 *>(x + m * a.ldx + k)), xv);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              sum[m] = fmaf(xv[j], f0[j], sum[m]);
+              if (DUAL) sum[MR * (DUAL ? 1 : 0) + m] = fmaf(xv[j], f1[j], sum[MR * (DUAL ? 1 : 0) + m]);
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < kDepth; ++u) {
+          const int64_t k = k0 + u * step;
+          if (k >= a.K) break;
+          const float f0 = to_f(w0[k]), f1 = DUAL ? to_f(w1[k]) : 0.f;
+#pragma unroll
+          for (int m = 0; m < MR; ++m) {
+            if (m >= a.M) break;
+            const float xv = to_f(x[m * a.ldx + k]);
+            sum[m] = fmaf(xv, f0, sum[m]);
+            if (DUAL) sum[MR * (DUAL ? 1 : 0) + m] = fmaf(xv, f1, sum[MR * (DUAL ? 1 : 0) + m]);
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NS; ++i) sum[i] = warp_sum(sum[i]);
+  if (wpr > 1) {
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) part[warp][i] = sum[i];
+    }
+    __syncthreads();
+    if (sub) return;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      float t = 0.f;
+      for (int w = 0; w < wpr; ++w) t += part[warp + w][i];
+      sum[i] = t;
+    }
+  }
+  // lane m finishes row m
+  float v = 0.f, w = 0.f;
+#pragma unroll
+  for (int m = 0; m < MR; ++m)
+    if (lane == m) {
+      v = sum[m];
+      if (DUAL) w = sum[MR * (DUAL ? 1 : 0) + m];
+    }
+  if (n >= a.N || lane >= a.M) return;
+  if (a.b0) v += to_f(static_cast<const T *>(a.b0)[n]);
+  if (DUAL && a.b1) w += to_f(static_cast<const T *>(a.b1)[n]);
+  with_act(a.act, [&](auto A) { v = act_only<decltype(A)::value, sizeof(T) == 2>(v); });
+  if (DUAL) v *= w;
+  else v = v * a.scale + (a.res ? to_f(static_cast<const T *>(a.res)[lane * a.ldr + n]) : 0.f);
+  static_cast<T *>(a.out)[lane * a.ldo + n] = from_f<T>(v);
+}
+
+template <typename T, int MR, bool DUAL>
+void launch_rows(const FewRows &a, cudaStream_t s) {
+  constexpr int V = 16 / static_cast<int>(sizeof(T));
+  const bool vec = a.K % V == 0 && rows16(a.x, a.ldx, a.dt) && rows16(a.w0, a.ldw0, a.dt) &&
+                   (!DUAL || rows16(a.w1, a.ldw1, a.dt));
+  // warps per output feature: enough of them for every SM to have 16, as
+  // long as each still has a full load of its own
+  int wpr = 1;
+  while (wpr < 8 && a.N * wpr < 16LL * sm_count() && a.K > 64LL * wpr * (vec ? V : 1)) wpr *= 2;
+  const unsigned grid = static_cast<unsigned>((a.N + 8 / wpr - 1) / (8 / wpr));
+  if (vec) k_few_rows<T, MR, DUAL, true><<<grid, 256, 0, s>>>(a, wpr);
+  else k_few_rows<T, MR, DUAL, false><<<grid, 256, 0, s>>>(a, wpr);
+  CUDA_LAUNCH_CHECK();
+}
+template <typename T, bool DUAL>
+void rows_of(const FewRows &a, cudaStream_t s) {
+  if (a.M == 1) launch_rows<T, 1, DUAL>(a, s);
+  else if (a.M <= 4) launch_rows<T, 4, DUAL>(a, s);
+  else launch_rows<T, kFewRows, DUAL>(a, s);
+}
+
+// Sums of columns over a strip of rows, a fixed share of it per warp.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) k_column_part(const T *__restrict__ p, int64_t ld, int64_t M, int64_t N,
+                                                     int64_t strip, float *part) {
+  constexpr int V = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
+  __shared__ float sums[8][32 * V];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t c = (static_cast<int64_t>(blockIdx.x) * 32 + lane) * V;
+  const int64_t r0 = blockIdx.y * strip, r1 = min(M, r0 + strip);
+  float acc[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) acc[j] = 0.f;
+  if (c < N) {
+#pragma unroll 4
+    for (int64_t r = r0 + warp; r < r1; r += 8) {
+      if (VEC) {
+        float v[16 / sizeof(T)];
+        unpack<T>(__ldg(reinterpret_cast<const uint4 *>(p + r * ld + c)), v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[j] += v[j];
+      } else {
+        acc[0] += to_f(p[r * ld + c]);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) sums[warp][lane * V + j] = acc[j];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * V; i += 256) {
+    const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 * V + i;
+    if (col >= N) continue;
+    float t = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) t += sums[w][i];
+    part[blockIdx.y * N + col] = t;
+  }
+}
+
+// out[c] = scale sum_p part[p][c], the parts in 8 interleaved shares.
+__global__ void __launch_bounds__(256) k_column_join(const float *__restrict__ part, int P, int64_t N, float scale,
+                                                     void *out, int dt) {
+  __shared__ float sums[8][33];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  float acc = 0.f;
+  if (c < N)
+    for (int q = warp; q < P; q += 8) acc += part[q * N + c];
+  sums[warp][lane] = acc;
+  __syncthreads();
+  if (warp == 0 && c < N) {
+    float t = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) t += sums[w][lane];
+    store_dt(out, dt, c, t * scale);
+  }
+}
+
+constexpr int kStrips = 128;
+int strips(int64_t M) { return static_cast<int>(std::min<int64_t>(kStrips, (M + 63) / 64)); }
+
+template <typename T>
+void column_parts(const void *p, int dt, int64_t ld, int64_t M, int64_t N, int y, float *part, cudaStream_t s) {
+  constexpr int V = 16 / static_cast<int>(sizeof(T));
+  const int64_t strip = (M + y - 1) / y;
+  const T *t = static_cast<const T *>(p);
+  if (N % V == 0 && rows16(p, ld, dt)) {
+    const dim3 g(static_cast<unsigned>((N + 32 * V - 1) / (32 * V)), y);
+    k_column_part<T, true><<<g, 256, 0, s>>>(t, ld, M, N, strip, part);
+  } else {
+    const dim3 g(static_cast<unsigned>((N + 31) / 32), y);
+    k_column_part<T, false><<<g, 256, 0, s>>>(t, ld, M, N, strip, part);
+  }
+  CUDA_LAUNCH_CHECK();
+}
+
+}  // namespace
+
+void few_rows(const FewRows &a, cudaStream_t s) {
+  if (a.dt == DT_F32) a.w1 ? rows_of<float, true>(a, s) : rows_of<float, false>(a, s);
+  else if (a.dt == DT_F16) a.w1 ? rows_of<__half, true>(a, s) : rows_of<__half, false>(a, s);
+  else a.w1 ? rows_of<__nv_bfloat16, true>(a, s) : rows_of<__nv_bfloat16, false>(a, s);
+}
+
+size_t column_sum_floats(int64_t M, int64_t N) { return static_cast<size_t>(strips(M)) * N; }
+
+void column_join(const float *part, int P, int64_t N, float scale, void *out, int dt, cudaStream_t s) {
+  k_column_join<<<static_cast<unsigned>((N + 31) / 32), 256, 0, s>>>(part, P, N, scale, out, dt);
+  CUDA_LAUNCH_CHECK();
+}
+
+void column_sum(const void *p, int dt_in, int64_t ld, int64_t M, int64_t N, float scale, void *out, int dt_out,
+                float *part, cudaStream_t s) {
+  const int y = strips(M);
+  if (dt_in == DT_F32) column_parts<float>(p, dt_in, ld, M, N, y, part, s);
+  else if (dt_in == DT_F16) column_parts<__half>(p, dt_in, ld, M, N, y, part, s);
+  else column_parts<__nv_bfloat16>(p, dt_in, ld, M, N, y, part, s);
+  column_join(part, y, N, scale, out, dt_out, s);
+}
+
+}  // namespace blk
+}  // namespace pet
