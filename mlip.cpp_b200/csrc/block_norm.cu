@@ -7,21 +7,26 @@
 //
 // The backward recomputes both norms from r and y: it reads r, y, dstream and
 // dout and writes dr and dy, with no statistics stored by the forward.
-//   dn = dout w,     dstream' = dstream + norm'(dn)
-//   dr = scale dstream',  dgate = dstream' u,  dp = gate dstream' pw
-//   dy = post'(dp)
+//   dn = dout w,     g = dstream + norm'(dn)
+//   dr = scale g,  dgate = g u,  dp = gate g pw,  dy = post'(dp)
 // where norm'(dn) = (dn - [mean dn] - n mean(dn n)) / sigma.  The gradients
-// of the vectors (weights, biases, a gate of one row) are summed per CTA over
-// its rows in registers, written once per CTA and added in a fixed order by a
-// second kernel.
+// of the vectors (weights, biases, a gate of one row) come from two sums over
+// rows per column, four with biases (k_norm_vectors): kept per CTA over its
+// rows in registers, written once per CTA and added in a fixed order.
 //
-// A row takes 32 threads (up to 512 or 1,024 columns; eight rows per CTA) or
-// a CTA.  Rows of 16-byte-aligned tensors move in 16-byte pieces, others by
-// elements.
+// A CTA of 256 or more threads holds one or more groups of threads that take
+// a row each, 8 or 16 elements a thread.  A group is persistent: the inputs of
+// its next rows come into a ring in shared memory with bulk copies while it
+// works on one, so that loads need no registers and the reductions' latency
+// (two to six a row) is covered by the other groups and CTAs of the SM.  What
+// has rows that are not 16-byte aligned, or too long for the ring, is read
+// directly.
 #include <algorithm>
+#include <type_traits>
 
 #include "block.cuh"
 #include "split16.cuh"
+#include "tc_common.cuh"
 
 namespace pet {
 namespace blk {
@@ -42,449 +47,660 @@ struct NormArgs {
   int64_t ldds, lddo;
   void *dr, *dy, *dgate;       // dgate: the gate of each row
   int64_t lddr, lddy, lddg;
-  float *part;                 // [CTA][vector][d] of the vectors' gradients
-  int want;                    // bit v: vector v wanted (0 w, 1 b, 2 pw, 3 pb, 4 gate)
+  float *part;                 // [sum][CTA][d] of the vectors' gradients, or null
+  bool hb;                     // a bias or its gradient is there
 };
 
-// Column of element j of chunk i of thread t (VEC: 16-byte chunks).
-template <typename T, int TPR, bool VEC>
+// 16 bytes of T <-> pairs of floats
+template <typename T>
+__device__ __forceinline__ void open16(const uint4 &v, float2 *x) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  if constexpr (sizeof(T) == 4) {
+    x[0] = make_float2(__uint_as_float(w[0]), __uint_as_float(w[1]));
+    x[1] = make_float2(__uint_as_float(w[2]), __uint_as_float(w[3]));
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (std::is_same<T, __half>::value) x[k] = __half22float2(*reinterpret_cast<const __half2 *>(&w[k]));
+      else x[k] = make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 close16(const float2 *x) {
+  uint32_t w[4];
+  if constexpr (sizeof(T) == 4) {
+    w[0] = __float_as_uint(x[0].x);
+    w[1] = __float_as_uint(x[0].y);
+    w[2] = __float_as_uint(x[1].x);
+    w[3] = __float_as_uint(x[1].y);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(x[k].x, x[k].y);
+        w[k] = *reinterpret_cast<const uint32_t *>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x[k].x, x[k].y);
+        w[k] = *reinterpret_cast<const uint32_t *>(&h);
+      }
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A thread's share of a row: E elements as E / 2 pairs (the pair forms of the
+// fp32 instructions take one issue slot for two elements).  VEC: element e is
+// in 16-byte chunk e / V, chunks of a row dealt out over its TPR threads;
+// otherwise the elements are dealt out one by one.
+// FULL: the row has exactly TPR * E columns, so nothing needs a bound.
+template <typename T, int TPR, int E, bool VEC, bool FULL = false>
 struct Row {
   static constexpr int V = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
+  static constexpr int NV = E / V, P = E / 2;
   static __device__ __forceinline__ int col(int i, int t) { return (i * TPR + t) * V; }
-  // zeros past d (VEC: d is a multiple of V)
-  static __device__ __forceinline__ void load(const void *p, int64_t off, int c, int d, float (&v)[V]) {
-    const T *q = static_cast<const T *>(p) + off + c;
-    if (VEC) {
-      uint4 u = make_uint4(0u, 0u, 0u, 0u);
-      if (c < d) u = *reinterpret_cast<const uint4 *>(q);
-      float f[16 / sizeof(T)];
-      unpack<T>(u, f);
+  // elements of one row at p + off; zeros past d (VEC: d is a multiple of V)
+  static __device__ __forceinline__ void load(const void *p, int64_t off, int t, int d, float2 (&x)[P]) {
+    const T *q = static_cast<const T *>(p) + off;
+    if constexpr (VEC) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = f[j];
+      for (int i = 0; i < NV; ++i) {
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (FULL || col(i, t) < d) v = *reinterpret_cast<const uint4 *>(q + col(i, t));
+        open16<T>(v, &x[i * V / 2]);
+      }
     } else {
-      v[0] = c < d ? to_f(*q) : 0.f;
+#pragma unroll
+      for (int k = 0; k < P; ++k) {
+        const int c0 = col(2 * k, t), c1 = col(2 * k + 1, t);
+        x[k] = make_float2(c0 < d ? to_f(q[c0]) : 0.f, c1 < d ? to_f(q[c1]) : 0.f);
+      }
     }
   }
-  static __device__ __forceinline__ void store(void *p, int64_t off, int c, int d, const float (&v)[V]) {
-    if (c >= d) return;
-    T *q = static_cast<T *>(p) + off + c;
-    if (VEC) {
-      float f[16 / sizeof(T)];
+  static __device__ __forceinline__ void store(void *p, int64_t off, int t, int d, const float2 (&x)[P]) {
+    T *q = static_cast<T *>(p) + off;
+    if constexpr (VEC) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) f[j] = v[j];
-      *reinterpret_cast<uint4 *>(q) = pack<T>(f);
+      for (int i = 0; i < NV; ++i)
+        if (FULL || col(i, t) < d) *reinterpret_cast<uint4 *>(q + col(i, t)) = close16<T>(&x[i * V / 2]);
     } else {
-      *q = from_f<T>(v[0]);
+#pragma unroll
+      for (int k = 0; k < P; ++k) {
+        const int c0 = col(2 * k, t), c1 = col(2 * k + 1, t);
+        if (c0 < d) q[c0] = from_f<T>(x[k].x);
+        if (c1 < d) q[c1] = from_f<T>(x[k].y);
+      }
+    }
+  }
+  // fp32 copy of a vector in shared memory (VEC), zeros from d on, in the
+  // order in which a warp reads it 16 bytes a lane: place of column c
+  static constexpr int kCopy = TPR * E;
+  static __device__ __forceinline__ int place(int c) {
+    const int i = c / (TPR * V), t = c / V % TPR, j = c % V;
+    return ((i * (V / 4) + j / 4) * TPR + t) * 4 + j % 4;
+  }
+  static __device__ __forceinline__ void load_copy(const float *p, int t, float2 (&x)[P]) {
+#pragma unroll
+    for (int k = 0; k < P; k += 2) {
+      const float4 v = *reinterpret_cast<const float4 *>(p + (k / 2 * TPR + t) * 4);
+      x[k] = make_float2(v.x, v.y);
+      x[k + 1] = make_float2(v.z, v.w);
+    }
+  }
+  // zeros into the columns past d
+  static __device__ __forceinline__ void trim(int t, int d, float2 (&x)[P]) {
+    if (FULL) return;
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      if (col(2 * k / V, t) >= d) x[k].x = 0.f;
+      if (col((2 * k + 1) / V, t) >= d) x[k].y = 0.f;
     }
   }
 };
 
-// Sums over the threads of a row.  Two slots in turn, so one barrier each:
-// a slot is written again only after every thread has passed the barrier
-// that follows its last read.
+__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
+template <int P>
+__device__ __forceinline__ float dot(const float2 (&a)[P], const float2 (&b)[P]) {
+  float2 s = __fmul2_rn(a[0], b[0]);
+#pragma unroll
+  for (int k = 1; k < P; ++k) s = __ffma2_rn(a[k], b[k], s);
+  return s.x + s.y;
+}
+template <int P>
+__device__ __forceinline__ float total(const float2 (&a)[P]) {
+  float2 s = a[0];
+#pragma unroll
+  for (int k = 1; k < P; ++k) s = __fadd2_rn(a[k], s);
+  return s.x + s.y;
+}
+
+// The threads of one row: TPR of a CTA's, at a barrier of their own.
+template <int TPR>
+__device__ __forceinline__ void group_sync(int group) {
+  if (TPR == 32) __syncwarp();
+  else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(TPR) : "memory");
+}
+
+// Sums over the threads of a row, in a fixed order.  Two slots in turn, so
+// one barrier each: a slot is written again only after every thread has
+// passed the barrier that follows its last read.
 template <int TPR>
 struct Sum {
-  float2 *slots;
-  int k;
-  __device__ __forceinline__ float2 two(float a, float b) {
-    a = warp_sum(a);
-    b = warp_sum(b);
-    if (TPR == 32) return make_float2(a, b);
-    float2 *s = slots + (k & 1) * 32;
-    k ^= 1;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (lane == 0) s[warp] = make_float2(a, b);
-    __syncthreads();
-    float2 v = lane < TPR / 32 ? s[lane] : make_float2(0.f, 0.f);
-    return make_float2(warp_sum(v.x), warp_sum(v.y));
-  }
-  __device__ __forceinline__ float one(float a) {
+  static constexpr int W = TPR / 32;  // warps of a row
+  float *slots;                       // [2][32] of this group, 16-byte aligned
+  int group, k;
+  __device__ __forceinline__ float operator()(float a) {
     a = warp_sum(a);
     if (TPR == 32) return a;
-    float2 *s = slots + (k & 1) * 32;
+    float *s = slots + (k & 1) * 32;
     k ^= 1;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (lane == 0) s[warp].x = a;
-    __syncthreads();
-    return warp_sum(lane < TPR / 32 ? s[lane].x : 0.f);
+    if ((threadIdx.x & 31) == 0) s[(threadIdx.x >> 5) % W] = a;
+    group_sync<TPR>(group);
+    if (W == 2) return s[0] + s[1];
+    float4 v = *reinterpret_cast<const float4 *>(s);
+#pragma unroll
+    for (int i = 4; i < (W > 4 ? W : 4); i += 4) {
+      const float4 u = *reinterpret_cast<const float4 *>(s + i);
+      v.x += u.x;
+      v.y += u.y;
+      v.z += u.z;
+      v.w += u.w;
+    }
+    return (v.x + v.y) + (v.z + v.w);
   }
 };
 
 // x -> its normalised row (columns past d stay 0); returns 1 / sigma.
-template <typename R, int TPR, int NV>
-__device__ __forceinline__ float normalise(int kind, float eps, int d, int t, Sum<TPR> &sum, float (&x)[NV][R::V]) {
+template <typename R, int TPR>
+__device__ __forceinline__ float normalise(int kind, float eps, int d, float rd, int t, Sum<TPR> &sum, float2 (&x)[R::P]) {
   if (kind == NORM_LAYER) {
-    float a = 0.f;
+    const float mean = sum(total(x)) * rd;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < R::V; ++j) a += x[i][j];
-    const float mean = sum.one(a) / static_cast<float>(d);
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < R::V; ++j)
-        if (R::col(i, t) < d) x[i][j] -= mean;
+    for (int k = 0; k < R::P; ++k) x[k] = __fadd2_rn(x[k], both(-mean));
+    R::trim(t, d, x);
   }
-  float q = 0.f;
+  const float inv = rsqrtf(fmaf(sum(dot(x, x)), rd, eps));  // 2 ulp
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < R::V; ++j) q = fmaf(x[i][j], x[i][j], q);
-  const float inv = 1.f / sqrtf(sum.one(q) / static_cast<float>(d) + eps);
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < R::V; ++j) x[i][j] *= inv;
+  for (int k = 0; k < R::P; ++k) x[k] = __fmul2_rn(x[k], both(inv));
   return inv;
 }
 
-template <int TPR>
-constexpr int block_threads() { return TPR == 32 ? 256 : TPR; }
+__device__ int g_norm_err = 0;
 
-template <typename T, int TPR, int E, bool VEC>
-__global__ void __launch_bounds__(block_threads<TPR>()) k_norm_fwd(const NormArgs a) {
-  using R = Row<T, TPR, VEC>;
-  constexpr int V = R::V, NV = E / V;
-  __shared__ float2 slots[64];
-  const int t = TPR == 32 ? (threadIdx.x & 31) : threadIdx.x;
-  const int64_t row = TPR == 32 ? static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5) : blockIdx.x;
-  if (row >= a.M) return;
-  Sum<TPR> sum{slots, 0};
-  const int d = a.d;
-  float x[NV][V];
+constexpr int kMaxStages = 4;
+constexpr int kInputs = 5;  // rows of a stage: r, y, dstream, dout, gate
+
+// Shared memory of a CTA: fp32 copies of the vectors there are (Vectors),
+// then per group a ring of `stages` stages of `inputs` rows.
+struct Ring {
+  int stages, inputs;  // stages 0: rows are read directly
+  int row_bytes, vector_bytes;
+  int bytes(int groups) const { return vector_bytes + row_bytes * groups * stages * inputs; }
+};
+
+// One group's ring: `take` waits for the next row's inputs.
+template <int TPR>
+struct Feed {
+  const NormArgs &a;
+  const Ring &ring;
+  uint64_t *bars;
+  char *base;
+  int64_t row, step;
+  int t, stage, phase;
+  bool ok;
+  __device__ __forceinline__ void issue(int s, int64_t at) {
+    const void *src[kInputs] = {a.r, a.y, a.ds, a.dout, a.ldg ? a.gate : nullptr};
+    const int64_t ld[kInputs] = {a.ldr, a.ldy, a.ldds, a.lddo, a.ldg};
+    const uint32_t bar = tc::smem_u32(bars + s);
+    const int64_t es = ring.row_bytes / a.d;
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(ring.inputs * ring.row_bytes) : "memory");
+    char *dst = base + static_cast<size_t>(s) * ring.inputs * ring.row_bytes;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) R::load(a.r, row * a.ldr, R::col(i, t), d, x[i]);
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) x[i][j] *= a.scale;
-  if (a.y) {
-    float u[NV][V];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) R::load(a.y, row * a.ldy, R::col(i, t), d, u[i]);
-    if (a.post != NORM_NONE) normalise<R, TPR, NV>(a.post, a.eps, d, t, sum, u);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = R::col(i, t);
-      float f[V];
-      if (a.pw) {
-        R::load(a.pw, 0, c, d, f);
-#pragma unroll
-        for (int j = 0; j < V; ++j) u[i][j] *= f[j];
-      }
-      if (a.pb) {
-        R::load(a.pb, 0, c, d, f);
-#pragma unroll
-        for (int j = 0; j < V; ++j) u[i][j] += f[j];
-      }
-      if (a.gate) {
-        R::load(a.gate, row * a.ldg, c, d, f);
-#pragma unroll
-        for (int j = 0; j < V; ++j) u[i][j] *= f[j];
-      }
-#pragma unroll
-      for (int j = 0; j < V; ++j) x[i][j] += u[i][j];
+    for (int k = 0; k < kInputs; ++k) {
+      if (!src[k]) continue;
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                   ::"r"(tc::smem_u32(dst)), "l"(static_cast<const char *>(src[k]) + at * ld[k] * es),
+                     "r"(ring.row_bytes), "r"(bar) : "memory");
+      dst += ring.row_bytes;
     }
   }
-  if (a.stream) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) R::store(a.stream, row * a.lds, R::col(i, t), d, x[i]);
+  __device__ __forceinline__ void start() {
+    if (t == 0)
+      for (int s = 0; s < ring.stages && row + s * step < a.M; ++s) issue(s, row + s * step);
   }
-  if (!a.out && !a.split.hi) return;
-  if (a.norm != NORM_NONE) normalise<R, TPR, NV>(a.norm, a.eps, d, t, sum, x);
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = R::col(i, t);
-    float f[V];
-    if (a.w) {
-      R::load(a.w, 0, c, d, f);
-#pragma unroll
-      for (int j = 0; j < V; ++j) x[i][j] *= f[j];
+  __device__ __forceinline__ const char *take() {
+    const uint32_t bar = tc::smem_u32(bars + stage);
+    if (ok && !tc::mbar_try_wait(bar, phase) && !tc::wait_bounded(bar, phase)) {
+      ok = false;  // waits no more: the results are void, the copies land by themselves
+      atomicExch(&g_norm_err, 1);
     }
-    if (a.b) {
-      R::load(a.b, 0, c, d, f);
-#pragma unroll
-      for (int j = 0; j < V; ++j) x[i][j] += f[j];
+    return base + static_cast<size_t>(stage) * ring.inputs * ring.row_bytes;
+  }
+  // every thread of the group has read the stage (after a group barrier)
+  __device__ __forceinline__ void give(int64_t at) {
+    if (t == 0 && at + ring.stages * step < a.M) issue(stage, at + ring.stages * step);
+    if (++stage == ring.stages) {
+      stage = 0;
+      phase ^= 1;
     }
-    if (a.out) R::store(a.out, row * a.ldo, c, d, x[i]);
-    if (sizeof(T) == 4 && VEC) {
+  }
+};
+
+// What a row is multiplied with and shifted by after post (gw, gb, with the
+// gate where it is one row for all) and after norm (w, b): in shared memory
+// in fp32 (RING) or the tensors themselves.
+template <typename R, typename T, bool RING>
+struct Vectors {
+  const NormArgs &a;
+  const float *w = nullptr, *b = nullptr, *gw = nullptr, *gb = nullptr;
+  static __host__ __device__ int count(const NormArgs &a) {
+    const bool row = a.gate && !a.ldg;
+    return (a.w ? 1 : 0) + (a.b ? 1 : 0) + (a.pw || row ? 1 : 0) + (a.pb ? 1 : 0);
+  }
+  // all threads of the CTA; returns the end of the copies
+  __device__ __forceinline__ void copy(float *dst) {
+    const T *gate = a.ldg ? nullptr : static_cast<const T *>(a.gate);
+    auto one = [&](const void *p, const T *times, const float *&out) {
+      if (!p && !times) return;
+      const T *q = static_cast<const T *>(p);
+      for (int c = threadIdx.x; c < R::kCopy; c += blockDim.x)
+        dst[R::place(c)] = c < a.d ? (q ? to_f(q[c]) : 1.f) * (times ? to_f(times[c]) : 1.f) : 0.f;
+      out = dst;
+      dst += R::kCopy;
+    };
+    one(a.w, nullptr, w);
+    one(a.b, nullptr, b);
+    one(a.pw, gate, gw);
+    if (a.pb) one(a.pb, gate, gb);
+  }
+  __device__ __forceinline__ void scale(const float *in, const void *p, const void *times, int t, float2 (&x)[R::P], bool add) const {
+    float2 f[R::P];
+    if (RING) {
+      if (!in) return;
+      R::load_copy(in, t, f);
+    } else {
+      if (!p && !times) return;
+      if (p) R::load(p, 0, t, a.d, f);
+      if (times) {
+        float2 g[R::P];
+        R::load(times, 0, t, a.d, g);
+#pragma unroll
+        for (int k = 0; k < R::P; ++k) f[k] = p ? __fmul2_rn(f[k], g[k]) : g[k];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < R::P; ++k) x[k] = add ? __fadd2_rn(x[k], f[k]) : __fmul2_rn(x[k], f[k]);
+  }
+  __device__ __forceinline__ const void *row_gate() const { return a.ldg ? nullptr : a.gate; }
+  __device__ __forceinline__ void times_w(int t, float2 (&x)[R::P]) const { scale(w, a.w, nullptr, t, x, false); }
+  __device__ __forceinline__ void plus_b(int t, float2 (&x)[R::P]) const { scale(b, a.b, nullptr, t, x, true); }
+  __device__ __forceinline__ void times_gw(int t, float2 (&x)[R::P]) const { scale(gw, a.pw, row_gate(), t, x, false); }
+  __device__ __forceinline__ void plus_gb(int t, float2 (&x)[R::P]) const {
+    if (a.pb) scale(gb, a.pb, row_gate(), t, x, true);
+  }
+};
+
+// What both directions set up: this thread's group, its first row, its ring
+// and the vectors.
+#define PET_NORM_SETUP                                                                                     \
+  extern __shared__ __align__(128) char smem[];                                                            \
+  __shared__ alignas(16) float slots[NG][64];                                                              \
+  __shared__ uint64_t bars[NG][kMaxStages];                                                                \
+  const int t = threadIdx.x % TPR, group = threadIdx.x / TPR, d = a.d;                                     \
+  const float rd = 1.f / static_cast<float>(d);                                                            \
+  const int64_t step = static_cast<int64_t>(gridDim.x) * NG;                                               \
+  int64_t row = static_cast<int64_t>(blockIdx.x) * NG + group;                                             \
+  Sum<TPR> sum{slots[group], group, 0};                                                                    \
+  Vectors<R, T, RING> vec{a};                                                                              \
+  Feed<TPR> feed{a, ring, bars[group], nullptr, row, step, t, 0, 0, true};                                 \
+  if (RING) {                                                                                              \
+    if (threadIdx.x == 0) {                                                                                \
+      for (int g = 0; g < NG; ++g)                                                                         \
+        for (int s = 0; s < ring.stages; ++s) tc::mbar_init(tc::smem_u32(&bars[g][s]), 1);                 \
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");                                   \
+    }                                                                                                      \
+    __syncthreads();                                                                                       \
+    feed.base = smem + ring.vector_bytes + static_cast<size_t>(ring.row_bytes) * group * ring.stages * ring.inputs; \
+    feed.start();                                                                                          \
+    vec.copy(reinterpret_cast<float *>(smem));                                                             \
+    __syncthreads();                                                                                       \
+  }
+
+// NT threads, NT / TPR groups.  MODE 0: single elements, 1: 16-byte pieces,
+// 2: with the inputs' rows in the ring, 3: and FULL rows.
+template <typename T, int TPR, int NT, int E, int MODE>
+__global__ void __launch_bounds__(NT, 1024 / NT) k_norm_fwd(const NormArgs a, const Ring ring) {
+  using R = Row<T, TPR, E, MODE != 0, MODE == 3>;
+  constexpr int P = R::P, NG = NT / TPR;
+  constexpr bool RING = MODE >= 2;
+  PET_NORM_SETUP
+  for (; row < a.M; row += step) {
+    float2 x[P];
+    const char *in = nullptr;
+    if (RING) in = feed.take();
+    if (RING) R::load(in, 0, t, d, x);
+    else R::load(a.r, row * a.ldr, t, d, x);
+#pragma unroll
+    for (int k = 0; k < P; ++k) x[k] = __fmul2_rn(x[k], both(a.scale));
+    if (a.y) {
+      float2 u[P];
+      if (RING) R::load(in + ring.row_bytes, 0, t, d, u);
+      else R::load(a.y, row * a.ldy, t, d, u);
+      if (a.post != NORM_NONE) normalise<R, TPR>(a.post, a.eps, d, rd, t, sum, u);
+      vec.times_gw(t, u);
+      vec.plus_gb(t, u);
+      if (a.ldg) {
+        float2 f[P];
+        if (RING) R::load(in + 2 * ring.row_bytes, 0, t, d, f);
+        else R::load(a.gate, row * a.ldg, t, d, f);
+#pragma unroll
+        for (int k = 0; k < P; ++k) x[k] = __ffma2_rn(u[k], f[k], x[k]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < P; ++k) x[k] = __fadd2_rn(x[k], u[k]);
+      }
+    }
+    if (RING) {
+      group_sync<TPR>(group);
+      feed.give(row);
+    }
+    if (a.stream) R::store(a.stream, row * a.lds, t, d, x);
+    if (!a.out && !a.split.hi) continue;
+    if (a.norm != NORM_NONE) normalise<R, TPR>(a.norm, a.eps, d, rd, t, sum, x);
+    vec.times_w(t, x);
+    vec.plus_b(t, x);
+    if (a.out) R::store(a.out, row * a.ldo, t, d, x);
+    if constexpr (sizeof(T) == 4 && MODE != 0) {
       // a warp's 16-byte chunks are one 128-column block
-      if (a.split.hi && c / 128 * 128 < d)
-        warp_split_block(a.split, static_cast<int>(row), c / 128,
-                         make_float4(x[i][0], x[i][V > 1 ? 1 : 0], x[i][V > 2 ? 2 : 0], x[i][V > 3 ? 3 : 0]),
-                         threadIdx.x & 31);
+      if (a.split.hi) {
+#pragma unroll
+        for (int i = 0; i < R::NV; ++i) {
+          const int blk = R::col(i, t) / 128;
+          if (blk * 128 < d)
+            warp_split_block(a.split, static_cast<int>(row), blk, make_float4(x[2 * i].x, x[2 * i].y, x[2 * i + 1].x, x[2 * i + 1].y),
+                             threadIdx.x & 31);
+        }
+      }
     }
   }
 }
 
-// One row's four inputs as they lie in memory, read a row ahead.
-template <typename T, int TPR, int E, bool VEC>
-struct Raw {
-  using R = Row<T, TPR, VEC>;
-  static constexpr int V = R::V, NV = E / V;
-  struct alignas(VEC ? 16 : sizeof(T)) Piece {
-    T e[V];
-  };
-  Piece p[4][NV];
-  __device__ __forceinline__ void load(const NormArgs &a, int64_t row, int t) {
-    const void *src[4] = {a.r, a.y, a.ds, a.dout};
-    const int64_t ld[4] = {a.ldr, a.ldy, a.ldds, a.lddo};
+// HB: a bias or its gradient is there (its sums take E registers each).
+template <typename T, int TPR, int NT, int E, int MODE, bool HB>
+__global__ void __launch_bounds__(NT, NT == 256 ? 2 : 1) k_norm_bwd(const NormArgs a, const Ring ring) {
+  using R = Row<T, TPR, E, MODE != 0, MODE == 3>;
+  constexpr int P = R::P, NG = NT / TPR;
+  constexpr bool RING = MODE >= 2;
+  PET_NORM_SETUP
+  const bool each = a.ldg != 0;  // a gate for every row
+  // sums over rows of do n, q u (and do, q), where q is the stream's
+  // gradient, times the gate if each row has its own
+  constexpr int NA = HB ? 4 : 2;
+  float2 acc[NA][P];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+  for (int v = 0; v < NA; ++v)
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = R::col(i, t);
-        if (src[k] && c < a.d)
-          p[k][i] = *reinterpret_cast<const Piece *>(static_cast<const T *>(src[k]) + row * ld[k] + c);
-        else
-#pragma unroll
-          for (int j = 0; j < V; ++j) p[k][i].e[j] = from_f<T>(0.f);
-      }
-  }
-};
-
-template <typename T, int TPR, int E, bool VEC>
-__global__ void __launch_bounds__(block_threads<TPR>()) k_norm_bwd(const NormArgs a) {
-  using R = Row<T, TPR, VEC>;
-  constexpr int V = R::V, NV = E / V;
-  __shared__ float2 slots[64];
-  const int warp = threadIdx.x >> 5;
-  const int t = TPR == 32 ? (threadIdx.x & 31) : threadIdx.x;
-  const int64_t step = TPR == 32 ? static_cast<int64_t>(gridDim.x) * 8 : gridDim.x;
-  const int d = a.d;
-  const float rd = 1.f / static_cast<float>(d);
-  Sum<TPR> sum{slots, 0};
-  float acc[5][NV][V];
-#pragma unroll
-  for (int v = 0; v < 5; ++v)
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) acc[v][i][j] = 0.f;
-  int64_t row = TPR == 32 ? static_cast<int64_t>(blockIdx.x) * 8 + warp : blockIdx.x;
-  Raw<T, TPR, E, VEC> raw;
-  if (row < a.M) raw.load(a, row, t);
+    for (int k = 0; k < P; ++k) acc[v][k] = both(0.f);
   for (; row < a.M; row += step) {
-    float n[NV][V], u[NV][V], g[NV][V], o[NV][V];
+    float2 n[P], u[P], g[P], f[P];
+    const char *in[kInputs] = {};
+    if (RING) {
+      const char *p = feed.take();
+      const void *there[kInputs] = {a.r, a.y, a.ds, a.dout, each ? a.gate : nullptr};
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        n[i][j] = to_f(raw.p[0][i].e[j]) * a.scale;
-        u[i][j] = to_f(raw.p[1][i].e[j]);
-        g[i][j] = to_f(raw.p[2][i].e[j]);
-        o[i][j] = to_f(raw.p[3][i].e[j]);
-      }
-    if (row + step < a.M) raw.load(a, row + step, t);
-    // u: post's normalised row; n: the stream, then its normalised row
-    float pinv = 1.f, inv = 1.f;
-    if (a.y) {
-      if (a.post != NORM_NONE) pinv = normalise<R, TPR, NV>(a.post, a.eps, d, t, sum, u);
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = R::col(i, t);
-        float w[V], b[V], gt[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          w[j] = 1.f;
-          b[j] = 0.f;
-          gt[j] = 1.f;
-        }
-        if (a.pw) R::load(a.pw, 0, c, d, w);
-        if (a.pb) R::load(a.pb, 0, c, d, b);
-        if (a.gate) R::load(a.gate, row * a.ldg, c, d, gt);
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (c < d) n[i][j] = fmaf(gt[j], fmaf(u[i][j], w[j], b[j]), n[i][j]);
+      for (int k = 0; k < kInputs; ++k) {
+        in[k] = p;
+        if (there[k]) p += ring.row_bytes;
       }
     }
+    auto input = [&](int k, const void *p, int64_t ld, float2(&x)[P]) {
+      if (RING) R::load(in[k], 0, t, d, x);
+      else R::load(p, row * ld, t, d, x);
+    };
+    // times the row's own gate
+    auto gated = [&](float2(&x)[P]) {
+      if (!each) return;
+      input(4, a.gate, a.ldg, f);
+#pragma unroll
+      for (int k = 0; k < P; ++k) x[k] = __fmul2_rn(x[k], f[k]);
+    };
+    // u: post's normalised row; n: the stream, then its normalised row
+    input(0, a.r, a.ldr, n);
+#pragma unroll
+    for (int k = 0; k < P; ++k) n[k] = __fmul2_rn(n[k], both(a.scale));
+    float pinv = 1.f;
+    if (a.y) {
+      input(1, a.y, a.ldy, u);
+      if (a.post != NORM_NONE) pinv = normalise<R, TPR>(a.post, a.eps, d, rd, t, sum, u);
+#pragma unroll
+      for (int k = 0; k < P; ++k) g[k] = u[k];
+      vec.times_gw(t, g);
+      if (HB) vec.plus_gb(t, g);
+      gated(g);
+#pragma unroll
+      for (int k = 0; k < P; ++k) n[k] = __fadd2_rn(n[k], g[k]);
+    }
+    float inv = 1.f;
     if (a.dout) {
-      if (a.norm != NORM_NONE) inv = normalise<R, TPR, NV>(a.norm, a.eps, d, t, sum, n);
-      float s0 = 0.f, s1 = 0.f;
+      float2 (&o)[P] = g;
+      if (a.norm != NORM_NONE) inv = normalise<R, TPR>(a.norm, a.eps, d, rd, t, sum, n);
+      input(3, a.dout, a.lddo, o);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = R::col(i, t);
-        float w[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) w[j] = 1.f;
-        if (a.w) R::load(a.w, 0, c, d, w);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          acc[0][i][j] = fmaf(o[i][j], n[i][j], acc[0][i][j]);
-          acc[1][i][j] += o[i][j];
-          o[i][j] *= w[j];
-          s0 += o[i][j];
-          s1 = fmaf(o[i][j], n[i][j], s1);
-        }
+      for (int k = 0; k < P; ++k) {
+        acc[0][k] = __ffma2_rn(o[k], n[k], acc[0][k]);
+        if (HB) acc[NA / 2][k] = __fadd2_rn(acc[NA / 2][k], o[k]);
       }
+      vec.times_w(t, o);
       if (a.norm != NORM_NONE) {
-        const float2 m = sum.two(s0, s1);
-        const float m0 = a.norm == NORM_LAYER ? m.x * rd : 0.f, m1 = m.y * rd;
+        if (a.norm == NORM_LAYER) {
+          const float m0 = sum(total(o)) * rd;
+          // (the mean of n is 0: what follows does not see the shift)
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+          for (int k = 0; k < P; ++k) o[k] = __fadd2_rn(o[k], both(-m0));
+          R::trim(t, d, o);
+        }
+        const float m1 = -sum(dot(o, n)) * rd;
 #pragma unroll
-          for (int j = 0; j < V; ++j) g[i][j] += (o[i][j] - m0 - n[i][j] * m1) * inv;
-      } else {
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-          for (int j = 0; j < V; ++j) g[i][j] += o[i][j];
+        for (int k = 0; k < P; ++k) o[k] = __fmul2_rn(__ffma2_rn(n[k], both(m1), o[k]), both(inv));
       }
+    } else {
+#pragma unroll
+      for (int k = 0; k < P; ++k) g[k] = both(0.f);
+    }
+    if (a.ds) {
+      input(2, a.ds, a.ldds, f);
+#pragma unroll
+      for (int k = 0; k < P; ++k) g[k] = __fadd2_rn(g[k], f[k]);
     }
     // g: the stream's gradient
     if (a.dr) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        float v[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = g[i][j] * a.scale;
-        R::store(a.dr, row * a.lddr, R::col(i, t), d, v);
-      }
+      for (int k = 0; k < P; ++k) f[k] = __fmul2_rn(g[k], both(a.scale));
+      R::store(a.dr, row * a.lddr, t, d, f);
     }
-    if (!a.y) continue;
-    float s0 = 0.f, s1 = 0.f;
+    if (a.y) {
+      if (a.dgate) {  // (the gate is the row's own: gw and gb are pw and pb)
+        float2 (&v)[P] = n;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = R::col(i, t);
-      float w[V], b[V], gt[V], dg[V];
+        for (int k = 0; k < P; ++k) v[k] = u[k];
+        vec.times_gw(t, v);
+        if (HB) vec.plus_gb(t, v);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        w[j] = 1.f;
-        b[j] = 0.f;
-        gt[j] = 1.f;
+        for (int k = 0; k < P; ++k) v[k] = __fmul2_rn(v[k], g[k]);
+        R::store(a.dgate, row * a.lddg, t, d, v);
       }
-      if (a.pw) R::load(a.pw, 0, c, d, w);
-      if (a.gate) {
-        if (a.pb) R::load(a.pb, 0, c, d, b);
-        R::load(a.gate, row * a.ldg, c, d, gt);
-      }
+      gated(g);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const bool in = c < d;
-        const float gj = in ? g[i][j] : 0.f;
-        dg[j] = gj * fmaf(u[i][j], w[j], b[j]);
-        acc[4][i][j] += dg[j];
-        const float du = gj * gt[j];
-        acc[2][i][j] = fmaf(du, u[i][j], acc[2][i][j]);
-        acc[3][i][j] += du;
-        g[i][j] = du * w[j];
-        s0 += g[i][j];
-        s1 = fmaf(g[i][j], u[i][j], s1);
+      for (int k = 0; k < P; ++k) {
+        acc[1][k] = __ffma2_rn(g[k], u[k], acc[1][k]);
+        if (HB) acc[NA - 1][k] = __fadd2_rn(acc[NA - 1][k], g[k]);
       }
-      if (a.dgate) R::store(a.dgate, row * a.lddg, c, d, dg);
+      vec.times_gw(t, g);
+    }
+    if (RING) {
+      group_sync<TPR>(group);
+      feed.give(row);
     }
     if (a.dy) {
       if (a.post != NORM_NONE) {
-        const float2 m = sum.two(s0, s1);
-        const float m0 = a.post == NORM_LAYER ? m.x * rd : 0.f, m1 = m.y * rd;
+        if (a.post == NORM_LAYER) {
+          const float m0 = sum(total(g)) * rd;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+          for (int k = 0; k < P; ++k) g[k] = __fadd2_rn(g[k], both(-m0));
+          R::trim(t, d, g);
+        }
+        const float m1 = -sum(dot(g, u)) * rd;
 #pragma unroll
-          for (int j = 0; j < V; ++j) g[i][j] = (g[i][j] - m0 - u[i][j] * m1) * pinv;
+        for (int k = 0; k < P; ++k) g[k] = __fmul2_rn(__ffma2_rn(u[k], both(m1), g[k]), both(pinv));
       }
-#pragma unroll
-      for (int i = 0; i < NV; ++i) R::store(a.dy, row * a.lddy, R::col(i, t), d, g[i]);
+      R::store(a.dy, row * a.lddy, t, d, g);
     }
   }
-  // this CTA's sums of the wanted vectors
+  // this CTA's sums, each [CTA][d], the groups' added in order
   if (!a.part) return;
-  if (TPR == 32) {
-    __shared__ float total[TPR == 32 ? 32 * E : 1];
-    int slot = 0;
-    for (int v = 0; v < 5; ++v) {
-      if (!((a.want >> v) & 1)) continue;
-      for (int w = 0; w < 8; ++w) {
-        if (warp == w) {
 #pragma unroll
-          for (int k = 0; k < 5; ++k)
-            if (k == v)
+  for (int v = 0; v < NA; ++v) {
+    float *dst = a.part + (static_cast<size_t>(v) * gridDim.x + blockIdx.x) * d;
+    if constexpr (NG == 1) {
 #pragma unroll
-              for (int i = 0; i < NV; ++i)
+      for (int e = 0; e < E; ++e) {
+        const int c = R::col(e / R::V, t) + e % R::V;
+        if (c < d) dst[c] = e % 2 ? acc[v][e / 2].y : acc[v][e / 2].x;
+      }
+    } else {
+      __shared__ float sums[NG > 1 ? TPR * E : 1];
+      for (int i = 0; i < NG; ++i) {
+        if (group == i) {
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                  const int c = R::col(i, t) + j;
-                  total[c] = w ? total[c] + acc[k][i][j] : acc[k][i][j];
-                }
+          for (int e = 0; e < E; ++e) {
+            const int c = R::col(e / R::V, t) + e % R::V;
+            const float x = e % 2 ? acc[v][e / 2].y : acc[v][e / 2].x;
+            sums[c] = i ? sums[c] + x : x;
+          }
         }
         __syncthreads();
       }
-      float *dst = a.part + (static_cast<size_t>(slot) * gridDim.x + blockIdx.x) * d;
-      for (int c = threadIdx.x; c < d; c += 256) dst[c] = total[c];
+      for (int c = threadIdx.x; c < d; c += NT) dst[c] = sums[c];
       __syncthreads();
-      ++slot;
-    }
-  } else {
-    int slot = 0;
-#pragma unroll
-    for (int v = 0; v < 5; ++v) {
-      if (!((a.want >> v) & 1)) continue;
-      float *dst = a.part + (static_cast<size_t>(slot) * gridDim.x + blockIdx.x) * d;
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int c = R::col(i, t) + j;
-          if (c < d) dst[c] = acc[v][i][j];
-        }
-      ++slot;
     }
   }
 }
 
-template <typename T, int TPR, int E, bool VEC, bool BWD>
-void launch(const NormArgs &a, int grid, cudaStream_t s) {
-  if constexpr (BWD) k_norm_bwd<T, TPR, E, VEC><<<grid, block_threads<TPR>(), 0, s>>>(a);
-  else k_norm_fwd<T, TPR, E, VEC><<<grid, block_threads<TPR>(), 0, s>>>(a);
-  CUDA_LAUNCH_CHECK();
+// The vectors' gradients from the CTAs' sums, in a fixed order; block: 32
+// columns x 8 interleaved shares.
+//   dw = sum do n, db = sum do;  with one gate for all rows (or none)
+//   dpw = gate sum q u, dpb = gate sum q, dgate = pw sum q u + pb sum q.
+struct VectorGrads {
+  const float *part;
+  int P, d, dt;
+  bool hb;
+  const void *pw, *pb, *gate;  // gate: of one row, or null
+  void *dw, *db, *dpw, *dpb, *dgate;
+};
+__global__ void __launch_bounds__(256) k_norm_vectors(const VectorGrads a) {
+  __shared__ float sums[4][8][33];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c = blockIdx.x * 32 + lane, na = a.hb ? 4 : 2;
+  for (int v = 0; v < na; ++v) {
+    float s = 0.f;
+    if (c < a.d) {
+      const float *p = a.part + static_cast<size_t>(v) * a.P * a.d + c;
+#pragma unroll 16
+      for (int q = warp; q < a.P; q += 8) s += p[static_cast<size_t>(q) * a.d];
+    }
+    sums[v][warp][lane] = s;
+  }
+  __syncthreads();
+  if (warp || c >= a.d) return;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int v = 0; v < na; ++v)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[v] += sums[v][i][lane];
+  const float gate = a.gate ? load_dt(a.gate, a.dt, c) : 1.f;
+  if (a.dw) store_dt(a.dw, a.dt, c, s[0]);
+  if (a.db) store_dt(a.db, a.dt, c, s[2]);
+  if (a.dpw) store_dt(a.dpw, a.dt, c, gate * s[1]);
+  if (a.dpb) store_dt(a.dpb, a.dt, c, gate * s[3]);
+  if (a.dgate) {
+    const float pw = a.pw ? load_dt(a.pw, a.dt, c) : 1.f, pb = a.pb ? load_dt(a.pb, a.dt, c) : 0.f;
+    store_dt(a.dgate, a.dt, c, pw * s[1] + pb * s[3]);
+  }
 }
 
-// Threads per row of the backward (8 elements each, 16 at the ends of the
-// range): its gradients' sums take five registers per element.
-int bwd_threads(int d) { return d <= 512 ? 32 : d <= 1024 ? 128 : d <= 2048 ? 256 : d <= 4096 ? 512 : 1024; }
-// CTAs of the backward: as many as are resident at once, each with its own
-// share of the rows and one set of sums.
-int bwd_grid(int64_t M, int d) {
-  const int tpr = bwd_threads(d);
-  const int64_t rows = tpr == 32 ? (M + 7) / 8 : M;
-  const int per_sm = tpr <= 128 ? 4 : tpr == 256 ? 2 : 1;
-  return static_cast<int>(std::min<int64_t>(rows, static_cast<int64_t>(per_sm) * sm_count()));
+constexpr int kSmemPerSm = 224 * 1024;
+
+// How a call is laid out: threads per row and per CTA, CTAs per SM and the
+// ring.  16-bit rows take 16 elements a thread and two CTAs of 256 threads an
+// SM (128 registers a thread hold a row's values and its column sums); f32
+// rows 8 and one of 512, since their ring is twice as large.  The grid is what
+// is resident at once.
+struct Layout {
+  int tpr, nt, grid;
+  Ring ring;
+};
+Layout layout_of(const NormArgs &a, int dt, bool vec, bool bwd) {
+  const int es = static_cast<int>(dtype_size(dt)), e = dt == DT_F32 ? 8 : 16;
+  Layout l{32, dt == DT_F32 ? 512 : 256, 0, {0, 0, a.d * es, Vectors<Row<float, 32, 8, true>, float, true>::count(a)}};
+  while (l.tpr * e < a.d && l.tpr < 1024) l.tpr *= 2;
+  l.ring.vector_bytes *= 4 * l.tpr * (l.tpr == 1024 ? 16 : e);
+  l.nt = std::max(l.nt, l.tpr);
+  const int groups = l.nt / l.tpr;
+  // forwards hold half the registers
+  int per_sm = std::max(1, (bwd ? 512 : 1024) / l.nt);
+  if (vec) {
+    Ring &r = l.ring;
+    for (const void *p : {a.r, a.y, a.ds, a.dout, a.ldg ? a.gate : nullptr}) r.inputs += p ? 1 : 0;
+    // at least two stages, fewer CTAs rather than fewer stages
+    for (; per_sm >= 1; --per_sm) {
+      const int room = kSmemPerSm / per_sm - 15 * 1024 - r.vector_bytes;
+      r.stages = std::min(kMaxStages, room / (groups * r.inputs * r.row_bytes));
+      if (r.stages >= 2) break;
+    }
+    if (per_sm < 1) {
+      r.stages = 0;
+      per_sm = std::max(1, (bwd ? 512 : 1024) / l.nt);
+    }
+  }
+  l.grid = static_cast<int>(std::min<int64_t>((a.M + groups - 1) / groups, static_cast<int64_t>(per_sm) * sm_count()));
+  return l;
 }
 
-template <typename T, bool VEC>
-void fwd(const NormArgs &a, cudaStream_t s) {
-  const int d = a.d;
-  const int64_t M = a.M;
-  const int warps = static_cast<int>((M + 7) / 8), rows = static_cast<int>(M);
-  if (d <= 256) launch<T, 32, 8, VEC, false>(a, warps, s);
-  else if (d <= 512) launch<T, 32, 16, VEC, false>(a, warps, s);
-  else if (d <= 1024) launch<T, 32, 32, VEC, false>(a, warps, s);
-  else if (d <= 2048) launch<T, 128, 16, VEC, false>(a, rows, s);
-  else if (d <= 4096) launch<T, 256, 16, VEC, false>(a, rows, s);
-  else if (d <= 8192) launch<T, 256, 32, VEC, false>(a, rows, s);
-  else launch<T, 512, 32, VEC, false>(a, rows, s);
+template <typename T, int TPR, int NT, int E, int MODE, bool BWD>
+void launch(const NormArgs &a, const Layout &l, cudaStream_t s) {
+  const int smem = MODE >= 2 ? l.ring.bytes(NT / TPR) : 0;
+  auto go = [&](auto *kernel) {
+    if (smem) CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    kernel<<<l.grid, NT, smem, s>>>(a, l.ring);
+    CUDA_LAUNCH_CHECK();
+  };
+  if constexpr (!BWD) go(k_norm_fwd<T, TPR, NT, E, MODE>);
+  else if (a.hb) go(k_norm_bwd<T, TPR, NT, E, MODE, true>);
+  else go(k_norm_bwd<T, TPR, NT, E, MODE, false>);
 }
-template <typename T, bool VEC>
-void bwd(const NormArgs &a, cudaStream_t s) {
-  const int d = a.d, grid = bwd_grid(a.M, a.d);
-  if (d <= 256) launch<T, 32, 8, VEC, true>(a, grid, s);
-  else if (d <= 512) launch<T, 32, 16, VEC, true>(a, grid, s);
-  else if (d <= 1024) launch<T, 128, 8, VEC, true>(a, grid, s);
-  else if (d <= 2048) launch<T, 256, 8, VEC, true>(a, grid, s);
-  else if (d <= 4096) launch<T, 512, 8, VEC, true>(a, grid, s);
-  else if (d <= 8192) launch<T, 1024, 8, VEC, true>(a, grid, s);
-  else launch<T, 1024, 16, VEC, true>(a, grid, s);
+template <typename T, int TPR, int NT, int E, bool BWD>
+void by_feed(const NormArgs &a, const Layout &l, bool vec, cudaStream_t s) {
+  if (l.ring.stages && a.d == TPR * E) launch<T, TPR, NT, E, 3, BWD>(a, l, s);
+  else if (l.ring.stages) launch<T, TPR, NT, E, 2, BWD>(a, l, s);
+  else if (vec) launch<T, TPR, NT, E, 1, BWD>(a, l, s);
+  else launch<T, TPR, NT, E, 0, BWD>(a, l, s);
+}
+template <typename T, bool BWD>
+void by_width(const NormArgs &a, const Layout &l, bool vec, cudaStream_t s) {
+  constexpr int E = sizeof(T) == 4 ? 8 : 16, NT = sizeof(T) == 4 ? 512 : 256;
+  switch (l.tpr) {
+    case 32: by_feed<T, 32, NT, E, BWD>(a, l, vec, s); break;
+    case 64: by_feed<T, 64, NT, E, BWD>(a, l, vec, s); break;
+    case 128: by_feed<T, 128, NT, E, BWD>(a, l, vec, s); break;
+    case 256: by_feed<T, 256, NT, E, BWD>(a, l, vec, s); break;
+    case 512: by_feed<T, 512, 512, E, BWD>(a, l, vec, s); break;
+    default: by_feed<T, 1024, 1024, 16, BWD>(a, l, vec, s); break;  // up to 16,384
+  }
 }
 template <bool BWD>
-void by_type(int dt, bool vec, const NormArgs &a, cudaStream_t s) {
-  auto go = [&](auto tag, auto v) {
-    using T = decltype(tag);
-    if constexpr (BWD) bwd<T, decltype(v)::value != 0>(a, s);
-    else fwd<T, decltype(v)::value != 0>(a, s);
-  };
-  if (dt == DT_F32) vec ? go(float{}, Const<1>{}) : go(float{}, Const<0>{});
-  else if (dt == DT_F16) vec ? go(__half{}, Const<1>{}) : go(__half{}, Const<0>{});
-  else vec ? go(__nv_bfloat16{}, Const<1>{}) : go(__nv_bfloat16{}, Const<0>{});
+void by_type(int dt, bool vec, const NormArgs &a, const Layout &l, cudaStream_t s) {
+  if (dt == DT_F32) by_width<float, BWD>(a, l, vec, s);
+  else if (dt == DT_F16) by_width<__half, BWD>(a, l, vec, s);
+  else by_width<__nv_bfloat16, BWD>(a, l, vec, s);
 }
 
 // Every tensor of the call can move in 16-byte pieces.
@@ -537,27 +753,18 @@ void residual_norm_fwd(const ResidualNorm &a, Workspace &ws, cudaStream_t s) {
     if (a.dtype != DT_F32 || !vec || a.d % 128) throw Error(kErrInternal, "residual_norm: split output needs aligned f32 rows");
     n.split = *a.out_split;
   }
-  by_type<false>(a.dtype, vec, n, s);
+  by_type<false>(a.dtype, vec, n, layout_of(n, a.dtype, vec, false), s);
 }
 
 void residual_norm_bwd(const ResidualNorm &a, Workspace &ws, cudaStream_t s) {
-  // the vectors' gradients, in the order of NormArgs::want
-  void *const grads[5] = {a.dw, a.db, a.dpw, a.dpb, a.dgate.p && a.gate.ld == 0 ? a.dgate.p : nullptr};
+  void *const dgate = a.gate.ld == 0 ? a.dgate.p : nullptr;  // of one row
   if (a.M == 0) {
-    for (void *g : grads)
+    for (void *g : {a.dw, a.db, a.dpw, a.dpb, dgate})
       if (g && !ws.sizing()) CUDA_CHECK(cudaMemsetAsync(g, 0, a.d * dtype_size(a.dtype), s));
     return;
   }
   NormArgs n = args_of(a);
-  int count = 0;
-  for (int v = 0; v < 5; ++v)
-    if (grads[v]) {
-      n.want |= 1 << v;
-      ++count;
-    }
-  const int grid = bwd_grid(a.M, a.d);
-  if (count) n.part = static_cast<float *>(ws.take(4 * static_cast<size_t>(count) * grid * a.d));
-  if (ws.sizing()) return;
+  n.hb = a.pb || a.db || a.dpb;
   n.ds = a.dstream.p;
   n.ldds = a.dstream.ld;
   n.dout = a.dout.p;
@@ -570,13 +777,16 @@ void residual_norm_bwd(const ResidualNorm &a, Workspace &ws, cudaStream_t s) {
     n.dgate = a.dgate.p;
     n.lddg = a.dgate.ld;
   }
-  by_type<true>(a.dtype, vectorised(a), n, s);
-  int slot = 0;
-  for (int v = 0; v < 5; ++v)
-    if (grads[v]) {
-      column_join(n.part + static_cast<size_t>(slot) * grid * a.d, grid, a.d, 1.f, grads[v], a.dtype, s);
-      ++slot;
-    }
+  const bool vec = vectorised(a), vectors = a.dw || a.db || a.dpw || a.dpb || dgate;
+  const Layout l = layout_of(n, a.dtype, vec, true);
+  if (vectors) n.part = static_cast<float *>(ws.take(4 * static_cast<size_t>(n.hb ? 4 : 2) * l.grid * a.d));
+  if (ws.sizing()) return;
+  by_type<true>(a.dtype, vec, n, l, s);
+  if (!vectors) return;
+  const VectorGrads v{n.part, l.grid, a.d, a.dtype, n.hb, a.pw, a.pb, a.gate.ld == 0 ? a.gate.p : nullptr,
+                      a.dw, a.db, a.dpw, a.dpb, dgate};
+  k_norm_vectors<<<ceil_div(a.d, 32), 256, 0, s>>>(v);
+  CUDA_LAUNCH_CHECK();
 }
 
 }  // namespace pet

@@ -23,7 +23,7 @@ precision and limits; a refused call raises MLIPError.
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 from collections import namedtuple
 
 import torch
@@ -35,34 +35,12 @@ ACTIVATIONS = ("identity", "sigmoid", "silu", "gelu", "gelu_tanh", "relu")
 NORMS = ("none", "rms", "layer")
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_vp, _i32, _i64, _f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
-
-
-def _fields(spec: str, kind):
-    return [(name, kind) for name in spec.split()]
-
-
-class _GatedLinear(ctypes.Structure):
-    _fields_ = (_fields("dtype activation", _i32) + _fields("rows in_features hidden", _i64)
-                + _fields("x w_gate w_value b_gate b_value", _vp) + _fields("ldx ldw_gate ldw_value", _i64)
-                + [("h", _vp), ("ldh", _i64), ("dh", _vp), ("lddh", _i64)]
-                + _fields("dx dw_gate dw_value db_gate db_value", _vp) + _fields("lddx lddw_gate lddw_value", _i64))
-
-
-class _Linear(ctypes.Structure):
-    _fields_ = (_fields("dtype activation", _i32) + _fields("rows in_features out_features", _i64)
-                + [("scale", _f32)] + _fields("x w b residual", _vp) + _fields("ldx ldw ldresidual", _i64)
-                + [("y", _vp), ("ldy", _i64), ("dy", _vp), ("lddy", _i64)]
-                + _fields("dx dw db", _vp) + _fields("lddx lddw", _i64))
-
-
-class _ResidualNorm(ctypes.Structure):
-    _fields_ = (_fields("dtype norm post_norm", _i32) + _fields("rows features", _i64) + _fields("scale eps", _f32)
-                + _fields("residual y weight bias post_weight post_bias gate", _vp)
-                + _fields("ldresidual ldy ldgate", _i64) + _fields("stream out", _vp) + _fields("ldstream ldout", _i64)
-                + _fields("dstream dout", _vp) + _fields("lddstream lddout", _i64)
-                + _fields("dresidual dy dweight dbias dpost_weight dpost_bias dgate", _vp)
-                + _fields("lddresidual lddy lddgate", _i64))
+# the C structures' layouts (native alignment), filled in the order of their
+# fields: int32 i, int64 and pointers q, float f.  A small call is mostly host
+# time, and packing costs a third of what a ctypes.Structure does.
+_GATED = struct.Struct("2i 3q 5q 3q 2q 2q 5q 3q")
+_LINEAR = struct.Struct("2i 3q f 4q 3q 2q 2q 3q 2q")
+_NORM = struct.Struct("3i 2q 2f 7q 3q 2q 2q 2q 2q 7q 3q")
 
 
 def _refuse(message: str):
@@ -70,90 +48,101 @@ def _refuse(message: str):
 
 
 def _index(name, names, what: str) -> int:
-    name = names[0] if name is None else name
+    if name is None:
+        return 0
     if name not in names:
         _refuse(f"{what} must be one of {', '.join(names)} (got {name!r})")
     return names.index(name)
 
 
-def _same(first: torch.Tensor, **others):
-    """Refuses tensors of another type or device than `first`."""
-    if first.dtype not in _DTYPES:
-        _refuse(f"the type must be float32, float16 or bfloat16 (got {first.dtype})")
-    if not first.is_cuda:
+def _dtype(t: torch.Tensor) -> int:
+    """The C type of a call's first tensor."""
+    dt = _DTYPES.get(t.dtype)
+    if dt is None:
+        _refuse(f"the type must be float32, float16 or bfloat16 (got {t.dtype})")
+    if not t.is_cuda:
         _refuse("the tensors must be on a CUDA device (this backend has no CPU fallback)")
-    for name, t in others.items():
-        if t is not None and (t.dtype != first.dtype or t.device != first.device):
-            _refuse(f"{name} is {t.dtype} on {t.device}, expected {first.dtype} on {first.device}")
+    return dt
 
 
-def _shape(t, name: str, shape):
-    if t is not None and tuple(t.shape) != tuple(shape):
-        _refuse(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-
-
-def _rows(t: torch.Tensor | None, cols: int):
-    """`t` as a [rows, cols] matrix with contiguous rows."""
+def _take(t, first, shape, cols: int, keep: list, name: str):
+    """(address, row stride) of `t`, a tensor of `shape` with rows of `cols`
+    elements and of the type and device of `first`; (0, cols) for None.  What
+    had to be copied is appended to `keep`."""
     if t is None:
-        return None
-    t = t.detach().reshape(-1, cols) if t.dim() != 2 else t.detach()
+        return 0, cols
+    if t.dtype is not first.dtype or t.get_device() != first.get_device():
+        _refuse(f"{name} is {t.dtype} on {t.device}, expected {first.dtype} on {first.device}")
+    if t.shape != shape:
+        _refuse(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.is_contiguous():
+        return t.data_ptr(), cols
+    t = t.detach()
+    if t.dim() != 2:
+        t = t.reshape(-1, cols)
     if t.shape[0] > 1 and t.stride(0) < cols or cols > 1 and t.stride(1) != 1:
         t = t.contiguous()
-    return t
+    keep.append(t)
+    return t.data_ptr(), max(t.stride(0), cols)
 
 
-def _vec(t: torch.Tensor | None):
-    return None if t is None else t.detach().contiguous()
-
-
-def _p(t: torch.Tensor | None):
-    return None if t is None else t.data_ptr()
-
-
-def _ld(t: torch.Tensor | None) -> int:
-    return 0 if t is None else t.stride(0)
-
-
-def _call(name: str, args, device: torch.device, backward: bool):
+def _call(name: str, args: bytes, index: int, backward: bool):
     """One operator on the device's current stream, with its workspace."""
-    if torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device):
-            return _call(name, args, device, backward)
-    L, ref = lib(), ctypes.byref(args)
-    need = getattr(L, name + "_workspace")(ref, backward)
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return _call(name, args, index, backward)
+    forms = _FORMS.get(name)
+    if forms is None:
+        L = lib()
+        forms = _FORMS[name] = tuple(getattr(L, f"mlipcpp_b200_{name}{end}") for end in
+                                     ("_workspace", "", "_backward"))
+    need = forms[0](args, backward)
     if need < 0:
         _check(-need)
-    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    _check(getattr(L, name + "_backward" if backward else name)(
-        ref, _p(ws), need, torch.cuda.current_stream(device).cuda_stream))
+    ws = torch.empty(need, dtype=torch.uint8, device=index) if need else None
+    code = forms[2 if backward else 1](args, ws.data_ptr() if need else 0, need,
+                                       torch._C._cuda_getCurrentRawStream(index))
+    if code:
+        _check(code)
+
+
+_FORMS: dict = {}
 
 
 def _recorded(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    return any(t is not None and t.requires_grad for t in tensors)
+
+
+def _grads(inputs, needs):
+    """Uninitialised gradients of the inputs that are there and needed, and
+    their addresses."""
+    out = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and need else None
+                for t, need in zip(inputs, needs))
+    return out, [0 if t is None else t.data_ptr() for t in out]
 
 
 # ---------------------------------------------------------------------------
 # gated_linear
 # ---------------------------------------------------------------------------
-def _gated_args(x, w_gate, w_value, b_gate, b_value, activation):
+def _gated_inputs(x, w_gate, w_value, b_gate, b_value, activation, keep):
+    """(rows, K, F, the leading fields of the C structure)."""
     act = _index(activation, ACTIVATIONS, "activation")
-    if w_gate.dim() != 2 or x.dim() < 1:
-        _refuse("w_gate must have two dimensions and x at least one")
+    dt = _dtype(x)
+    if w_gate.dim() != 2 or x.dim() < 1 or x.shape[-1] != w_gate.shape[1]:
+        _refuse(f"x {tuple(x.shape)} and w_gate {tuple(w_gate.shape)} do not fit: expected [..., K] and [F, K]")
     f, k = w_gate.shape
-    _same(x, w_gate=w_gate, w_value=w_value, b_gate=b_gate, b_value=b_value)
-    _shape(w_value, "w_value", (f, k))
-    _shape(b_gate, "b_gate", (f,))
-    _shape(b_value, "b_value", (f,))
-    if x.shape[-1] != k:
-        _refuse(f"x has {x.shape[-1]} features, expected {k}")
-    keep = (_rows(x, k), _rows(w_gate, k), _rows(w_value, k), _vec(b_gate), _vec(b_value))
-    a = _GatedLinear(dtype=_DTYPES[x.dtype], activation=act, rows=keep[0].shape[0], in_features=k, hidden=f,
-                     x=_p(keep[0]), w_gate=_p(keep[1]), w_value=_p(keep[2]), b_gate=_p(keep[3]), b_value=_p(keep[4]),
-                     ldx=_ld(keep[0]), ldw_gate=_ld(keep[1]), ldw_value=_ld(keep[2]))
-    return a, keep
+    if k < 1 or f < 1:
+        _refuse("there must be at least one feature")
+    px, lx = _take(x, x, x.shape, k, keep, "x")
+    pg, lg = _take(w_gate, x, w_gate.shape, k, keep, "w_gate")
+    pv, lv = _take(w_value, x, w_gate.shape, k, keep, "w_value")
+    pbg, _ = _take(b_gate, x, (f,), f, keep, "b_gate")
+    pbv, _ = _take(b_value, x, (f,), f, keep, "b_value")
+    m = x.numel() // k
+    return m, k, f, (dt, act, m, k, f, px, pg, pv, pbg, pbv, lx, lg, lv)
 
 
-class _GatedLinearFn(torch.autograd.Function):
+class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_value, b_gate, b_value, activation):
         ctx.save_for_backward(x, w_gate, w_value, b_gate, b_value)
@@ -170,12 +159,12 @@ def gated_linear(x, w_gate, w_value, b_gate=None, b_value=None, activation="silu
     """act(x w_gate^T + b_gate) * (x w_value^T + b_value): x [..., K], weights
     [F, K], biases [F] -> [..., F].  Both projections, the activation and the
     product are one kernel."""
-    if _recorded(x, w_gate, w_value, b_gate, b_value):
-        return _GatedLinearFn.apply(x, w_gate, w_value, b_gate, b_value, activation)
-    a, keep = _gated_args(x, w_gate, w_value, b_gate, b_value, activation)
-    h = torch.empty(x.shape[:-1] + (a.hidden,), dtype=x.dtype, device=x.device)
-    a.h, a.ldh = h.data_ptr(), a.hidden
-    _call("mlipcpp_b200_gated_linear", a, x.device, False)
+    if torch.is_grad_enabled() and _recorded(x, w_gate, w_value, b_gate, b_value):
+        return _GatedLinear.apply(x, w_gate, w_value, b_gate, b_value, activation)
+    keep: list = []
+    m, k, f, fields = _gated_inputs(x, w_gate, w_value, b_gate, b_value, activation, keep)
+    h = torch.empty(x.shape[:-1] + (f,), dtype=x.dtype, device=x.device)
+    _call("gated_linear", _GATED.pack(*fields, h.data_ptr(), f, 0, f, 0, 0, 0, 0, 0, k, k, k), x.get_device(), False)
     return h
 
 
@@ -183,38 +172,34 @@ def gated_linear_backward(dh, x, w_gate, w_value, b_gate=None, b_value=None, act
     """(dx, dw_gate, dw_value, db_gate, db_value) for the gradient dh [..., F]
     of gated_linear's result; None for those not in `needs` and for biases
     that are not there."""
-    a, keep = _gated_args(x, w_gate, w_value, b_gate, b_value, activation)
-    _same(x, dh=dh)
-    _shape(dh, "dh", x.shape[:-1] + (a.hidden,))
-    m = _rows(dh, a.hidden)
-    a.dh, a.lddh = _p(m), _ld(m)
-    out = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and need else None
-           for t, need in zip((x, w_gate, w_value, b_gate, b_value), needs)]
-    a.dx, a.dw_gate, a.dw_value, a.db_gate, a.db_value = (_p(t) for t in out)
-    a.lddx = a.lddw_gate = a.lddw_value = a.in_features
-    _call("mlipcpp_b200_gated_linear", a, x.device, True)
-    return tuple(out)
+    keep: list = []
+    m, k, f, fields = _gated_inputs(x, w_gate, w_value, b_gate, b_value, activation, keep)
+    pd, ld = _take(dh, x, x.shape[:-1] + (f,), f, keep, "dh")
+    out, at = _grads((x, w_gate, w_value, b_gate, b_value), needs)
+    _call("gated_linear", _GATED.pack(*fields, 0, f, pd, ld, *at, k, k, k), x.get_device(), True)
+    return out
 
 
 # ---------------------------------------------------------------------------
 # linear
 # ---------------------------------------------------------------------------
-def _linear_args(x, w, bias, activation, scale):
+def _linear_inputs(x, w, bias, activation, residual, scale, keep):
     act = _index(activation, ACTIVATIONS, "activation")
-    if w.dim() != 2 or x.dim() < 1:
-        _refuse("w must have two dimensions and x at least one")
+    dt = _dtype(x)
+    if w.dim() != 2 or x.dim() < 1 or x.shape[-1] != w.shape[1]:
+        _refuse(f"x {tuple(x.shape)} and w {tuple(w.shape)} do not fit: expected [..., K] and [N, K]")
     n, k = w.shape
-    _same(x, w=w, bias=bias)
-    _shape(bias, "bias", (n,))
-    if x.shape[-1] != k:
-        _refuse(f"x has {x.shape[-1]} features, expected {k}")
-    keep = (_rows(x, k), _rows(w, k), _vec(bias))
-    a = _Linear(dtype=_DTYPES[x.dtype], activation=act, rows=keep[0].shape[0], in_features=k, out_features=n,
-                scale=scale, x=_p(keep[0]), w=_p(keep[1]), b=_p(keep[2]), ldx=_ld(keep[0]), ldw=_ld(keep[1]))
-    return a, keep
+    if k < 1 or n < 1:
+        _refuse("there must be at least one feature")
+    px, lx = _take(x, x, x.shape, k, keep, "x")
+    pw, lw = _take(w, x, w.shape, k, keep, "w")
+    pb, _ = _take(bias, x, (n,), n, keep, "bias")
+    pr, lr = _take(residual, x, x.shape[:-1] + (n,), n, keep, "residual")
+    m = x.numel() // k
+    return m, k, n, (dt, act, m, k, n, scale, px, pw, pb, pr, lx, lw, lr)
 
 
-class _LinearFn(torch.autograd.Function):
+class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, activation, residual, scale):
         ctx.save_for_backward(x, w, bias)
@@ -231,17 +216,12 @@ class _LinearFn(torch.autograd.Function):
 def linear(x, w, bias=None, activation="identity", residual=None, scale=1.0):
     """residual + scale act(x w^T + bias): x [..., K], w [N, K], bias [N],
     residual [..., N] -> [..., N], in one kernel."""
-    if _recorded(x, w, bias, residual):
-        return _LinearFn.apply(x, w, bias, activation, residual, scale)
-    a, keep = _linear_args(x, w, bias, activation, scale)
-    shape = x.shape[:-1] + (a.out_features,)
-    _same(x, residual=residual)
-    _shape(residual, "residual", shape)
-    r = _rows(residual, a.out_features)
-    a.residual, a.ldresidual = _p(r), _ld(r)
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    a.y, a.ldy = y.data_ptr(), a.out_features
-    _call("mlipcpp_b200_linear", a, x.device, False)
+    if torch.is_grad_enabled() and _recorded(x, w, bias, residual):
+        return _Linear.apply(x, w, bias, activation, residual, scale)
+    keep: list = []
+    m, k, n, fields = _linear_inputs(x, w, bias, activation, residual, scale, keep)
+    y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
+    _call("linear", _LINEAR.pack(*fields, y.data_ptr(), n, 0, n, 0, 0, 0, k, k), x.get_device(), False)
     return y
 
 
@@ -249,17 +229,12 @@ def linear_backward(dy, x, w, bias=None, activation="identity", scale=1.0, needs
     """(dx, dw, dbias) for the gradient dy [..., N] of linear's result (the
     residual's gradient is dy itself); None for those not in `needs` and for
     a bias that is not there."""
-    a, keep = _linear_args(x, w, bias, activation, scale)
-    _same(x, dy=dy)
-    _shape(dy, "dy", x.shape[:-1] + (a.out_features,))
-    m = _rows(dy, a.out_features)
-    a.dy, a.lddy = _p(m), _ld(m)
-    out = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and need else None
-           for t, need in zip((x, w, bias), needs)]
-    a.dx, a.dw, a.db = (_p(t) for t in out)
-    a.lddx = a.lddw = a.in_features
-    _call("mlipcpp_b200_linear", a, x.device, True)
-    return tuple(out)
+    keep: list = []
+    m, k, n, fields = _linear_inputs(x, w, bias, activation, None, scale, keep)
+    pd, ld = _take(dy, x, x.shape[:-1] + (n,), n, keep, "dy")
+    out, at = _grads((x, w, bias), needs)
+    _call("linear", _LINEAR.pack(*fields, 0, n, pd, ld, *at, k, k), x.get_device(), True)
+    return out
 
 
 # ---------------------------------------------------------------------------
@@ -268,29 +243,26 @@ def linear_backward(dy, x, w, bias=None, activation="identity", scale=1.0, needs
 ResidualNormGrads = namedtuple("ResidualNormGrads", "residual y weight bias post_weight post_bias gate")
 
 
-def _norm_args(residual, y, weight, bias, post_weight, post_bias, gate, scale, norm, post_norm, eps):
+def _norm_inputs(residual, y, weight, bias, post_weight, post_bias, gate, scale, norm, post_norm, eps, keep):
     kinds = _index(norm, NORMS, "norm"), _index(post_norm, NORMS, "post_norm")
-    if residual.dim() < 1:
-        _refuse("residual must have at least one dimension")
-    d = residual.shape[-1]
-    _same(residual, y=y, weight=weight, bias=bias, post_weight=post_weight, post_bias=post_bias, gate=gate)
-    _shape(y, "y", residual.shape)
-    for name, t in (("weight", weight), ("bias", bias), ("post_weight", post_weight), ("post_bias", post_bias)):
-        _shape(t, name, (d,))
-    if gate is not None and tuple(gate.shape) not in ((d,), tuple(residual.shape)):
-        _refuse(f"gate has shape {tuple(gate.shape)}, expected {(d,)} or {tuple(residual.shape)}")
+    dt = _dtype(residual)
+    if residual.dim() < 1 or residual.shape[-1] < 1:
+        _refuse("residual must have at least one dimension and one feature")
+    shape, d = residual.shape, residual.shape[-1]
+    if y is None and (kinds[1] or gate is not None):
+        _refuse("a post norm or a gate needs y")
+    pr, lr = _take(residual, residual, shape, d, keep, "residual")
+    py, ly = _take(y, residual, shape, d, keep, "y")
+    vec = [_take(t, residual, (d,), d, keep, name)[0]
+           for name, t in (("weight", weight), ("bias", bias), ("post_weight", post_weight), ("post_bias", post_bias))]
     channel = gate is not None and gate.dim() == 1
-    keep = (_rows(residual, d), _rows(y, d), _vec(weight), _vec(bias), _vec(post_weight), _vec(post_bias),
-            _vec(gate) if channel else _rows(gate, d))
-    r, ym, g = keep[0], keep[1], keep[6]
-    a = _ResidualNorm(dtype=_DTYPES[r.dtype], norm=kinds[0], post_norm=kinds[1], rows=r.shape[0], features=d,
-                      scale=scale, eps=eps, residual=_p(r), y=_p(ym), weight=_p(keep[2]), bias=_p(keep[3]),
-                      post_weight=_p(keep[4]), post_bias=_p(keep[5]), gate=_p(g), ldresidual=_ld(r), ldy=_ld(ym),
-                      ldgate=0 if channel or g is None else max(g.stride(0), d))
-    return a, keep
+    pg, lg = _take(gate, residual, (d,) if channel else shape, d, keep, "gate")
+    if channel or gate is None:
+        lg = 0
+    return d, (dt, *kinds, residual.numel() // d, d, scale, eps, pr, py, *vec, pg, lr, ly, lg)
 
 
-class _ResidualNormFn(torch.autograd.Function):
+class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, residual, y, weight, bias, post_weight, post_bias, gate, *how):
         ctx.save_for_backward(residual, y, weight, bias, post_weight, post_bias, gate)
@@ -313,14 +285,15 @@ def residual_norm(residual, y=None, weight=None, bias=None, post_weight=None, po
     norm(stream), over the last dimension (at most 16384): norms "none", "rms"
     or "layer" with optional weight and bias, a gate [d] for all rows or one
     of the residual's shape.  y None: stream = scale residual."""
-    if _recorded(residual, y, weight, bias, post_weight, post_bias, gate):
-        return _ResidualNormFn.apply(residual, y, weight, bias, post_weight, post_bias, gate, scale, norm, post_norm,
-                                     eps)
-    a, keep = _norm_args(residual, y, weight, bias, post_weight, post_bias, gate, scale, norm, post_norm, eps)
+    if torch.is_grad_enabled() and _recorded(residual, y, weight, bias, post_weight, post_bias, gate):
+        return _ResidualNorm.apply(residual, y, weight, bias, post_weight, post_bias, gate, scale, norm, post_norm,
+                                   eps)
+    keep: list = []
+    d, fields = _norm_inputs(residual, y, weight, bias, post_weight, post_bias, gate, scale, norm, post_norm, eps, keep)
     stream = torch.empty(residual.shape, dtype=residual.dtype, device=residual.device)
     out = torch.empty_like(stream)
-    a.stream, a.out, a.ldstream, a.ldout = stream.data_ptr(), out.data_ptr(), a.features, a.features
-    _call("mlipcpp_b200_residual_norm", a, residual.device, False)
+    _call("residual_norm", _NORM.pack(*fields, stream.data_ptr(), out.data_ptr(), d, d, 0, 0, d, d,
+                                      0, 0, 0, 0, 0, 0, 0, d, d, d), residual.get_device(), False)
     return stream, out
 
 
@@ -328,19 +301,13 @@ def residual_norm_backward(dstream, dout, residual, y=None, weight=None, bias=No
                            gate=None, scale=1.0, norm="rms", post_norm="none", eps=1e-5, needs=(True,) * 7):
     """ResidualNormGrads for the gradients of residual_norm's two results
     (either may be None); None for inputs not in `needs` or not there."""
-    a, keep = _norm_args(residual, y, weight, bias, post_weight, post_bias, gate, scale, norm, post_norm, eps)
-    _same(residual, dstream=dstream, dout=dout)
-    _shape(dstream, "dstream", residual.shape)
-    _shape(dout, "dout", residual.shape)
-    d = a.features
-    ms, mo = _rows(dstream, d), _rows(dout, d)
-    a.dstream, a.dout, a.lddstream, a.lddout = _p(ms), _p(mo), _ld(ms), _ld(mo)
-    g = ResidualNormGrads(*(torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and need else None
-                            for t, need in zip((residual, y, weight, bias, post_weight, post_bias, gate), needs)))
-    a.dresidual, a.dy, a.dweight, a.dbias, a.dpost_weight, a.dpost_bias, a.dgate = (_p(t) for t in g)
-    a.lddresidual = a.lddy = a.lddgate = d
-    _call("mlipcpp_b200_residual_norm", a, residual.device, True)
-    return g
+    keep: list = []
+    d, fields = _norm_inputs(residual, y, weight, bias, post_weight, post_bias, gate, scale, norm, post_norm, eps, keep)
+    ps, ls = _take(dstream, residual, residual.shape, d, keep, "dstream")
+    po, lo = _take(dout, residual, residual.shape, d, keep, "dout")
+    out, at = _grads((residual, y, weight, bias, post_weight, post_bias, gate), needs)
+    _call("residual_norm", _NORM.pack(*fields, 0, 0, d, d, ps, po, ls, lo, *at, d, d, d), residual.get_device(), True)
+    return ResidualNormGrads(*out)
 
 
 def check_status(device=None):
