@@ -52,32 +52,27 @@ __device__ __forceinline__ uint4 pack(const float (&v)[16 / sizeof(T)]) {
   return u;
 }
 
-// 1 / (1 + e^-z).  kFast (16-bit results): the intrinsics, a few ulp of fp32,
-// far below the result's half step.  The exponent's argument stops at -80,
-// where the result is below 2e-35, so that e^-z stays finite.
-template <bool kFast>
-__device__ __forceinline__ float logistic(float z) {
-  const float t = fmaxf(z, -80.f);
-  return kFast ? __fdividef(1.f, 1.f + __expf(-t)) : 1.f / (1.f + expf(-t));
-}
+// 1 / (1 + e^-z) by the intrinsics: a few ulp of fp32, and 2^-23 |z| of
+// e^-z, which no result sees where |z| is large.  The exponent's argument stops
+// at -80, where the result is below 2e-35, so that e^-z stays finite.
+__device__ __forceinline__ float logistic(float z) { return __fdividef(1.f, 1.f + __expf(-fmaxf(z, -80.f))); }
 
 // a = act(z), da = act'(z)
-template <int ACT, bool kFast>
+template <int ACT>
 __device__ __forceinline__ void act_pair(float z, float &a, float &da) {
   if (ACT == ACT_SIGMOID) {
-    a = logistic<kFast>(z);
+    a = logistic(z);
     da = a * (1.f - a);
   } else if (ACT == ACT_SILU) {
-    const float p = logistic<kFast>(z);
+    const float p = logistic(z);
     a = z * p;
     da = p * (1.f + z * (1.f - p));
   } else if (ACT == ACT_GELU) {
     const float c = normcdff(z);
     a = z * c;
-    const float e = kFast ? __expf(-0.5f * z * z) : expf(-0.5f * z * z);
-    da = c + z * e * 0.3989422804014327f;
+    da = c + z * __expf(-0.5f * z * z) * 0.3989422804014327f;
   } else if (ACT == ACT_GELU_TANH) {
-    const float p = logistic<kFast>(1.5957691216057308f * (z + 0.044715f * z * z * z));
+    const float p = logistic(1.5957691216057308f * (z + 0.044715f * z * z * z));
     a = z * p;
     da = p + z * p * (1.f - p) * 1.5957691216057308f * (1.f + 0.134145f * z * z);
   } else if (ACT == ACT_RELU) {
@@ -87,12 +82,6 @@ __device__ __forceinline__ void act_pair(float z, float &a, float &da) {
     a = z;
     da = 1.f;
   }
-}
-template <int ACT, bool kFast>
-__device__ __forceinline__ float act_only(float z) {
-  float a, da;
-  act_pair<ACT, kFast>(z, a, da);
-  return a;
 }
 template <int V>
 struct Const {

@@ -14,8 +14,9 @@
 //    the whole contraction; BN = 256 (one 128 x 256 tile, two accumulators)
 //    or 128 (four accumulators) when 256-wide tiles would leave SMs idle.
 //  * f32: A = 2^-s (hi + lo) with one scale per row and 128 contraction
-//    elements, B = 2^-t (hi + lo) with one scale per matrix (split16.cuh);
-//    A_lo B_hi + A_hi B_lo + A_hi B_hi per step.  The tensor core truncates
+//    elements, B = 2^-t (hi + lo) with one scale per 128 x 128 block (or one
+//    for all) in the way of split16.cuh; A_lo B_hi + A_hi B_lo + A_hi B_hi per
+//    step.  The tensor core truncates
 //    when it adds to its accumulator, so every 128 contraction elements the
 //    accumulator warps add the partial sum to fp32 registers with
 //    round-to-nearest.
@@ -53,7 +54,7 @@ constexpr int BM = 128, BK = 64;
 constexpr int kTile = BM * 128;  // bytes of 128 rows x 64 16-bit elements
 constexpr int kAccWarps = 8;
 constexpr int kThreads = 64 + 32 * kAccWarps;
-constexpr int kStageFloats = 32 * 33;  // staging of one accumulator warp
+constexpr int kStageFloats = 32 * 32;  // staging of one accumulator warp
 
 enum Epi : int { E_LINEAR = 0, E_LINEAR_BWD = 1, E_GATED = 2, E_GATED_BWD = 3, E_PARTIAL = 4 };
 
@@ -92,8 +93,9 @@ struct Params {
   int a_mn, b_mn, dual, bf16, products;
   const int8_t *sc[2];             // f32: scale exponents of A, [block][row]
   int64_t scld[2];
-  const float *bs[2];              // f32: 2^-t of B on the device, or null
-  float bsc[2];                    // ... else this
+  const int8_t *bs[2];             // f32: scale exponents of B's blocks, or null
+  int64_t bsn[2], bsk[2];          // ... their strides by 128 rows and 128 k
+  float bsc[2];                    // ... else this factor
   EpiArgs e;
 };
 
@@ -120,6 +122,26 @@ __device__ __forceinline__ uint64_t mn_desc(uint32_t start) {
          (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
+// Two blocks of 32 lanes x 32 consecutive fp32 columns -> 32 registers each;
+// the wait names every register, so no use of one can move before it.
+__device__ __forceinline__ void tmem_ld2x32(uint32_t ta, uint32_t tb, float (&a)[32], float (&b)[32]) {
+#define PET_R8(x, k) "=f"(x[k]), "=f"(x[k + 1]), "=f"(x[k + 2]), "=f"(x[k + 3]), "=f"(x[k + 4]), "=f"(x[k + 5]), "=f"(x[k + 6]), "=f"(x[k + 7])
+#define PET_LD32(x, addr)                                                                          \
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "                                           \
+               "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"                           \
+               "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"          \
+               : PET_R8(x, 0), PET_R8(x, 8), PET_R8(x, 16), PET_R8(x, 24)                          \
+               : "r"(addr))
+#define PET_W8(x, k) "+f"(x[k]), "+f"(x[k + 1]), "+f"(x[k + 2]), "+f"(x[k + 3]), "+f"(x[k + 4]), "+f"(x[k + 5]), "+f"(x[k + 6]), "+f"(x[k + 7])
+  PET_LD32(a, ta);
+  PET_LD32(b, tb);
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : PET_W8(a, 0), PET_W8(a, 8), PET_W8(a, 16), PET_W8(a, 24)::"memory");
+  asm volatile("" : PET_W8(b, 0), PET_W8(b, 8), PET_W8(b, 16), PET_W8(b, 24)::"memory");
+#undef PET_R8
+#undef PET_LD32
+#undef PET_W8
+}
+
 // One tile's coordinates from its number: groups of 8 row tiles, columns
 // outer and rows inner within a group, so that the CTAs at work at one time
 // share both operands' tiles in L2.
@@ -140,106 +162,145 @@ __device__ __forceinline__ Item item_of(const Params &p, int it) {
   return o;
 }
 
-// Staged 32 x 32 block -> rows row0.., columns col0.. of `out`, in 16-byte
-// pieces of a row per lane.  HOW: 0 plain, 1 adds `in`, 2 multiplies by `in`.
-template <typename T, int HOW>
-__device__ __forceinline__ void block_out(const float *st, int lane, int row0, int col0, int M, int N, const T *in,
-                                          int64_t ldin, bool vin, T *out, int64_t ldo, bool vout) {
-  constexpr int V = 16 / sizeof(T), L = 32 / V;  // elements a lane, lanes a row
-  if (vout && (HOW == 0 || vin)) {
-    const int c = (lane % L) * V;
+// One warp's 32 x 32 block of a tile, read from tensor memory a row a lane,
+// is turned through shared memory to the layout of its loads and stores: a
+// lane has V consecutive columns (16 bytes of T) of row i * 32 / L + lane / L,
+// i < L.  16-byte piece k of row r lies at place k ^ (r % 8), which keeps both
+// accesses free of bank conflicts.
+__device__ __forceinline__ float4 *piece(float *st, int r, int k) {
+  return reinterpret_cast<float4 *>(st + r * 32 + ((k ^ (r & 7)) << 2));
+}
+template <typename T>
+struct Turned {
+  static constexpr int V = 16 / static_cast<int>(sizeof(T)), L = 32 / V;
+  float x[L][V];
+  static __device__ __forceinline__ int row(int i, int lane) { return i * (32 / L) + lane / L; }
+  static __device__ __forceinline__ int col(int lane) { return (lane % L) * V; }
+  __device__ __forceinline__ void turn(float *st, int lane, const float (&v)[32]) {
+    __syncwarp();  // the block before has been read
 #pragma unroll
-    for (int r0 = 0; r0 < 32; r0 += 32 / L) {
-      const int r = r0 + lane / L, row = row0 + r, col = col0 + c;
-      if (row >= M || col >= N) continue;
-      float v[V];
+    for (int j = 0; j < 32; j += 4)
+      *piece(st, lane, j / 4) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+    __syncwarp();
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = st[r * 33 + c + j];
-      const size_t io = static_cast<size_t>(row) * ldin + col, oo = static_cast<size_t>(row) * ldo + col;
-      if (col + V <= N) {
-        if (HOW) {
-          float u[V];
-          unpack<T>(*reinterpret_cast<const uint4 *>(in + io), u);  // `in` may be `out`
+    for (int i = 0; i < L; ++i)
 #pragma unroll
-          for (int j = 0; j < V; ++j) v[j] = HOW == 1 ? v[j] + u[j] : v[j] * u[j];
-        }
-        *reinterpret_cast<uint4 *>(out + oo) = pack<T>(v);
+      for (int j = 0; j < V; j += 4) {
+        const float4 u = *piece(st, row(i, lane), (col(lane) + j) / 4);
+        x[i][j] = u.x;
+        x[i][j + 1] = u.y;
+        x[i][j + 2] = u.z;
+        x[i][j + 3] = u.w;
+      }
+  }
+  // V elements of a bias from column c on, zeros past N
+  static __device__ __forceinline__ void bias(const void *p, int c, int N, float (&b)[V]) {
+    const T *q = static_cast<const T *>(p) + c;
+#pragma unroll
+    for (int j = 0; j < V; ++j) b[j] = c + j < N ? to_f(__ldg(q + j)) : 0.f;
+  }
+};
+
+// The block's elements of the epilogue's input (residual or upstream
+// gradient), requested ahead of the accumulator they are combined with.
+template <typename T>
+struct Input {
+  using U = Turned<T>;
+  uint4 v[U::L];
+  __device__ __forceinline__ void fetch(const Params &p, int lane, int row0, int col0) {
+    const T *in = static_cast<const T *>(p.e.in);
+    const int c = col0 + U::col(lane);
+#pragma unroll
+    for (int i = 0; i < U::L; ++i) {
+      const int r = row0 + U::row(i, lane);
+      v[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (r >= p.M || c >= p.N) continue;
+      const T *q = in + static_cast<size_t>(r) * p.e.ldin + c;  // (`in` may be `out`: no read-only loads)
+      if (p.e.vin && c + U::V <= p.N) {
+        v[i] = *reinterpret_cast<const uint4 *>(q);
       } else {
+        T *t = reinterpret_cast<T *>(&v[i]);
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (col + j < N) {
-            const float u = HOW ? to_f(in[io + j]) : 0.f;
-            out[oo + j] = from_f<T>(HOW == 0 ? v[j] : HOW == 1 ? v[j] + u : v[j] * u);
-          }
+        for (int j = 0; j < U::V; ++j)
+          if (c + j < p.N) t[j] = q[j];
       }
     }
-  } else {
-    const int col = col0 + lane;
-    if (col < N)
-      for (int r = 0; r < 32 && row0 + r < M; ++r) {
-        const float v = st[r * 33 + lane];
-        const float u = HOW ? to_f(in[static_cast<size_t>(row0 + r) * ldin + col]) : 0.f;
-        out[static_cast<size_t>(row0 + r) * ldo + col] = from_f<T>(HOW == 0 ? v : HOW == 1 ? v + u : v * u);
-      }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void block_store(const Turned<T> &b, T *out, int64_t ldo, bool vec, int lane, int row0,
+                                            int col0, int M, int N) {
+  using U = Turned<T>;
+  const int c = col0 + U::col(lane);
+#pragma unroll
+  for (int i = 0; i < U::L; ++i) {
+    const int r = row0 + U::row(i, lane);
+    if (r >= M || c >= N) continue;
+    T *q = out + static_cast<size_t>(r) * ldo + c;
+    if (vec && c + U::V <= N) {
+      *reinterpret_cast<uint4 *>(q) = pack<T>(b.x[i]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < U::V; ++j)
+        if (c + j < N) q[j] = from_f<T>(b.x[i][j]);
+    }
   }
 }
 
-// One warp's 32 x 32 block of a tile through the epilogue.  v (and w, the
-// value half of the gated forms): this lane's row, 32 consecutive columns.
-template <int EPI, typename T, bool kFast>
+// The epilogue of one block: v (and w, the value half of the gated forms) as
+// they come from the accumulator, `in` from the rows' input.
+template <int EPI, typename T>
 __device__ __forceinline__ void epilogue(const Params &p, int batch, float *st, int lane, int row0, int col0,
-                                         float (&v)[32], float (&w)[32]) {
+                                         const float (&v)[32], const float (&w)[32], const Input<T> &in) {
+  using U = Turned<T>;
+  constexpr bool kDual = EPI == E_GATED || EPI == E_GATED_BWD;
   const EpiArgs &e = p.e;
-  const T *in = static_cast<const T *>(e.in);
-  T *out0 = static_cast<T *>(batch ? e.out1 : e.out0);
+  const int c = col0 + U::col(lane);
+  U a, b;
+  a.turn(st, lane, v);
+  if (kDual) b.turn(st, lane, w);
   if (e.b0) {
+    float f[U::V];
+    U::bias(e.b0, c, p.N, f);
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] += col0 + j < p.N ? to_f(__ldg(static_cast<const T *>(e.b0) + col0 + j)) : 0.f;
+    for (int i = 0; i < U::L; ++i)
+#pragma unroll
+      for (int j = 0; j < U::V; ++j) a.x[i][j] += f[j];
   }
-  if ((EPI == E_GATED || EPI == E_GATED_BWD) && e.b1) {
+  if (kDual && e.b1) {
+    float f[U::V];
+    U::bias(e.b1, c, p.N, f);
 #pragma unroll
-    for (int j = 0; j < 32; ++j) w[j] += col0 + j < p.N ? to_f(__ldg(static_cast<const T *>(e.b1) + col0 + j)) : 0.f;
+    for (int i = 0; i < U::L; ++i)
+#pragma unroll
+      for (int j = 0; j < U::V; ++j) b.x[i][j] += f[j];
   }
   with_act(e.act, [&](auto A) {
     constexpr int ACT = decltype(A)::value;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      if (EPI == E_LINEAR) {
-        v[j] = act_only<ACT, kFast>(v[j]) * e.scale;
-      } else if (EPI == E_GATED) {
-        v[j] = act_only<ACT, kFast>(v[j]) * w[j];
-      } else {
-        float a, da;
-        act_pair<ACT, kFast>(v[j], a, da);
-        if (EPI == E_LINEAR_BWD) {
-          v[j] = da * e.scale;
+    for (int i = 0; i < U::L; ++i) {
+      float u[U::V];
+      if (EPI == E_LINEAR || EPI == E_LINEAR_BWD || EPI == E_GATED_BWD) unpack<T>(in.v[i], u);
+#pragma unroll
+      for (int j = 0; j < U::V; ++j) {
+        float y, dy;
+        act_pair<ACT>(a.x[i][j], y, dy);
+        if (EPI == E_LINEAR) {
+          a.x[i][j] = fmaf(y, e.scale, u[j]);
+        } else if (EPI == E_GATED) {
+          a.x[i][j] = y * b.x[i][j];
+        } else if (EPI == E_LINEAR_BWD) {
+          a.x[i][j] = dy * e.scale * u[j];
         } else {
-          v[j] = da * w[j];
-          w[j] = a;
+          a.x[i][j] = dy * b.x[i][j] * u[j];
+          b.x[i][j] = y * u[j];
         }
       }
     }
   });
-  float *mine = st + lane * 33;
-#pragma unroll
-  for (int j = 0; j < 32; ++j) mine[j] = v[j];
-  __syncwarp();
-  if (EPI == E_LINEAR) {
-    if (in) block_out<T, 1>(st, lane, row0, col0, p.M, p.N, in, e.ldin, e.vin, out0, e.ldo, e.vout);
-    else block_out<T, 0>(st, lane, row0, col0, p.M, p.N, in, e.ldin, e.vin, out0, e.ldo, e.vout);
-  } else if (EPI == E_GATED) {
-    block_out<T, 0>(st, lane, row0, col0, p.M, p.N, in, e.ldin, e.vin, out0, e.ldo, e.vout);
-  } else {
-    block_out<T, 2>(st, lane, row0, col0, p.M, p.N, in, e.ldin, e.vin, out0, e.ldo, e.vout);
-  }
-  __syncwarp();
-  if (EPI == E_GATED_BWD) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) mine[j] = w[j];
-    __syncwarp();
-    block_out<T, 2>(st, lane, row0, col0, p.M, p.N, in, e.ldin, e.vin, static_cast<T *>(e.out1), e.ldo, e.vout);
-    __syncwarp();
-  }
+  block_store<T>(a, static_cast<T *>(batch ? e.out1 : e.out0), e.ldo, e.vout, lane, row0, col0, p.M, p.N);
+  if (EPI == E_GATED_BWD) block_store<T>(b, static_cast<T *>(e.out1), e.ldo, e.vout, lane, row0, col0, p.M, p.N);
 }
 
 template <bool F32, int BN, int EPI, typename T>
@@ -396,6 +457,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_block_gemm(const __grid_constan
       const int row0 = t.tm * BM + q * 32, row = row0 + lane, n0 = t.tn * out_n;
       const int k0 = t.split * p.kt_split, k_end = min(p.kt, k0 + p.kt_split);
       constexpr int GA = F32 ? G : 1;
+      // output columns a warp finishes, in blocks of 32; column of block i / 32
+      constexpr int kCols = kDual ? G : 2 * G;
+      constexpr bool kIn = EPI == E_LINEAR || EPI == E_LINEAR_BWD || EPI == E_GATED_BWD;
+      auto col_of = [&](int i) {
+        const int c = kDual ? h * G + i : cb[i / G] + i % G;
+        return n0 + c - ((EPI == E_PARTIAL && p.dual) ? h * (BN / 2) : 0);
+      };
+      Input<T> next;
+      if (kIn) {
+        if (p.e.in) {
+          next.fetch(p, lane, row0, col_of(0));
+        } else {
+#pragma unroll
+          for (int i = 0; i < Turned<T>::L; ++i) next.v[i] = make_uint4(0u, 0u, 0u, 0u);
+        }
+      }
       float acc[2][GA];  // f32: the running sums
       int b = 0;
       if (F32) {
@@ -403,30 +480,37 @@ __global__ void __launch_bounds__(kThreads, 1) k_block_gemm(const __grid_constan
         for (int gi = 0; gi < 2; ++gi)
 #pragma unroll
           for (int j = 0; j < GA; ++j) acc[gi][j] = 0.f;
-        for (int kt = k0; kt < k_end; kt += C::Chunk, ++pass) {
+        // 2^-(s + t) of this thread's row and each group's columns in one
+        // pass, requested a pass ahead
+        float sa_next, sb_next[2];
+        auto scales = [&](int kt) {
           const int seg = kt >= p.kt0 ? 1 : 0, o = t.batch | seg;
           const int blk = (kt - (seg ? p.kt0 : 0)) / C::Chunk;
-          const float sa = row < p.M ? pow2f(-static_cast<int>(p.sc[o][static_cast<size_t>(blk) * p.scld[o] + row])) : 0.f;
+          sa_next = row < p.M ? pow2f(-static_cast<int>(p.sc[o][static_cast<size_t>(blk) * p.scld[o] + row])) : 0.f;
+#pragma unroll
+          for (int gi = 0; gi < 2; ++gi) {
+            const int bi = p.dual ? (cb[gi] >= BN / 2 ? 1 : 0) : seg;
+            sb_next[gi] = p.bs[bi] ? pow2f(-static_cast<int>(__ldg(p.bs[bi] + (n0 / 128) * p.bsn[bi] + blk * p.bsk[bi]))) : p.bsc[bi];
+          }
+        };
+        scales(k0);
+        for (int kt = k0; kt < k_end; kt += C::Chunk, ++pass) {
+          const float f[2] = {sa_next * sb_next[0], sa_next * sb_next[1]};
+          if (kt + C::Chunk < k_end) scales(kt + C::Chunk);
           b = pass % C::Bufs;
           if (!__all_sync(0xffffffffu, wait_or_abort(accf0 + 8 * b, (pass / C::Bufs) & 1, abort_flag))) {
             ok = false;
             break;
           }
           tc_fence_after();
-#pragma unroll
-          for (int gi = 0; gi < 2; ++gi) {
-            const int bi = p.dual ? (cb[gi] >= BN / 2 ? 1 : 0) : seg;
-            const float f = sa * (p.bs[bi] ? __ldg(p.bs[bi]) : p.bsc[bi]);
-#pragma unroll
-            for (int c = 0; c < G; c += 32) {
-              float v[32];
-              tmem_ld32(tq + static_cast<uint32_t>(b * BN + cb[gi] + c), v);
-#pragma unroll
-              for (int j = 0; j < 32; ++j) acc[gi][F32 ? c + j : 0] = __fmaf_rn(v[j], f, acc[gi][F32 ? c + j : 0]);
-            }
-          }
+          float v[2][32];
+          tmem_ld2x32(tq + static_cast<uint32_t>(b * BN + cb[0]), tq + static_cast<uint32_t>(b * BN + cb[1]), v[0], v[1]);
           tc_fence_before();
           mbar_arrive(acce0 + 8 * b);
+#pragma unroll
+          for (int gi = 0; gi < 2; ++gi)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) acc[gi][F32 ? j : 0] = __fmaf_rn(v[gi][j], f[gi], acc[gi][F32 ? j : 0]);
         }
         if (!ok) break;
       } else {
@@ -446,35 +530,32 @@ __global__ void __launch_bounds__(kThreads, 1) k_block_gemm(const __grid_constan
           tmem_ld32(tq + static_cast<uint32_t>(b * BN + cb[gi] + c), v);
         }
       };
-      auto chunk = [&](int gi, int c) {
+      auto chunk = [&](int i) {
+        const int gi = i / G, c = i % G;
         float v[32], w[32];
         get(gi, c, v);
         if (kDual) get(1, c, w);
+        const int col = col_of(i);
         if (EPI == E_PARTIAL) {
-          const int half = p.dual ? h : 0;
-          const int col = n0 + cb[gi] + c - half * (BN / 2);
-          if (col >= p.N) return;
-          float *mine = st + lane * 33;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) mine[j] = v[j];
-          __syncwarp();
-          float *dst = p.e.part + (static_cast<size_t>(t.batch) * p.splits + t.split) * p.M * p.e.nacc + half * p.N;
-          block_out<float, 0>(st, lane, row0, col, p.M, p.N, nullptr, 0, true, dst, p.e.nacc, p.e.vout);
-          __syncwarp();
-        } else {
-          const int col = n0 + (kDual ? h * G : cb[gi]) + c;
           if (col >= p.N || row0 >= p.M) return;
-          epilogue<EPI, T, !F32>(p, t.batch, st, lane, row0, col, v, w);
+          Turned<float> o;
+          o.turn(st, lane, v);
+          float *dst = p.e.part + (static_cast<size_t>(t.batch) * p.splits + t.split) * p.M * p.e.nacc +
+                       (p.dual ? h * p.N : 0);
+          block_store<float>(o, dst, p.e.nacc, p.e.vout, lane, row0, col, p.M, p.N);
+        } else {
+          const Input<T> cur = next;
+          if (kIn && p.e.in && i + 32 < kCols) next.fetch(p, lane, row0, col_of(i + 32));
+          if (col >= p.N || row0 >= p.M) return;
+          epilogue<EPI, T>(p, t.batch, st, lane, row0, col, v, w, cur);
         }
       };
       if (F32) {  // register arrays: constant indices
 #pragma unroll
-        for (int gi = 0; gi < (kDual ? 1 : 2); ++gi)
-#pragma unroll
-          for (int c = 0; c < G; c += 32) chunk(gi, c);
+        for (int i = 0; i < kCols; i += 32) chunk(i);
       } else {
 #pragma unroll 1
-        for (int i = 0; i < (kDual ? 1 : 2) * G; i += 32) chunk(i / G, i % G);
+        for (int i = 0; i < kCols; i += 32) chunk(i);
         tc_fence_before();
         mbar_arrive(acce0 + 8 * b);
       }
@@ -518,9 +599,8 @@ __global__ void __launch_bounds__(256) k_join(const Params p) {
     T *o = static_cast<T *>(batch ? e.out1 : e.out0) + row * e.ldo + col;
     with_act(e.act, [&](auto A) {
       constexpr int ACT = decltype(A)::value;
-      constexpr bool kFast = sizeof(T) == 2;
       float a, da;
-      act_pair<ACT, kFast>(v, a, da);
+      act_pair<ACT>(v, a, da);
       if (EPI == E_LINEAR) *o = from_f<T>(a * e.scale + in);
       else if (EPI == E_LINEAR_BWD) *o = from_f<T>(da * e.scale * in);
       else if (EPI == E_GATED) *o = from_f<T>(a * w);
@@ -542,118 +622,136 @@ __device__ __forceinline__ float finite_abs(float x) {
   return a < INFINITY ? a : 0.f;
 }
 
-// f32 rows -> split form with one scale per row and 128 columns; warp per
-// (row, block).  Columns past C are written as zeros up to the block's end.
-__global__ void __launch_bounds__(256) k_split_rows(const float *__restrict__ src, int64_t ld, int R, int C, bool vec,
-                                                    Split16View o) {
-  const int nb = o.cols / 128, lane = threadIdx.x & 31;
-  const int64_t n = static_cast<int64_t>(R) * nb, step = static_cast<int64_t>(gridDim.x) * 8;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); i < n; i += step) {
-    const int row = static_cast<int>(i / nb), blk = static_cast<int>(i - static_cast<int64_t>(row) * nb);
-    const int c = blk * 128 + lane * 4;
-    const float *p = src + static_cast<size_t>(row) * ld + c;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (vec && c + 4 <= C) {
-      v = __ldg(reinterpret_cast<const float4 *>(p));
-    } else {
-      if (c < C) v.x = p[0];
-      if (c + 1 < C) v.y = p[1];
-      if (c + 2 < C) v.z = p[2];
-      if (c + 3 < C) v.w = p[3];
-    }
-    float mx = fmaxf(fmaxf(finite_abs(v.x), finite_abs(v.y)), fmaxf(finite_abs(v.z), finite_abs(v.w)));
-    const int s = split_scale_exponent(warp_max(mx));
-    const float f = pow2f(s);
-    uint32_t h0, h1, l0, l1;
-    split2(v.x, v.y, f, h0, l0);
-    split2(v.z, v.w, f, h1, l1);
-    const size_t off = static_cast<size_t>(row) * o.cols + c;
-    *reinterpret_cast<uint2 *>(o.hi + off) = make_uint2(h0, h1);
-    *reinterpret_cast<uint2 *>(o.lo + off) = make_uint2(l0, l1);
-    if (lane == 0) o.sc[static_cast<size_t>(blk) * split_ld(o) + row] = static_cast<int8_t>(s);
-  }
-}
-
-// f32 [R, C] -> split form in the same layout [R, cp] (cp a multiple of 64)
-// with one scale per column and 128 rows (scales [row block][column]): the A
-// operand of a product that contracts over rows.  CTA: 128 rows x 64 columns
-// at a time.
-__global__ void __launch_bounds__(256) k_split_cols(const float *__restrict__ src, int64_t ld, int R, int C,
-                                                    uint16_t *hi, uint16_t *lo, int cp, int8_t *sc) {
-  __shared__ float mx[8][64];
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.x * 64 + 2 * lane;
-  for (int blk = blockIdx.y; blk * 128 < R; blk += gridDim.y) {
-    const int r0 = blk * 128 + w * 16;
-    float a[16], b[16], ma = 0.f, mb = 0.f;
+// f32 matrices -> split-fp16 operands, all of a step in one launch; a CTA
+// takes a 128 x 128 block of one of them, reads it once into registers and
+// writes each form that a product needs of it:
+//   rows    one scale per row and 128 columns, [column block][row]
+//   cols    one scale per column and 128 rows, [row block][column]
+//   blocks  one scale per block, [row block][column block]
+// and, for bias gradients, the sums of its columns, [row block][column].
+// All forms are [R][lp] hi, then lo.
+struct SplitForm {
+  uint16_t *hi;
+  int8_t *sc;
+};
+struct SplitJob {
+  const float *src;
+  int64_t ld;
+  int R, C, lp, first;  // first: number of the job's first block
+  bool vec;
+  SplitForm rows, cols, blocks;
+  float *sums;
+};
+constexpr int kMaxJobs = 4;
+struct SplitJobs {
+  SplitJob job[kMaxJobs];
+  int n, total;
+};
+__global__ void __launch_bounds__(256) k_split(const SplitJobs all) {
+  __shared__ float part[8][128];
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int id = blockIdx.x; id < all.total; id += gridDim.x) {
+    int ji = 0;
+    while (ji + 1 < all.n && id >= all.job[ji + 1].first) ++ji;
+    const SplitJob &q = all.job[ji];
+    const int nb = (q.C + 127) / 128, rb = (id - q.first) / nb, cb = (id - q.first) % nb;
+    const int c = cb * 128 + 4 * lane, r0 = rb * 128 + w * 16;
+    float v[16][4];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const bool in = r0 + i < R;
-      const float *p = src + static_cast<size_t>(r0 + i) * ld + c;
-      a[i] = in && c < C ? p[0] : 0.f;
-      b[i] = in && c + 1 < C ? p[1] : 0.f;
-      ma = fmaxf(ma, finite_abs(a[i]));
-      mb = fmaxf(mb, finite_abs(b[i]));
-    }
-    __syncthreads();  // the last block's maxima have been read
-    mx[w][2 * lane] = ma;
-    mx[w][2 * lane + 1] = mb;
-    __syncthreads();
+      const float *p = q.src + static_cast<size_t>(r0 + i) * q.ld + c;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      ma = fmaxf(ma, mx[i][2 * lane]);
-      mb = fmaxf(mb, mx[i][2 * lane + 1]);
-    }
-    const int sa = split_scale_exponent(ma), sb = split_scale_exponent(mb);
-    if (w == 0) {
-      sc[static_cast<size_t>(blk) * cp + c] = static_cast<int8_t>(sa);
-      sc[static_cast<size_t>(blk) * cp + c + 1] = static_cast<int8_t>(sb);
-    }
-    const float fa = pow2f(sa), fb = pow2f(sb);
+      for (int j = 0; j < 4; ++j) v[i][j] = 0.f;
+      if (r0 + i >= q.R) continue;
+      if (q.vec && c + 4 <= q.C) {
+        const float4 u = *reinterpret_cast<const float4 *>(p);
+        v[i][0] = u.x;
+        v[i][1] = u.y;
+        v[i][2] = u.z;
+        v[i][3] = u.w;
+      } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if (r0 + i >= R) continue;
-      uint32_t ha, la, hb, lb;
-      split2(a[i], 0.f, fa, ha, la);
-      split2(b[i], 0.f, fb, hb, lb);
-      const size_t off = static_cast<size_t>(r0 + i) * cp + c;
-      *reinterpret_cast<uint32_t *>(hi + off) = (ha & 0xffffu) | (hb << 16);
-      *reinterpret_cast<uint32_t *>(lo + off) = (la & 0xffffu) | (lb << 16);
+        for (int j = 0; j < 4; ++j)
+          if (c + j < q.C) v[i][j] = p[j];
+      }
     }
-  }
-}
-
-// Largest finite |element| as fp32 bits (ordered like the values, so an
-// integer maximum, whose result does not depend on the order).
-__global__ void __launch_bounds__(256) k_absmax(const float *__restrict__ src, int64_t ld, int64_t R, int64_t C,
-                                                unsigned *out) {
-  unsigned m = 0;
-  const int64_t n = R * C;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t r = i / C;
-    const unsigned u = __float_as_uint(src[r * ld + (i - r * C)]) & 0x7fffffffu;
-    if (u < 0x7f800000u) m = max(m, u);
-  }
+    const int64_t plane = static_cast<int64_t>(q.R) * q.lp;
+    // one row of the block in split form, each column by its own scale
+    auto put = [&](uint16_t *hi, int i, const float (&f)[4]) {
+      if (r0 + i >= q.R || c >= q.lp) return;
+      uint32_t h[2], l[2];
 #pragma unroll
-  for (int k = 16; k > 0; k >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, k));
-  if ((threadIdx.x & 31) == 0 && m) atomicMax(out, m);
-}
-
-// f32 [R, C] -> split form [R, cp] with the scale of *mx; writes 2^-s.
-__global__ void __launch_bounds__(256) k_split_whole(const float *__restrict__ src, int64_t ld, int64_t R, int C, int cp,
-                                                     const unsigned *mx, uint16_t *hi, uint16_t *lo, float *inv) {
-  const int s = split_scale_exponent(__uint_as_float(*mx));
-  const float f = pow2f(s);
-  const int64_t nc = cp / 2, n = R * nc;
-  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i0 == 0) *inv = pow2f(-s);
-  for (int64_t i = i0; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t r = i / nc;
-    const int c = static_cast<int>(i - r * nc) * 2;
-    const float *p = src + r * ld + c;
-    uint32_t h, l;
-    split2(c < C ? p[0] : 0.f, c + 1 < C ? p[1] : 0.f, f, h, l);
-    *reinterpret_cast<uint32_t *>(hi + r * cp + c) = h;
-    *reinterpret_cast<uint32_t *>(lo + r * cp + c) = l;
+      for (int j = 0; j < 2; ++j) split2(v[i][2 * j] * f[2 * j], v[i][2 * j + 1] * f[2 * j + 1], 1.f, h[j], l[j]);
+      uint16_t *o = hi + static_cast<size_t>(r0 + i) * q.lp + c;
+      if (c + 4 <= q.lp) {
+        *reinterpret_cast<uint2 *>(o) = make_uint2(h[0], h[1]);
+        *reinterpret_cast<uint2 *>(o + plane) = make_uint2(l[0], l[1]);
+      }
+    };
+    // maximum (or sum) over the block's rows, per column, in a fixed order
+    auto over_rows = [&](const float (&x)[4], bool add, float (&out)[4]) {
+      __syncthreads();
+      *reinterpret_cast<float4 *>(&part[w][4 * lane]) = make_float4(x[0], x[1], x[2], x[3]);
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) out[j] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) out[j] = add ? out[j] + part[k][4 * lane + j] : fmaxf(out[j], part[k][4 * lane + j]);
+    };
+    if (q.rows.hi) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float m = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m = fmaxf(m, finite_abs(v[i][j]));
+        const int s = split_scale_exponent(warp_max(m));
+        const float e = pow2f(s), f[4] = {e, e, e, e};
+        put(q.rows.hi, i, f);
+        if (lane == 0 && r0 + i < q.R) q.rows.sc[static_cast<size_t>(cb) * q.R + r0 + i] = static_cast<int8_t>(s);
+      }
+    }
+    if (q.cols.hi || q.blocks.hi) {
+      float m[4] = {0.f, 0.f, 0.f, 0.f}, top[4];
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m[j] = fmaxf(m[j], finite_abs(v[i][j]));
+      over_rows(m, false, top);
+      if (q.cols.hi) {
+        int s[4];
+        float f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s[j] = split_scale_exponent(top[j]);
+          f[j] = pow2f(s[j]);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) put(q.cols.hi, i, f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (w == 0 && c + j < q.lp) q.cols.sc[static_cast<size_t>(rb) * q.lp + c + j] = static_cast<int8_t>(s[j]);
+      }
+      if (q.blocks.hi) {
+        const int s = split_scale_exponent(warp_max(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))));
+        const float e = pow2f(s), f[4] = {e, e, e, e};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) put(q.blocks.hi, i, f);
+        if (threadIdx.x == 0) q.blocks.sc[static_cast<size_t>(rb) * nb + cb] = static_cast<int8_t>(s);
+      }
+    }
+    if (q.sums) {
+      float m[4] = {0.f, 0.f, 0.f, 0.f}, sum[4];
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m[j] += v[i][j];
+      over_rows(m, true, sum);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (w == 0 && c + j < q.C) q.sums[static_cast<size_t>(rb) * q.C + c + j] = sum[j];
+    }
   }
 }
 
@@ -679,11 +777,10 @@ struct Operand {
   const uint16_t *p = nullptr;
   int64_t rows = 0, cols = 0, ld = 0;
   int planes = 1;
-  int64_t plane = 0;            // elements between hi and lo
-  const int8_t *sc = nullptr;   // f32 A: scales [block][row]
-  int64_t scld = 0;
-  const float *bs = nullptr;    // f32 B: 2^-s on the device
-  float bsc = 1.f;
+  int64_t plane = 0;           // elements between hi and lo
+  const int8_t *sc = nullptr;  // f32: scale exponents
+  int64_t scld = 0;            // ... between the blocks of 128 (A: of the contraction; B: of rows)
+  float bsc = 1.f;             // f32 B without sc: one factor
 };
 
 Operand from_split(const Split16View &v) {
@@ -698,85 +795,98 @@ Operand from_split(const Split16View &v) {
   return o;
 }
 
-Operand packed(const Mat &m, int64_t rows, int64_t cols, int dt, Workspace &ws, cudaStream_t s) {
-  Operand o;
-  o.rows = rows;
-  o.cols = cols;
-  if (rows16(m.p, m.ld, dt)) {
-    o.p = static_cast<const uint16_t *>(m.p);
-    o.ld = m.ld;
+// Prepares operands: 16-bit ones where they lie (or packed), f32 ones as jobs
+// of one launch of k_split, issued by go().
+enum Form { FORM_NONE, FORM_ROWS, FORM_COLS, FORM_BLOCKS };
+class Operands {
+ public:
+  Operands(int dt, Workspace &ws, cudaStream_t s) : dt_(dt), ws_(ws), s_(s) {}
+
+  // `m` for a product: FORM_ROWS / FORM_COLS as its A operand, contracted over
+  // columns / rows, FORM_BLOCKS as its B operand
+  Operand add(const Mat &m, int64_t rows, int64_t cols, Form form) {
+    if (dt_ != DT_F32) return packed(m, rows, cols);
+    Operand o;
+    o.rows = rows;
+    o.cols = cols;
+    o.ld = (cols + 7) / 8 * 8;
+    o.planes = 2;
+    o.plane = rows * o.ld;
+    uint16_t *d = static_cast<uint16_t *>(ws_.take(4 * rows * o.ld));
+    const int64_t rb = (rows + 127) / 128, cb = (cols + 127) / 128;
+    o.scld = form == FORM_ROWS ? rows : form == FORM_COLS ? o.ld : cb;
+    int8_t *sc = static_cast<int8_t *>(ws_.take(form == FORM_ROWS ? cb * rows : rb * o.scld));
+    o.p = d;
+    o.sc = sc;
+    if (ws_.sizing()) return o;
+    of(job(m, rows, cols, form), form) = SplitForm{d, sc};
     return o;
   }
-  o.ld = (cols + 7) / 8 * 8;
-  uint16_t *d = static_cast<uint16_t *>(ws.take(2 * rows * o.ld));
-  o.p = d;
-  if (!ws.sizing()) {
-    k_pack<<<grid_for(rows * o.ld / 2), 256, 0, s>>>(static_cast<const uint16_t *>(m.p), m.ld, rows,
-                                                     static_cast<int>(cols), static_cast<int>(o.ld), d);
+  // sums of the columns of `m` (which add() has seen) into part [rows / 128][cols]
+  float *sums(const Mat &m, int64_t rows, int64_t cols) {
+    float *part = static_cast<float *>(ws_.take(4 * ((rows + 127) / 128) * cols));
+    if (!ws_.sizing()) job(m, rows, cols, FORM_NONE).sums = part;
+    return part;
+  }
+  void go() {
+    if (!all_.n) return;
+    all_.total = 0;
+    for (int i = 0; i < all_.n; ++i) {
+      SplitJob &j = all_.job[i];
+      j.first = all_.total;
+      const int64_t blocks = static_cast<int64_t>(ceil_div(j.R, 128)) * ceil_div(j.C, 128);
+      if (blocks > INT32_MAX / 2 - all_.total) throw Error(kErrInvalidParameter, "the operands have too many blocks");
+      all_.total += static_cast<int>(blocks);
+    }
+    k_split<<<std::min(all_.total, 8 * sm_count()), 256, 0, s_>>>(all_);
     CUDA_LAUNCH_CHECK();
+    all_.n = 0;
   }
-  return o;
-}
 
-// A operand.  over_rows: the product contracts over the matrix's rows.
-Operand operand_a(const Mat &m, int64_t rows, int64_t cols, int dt, bool over_rows, Workspace &ws, cudaStream_t s) {
-  if (dt != DT_F32) return packed(m, rows, cols, dt, ws, s);
-  Operand o;
-  o.rows = rows;
-  o.cols = cols;
-  o.ld = (cols + 127) / 128 * 128;
-  o.planes = 2;
-  o.plane = rows * o.ld;
-  uint16_t *d = static_cast<uint16_t *>(ws.take(4 * rows * o.ld));
-  const int64_t nblk = over_rows ? (rows + 127) / 128 : o.ld / 128;
-  o.scld = over_rows ? o.ld : rows;
-  int8_t *sc = static_cast<int8_t *>(ws.take(nblk * o.scld));
-  o.p = d;
-  o.sc = sc;
-  if (ws.sizing()) return o;
-  const float *src = static_cast<const float *>(m.p);
-  if (over_rows) {
-    const dim3 grid(static_cast<unsigned>(o.ld / 64), static_cast<unsigned>(std::min<int64_t>(nblk, 65535)));
-    k_split_cols<<<grid, 256, 0, s>>>(src, m.ld, static_cast<int>(rows), static_cast<int>(cols), d, d + o.plane,
-                                      static_cast<int>(o.ld), sc);
-  } else {
-    Split16View v;
-    v.hi = d;
-    v.lo = d + o.plane;
-    v.sc = sc;
-    v.rows = static_cast<int>(rows);
-    v.cols = static_cast<int>(o.ld);
-    k_split_rows<<<grid_for(rows * (o.ld / 128) * 32), 256, 0, s>>>(src, m.ld, static_cast<int>(rows),
-                                                                    static_cast<int>(cols), rows16(m.p, m.ld, dt), v);
+ private:
+  static SplitForm &of(SplitJob &j, Form f) { return f == FORM_ROWS ? j.rows : f == FORM_COLS ? j.cols : j.blocks; }
+  // the job that reads `m`: one for all forms of one matrix (a second one if
+  // it has this form already, as when both weights are the same tensor)
+  SplitJob &job(const Mat &m, int64_t rows, int64_t cols, Form form) {
+    for (int i = 0; i < all_.n; ++i) {
+      SplitJob &j = all_.job[i];
+      if (j.src == m.p && j.ld == m.ld && j.R == rows && j.C == cols && (form == FORM_NONE || !of(j, form).hi)) return j;
+    }
+    if (all_.n == kMaxJobs) throw Error(kErrInternal, "too many operands in one step");
+    SplitJob &j = all_.job[all_.n++];
+    j = SplitJob{};
+    j.src = static_cast<const float *>(m.p);
+    j.ld = m.ld;
+    j.R = static_cast<int>(rows);
+    j.C = static_cast<int>(cols);
+    j.lp = static_cast<int>((cols + 7) / 8 * 8);
+    j.vec = rows16(m.p, m.ld, DT_F32);
+    return j;
   }
-  CUDA_LAUNCH_CHECK();
-  return o;
-}
-
-// B operand (either way round).
-Operand operand_b(const Mat &m, int64_t rows, int64_t cols, int dt, Workspace &ws, cudaStream_t s) {
-  if (dt != DT_F32) return packed(m, rows, cols, dt, ws, s);
-  Operand o;
-  o.rows = rows;
-  o.cols = cols;
-  o.ld = (cols + 7) / 8 * 8;
-  o.planes = 2;
-  o.plane = rows * o.ld;
-  uint16_t *d = static_cast<uint16_t *>(ws.take(4 * rows * o.ld));
-  unsigned *word = static_cast<unsigned *>(ws.take(8));
-  o.p = d;
-  o.bs = reinterpret_cast<const float *>(word + 1);
-  if (ws.sizing()) return o;
-  CUDA_CHECK(cudaMemsetAsync(word, 0, 4, s));
-  const float *src = static_cast<const float *>(m.p);
-  k_absmax<<<grid_for(rows * cols), 256, 0, s>>>(src, m.ld, rows, cols, word);
-  CUDA_LAUNCH_CHECK();
-  k_split_whole<<<grid_for(rows * o.ld / 2), 256, 0, s>>>(src, m.ld, rows, static_cast<int>(cols),
-                                                          static_cast<int>(o.ld), word, d, d + o.plane,
-                                                          reinterpret_cast<float *>(word + 1));
-  CUDA_LAUNCH_CHECK();
-  return o;
-}
+  Operand packed(const Mat &m, int64_t rows, int64_t cols) {
+    Operand o;
+    o.rows = rows;
+    o.cols = cols;
+    if (rows16(m.p, m.ld, dt_)) {
+      o.p = static_cast<const uint16_t *>(m.p);
+      o.ld = m.ld;
+      return o;
+    }
+    o.ld = (cols + 7) / 8 * 8;
+    uint16_t *d = static_cast<uint16_t *>(ws_.take(2 * rows * o.ld));
+    o.p = d;
+    if (!ws_.sizing()) {
+      k_pack<<<grid_for(rows * o.ld / 2), 256, 0, s_>>>(static_cast<const uint16_t *>(m.p), m.ld, rows,
+                                                        static_cast<int>(cols), static_cast<int>(o.ld), d);
+      CUDA_LAUNCH_CHECK();
+    }
+    return o;
+  }
+  int dt_;
+  Workspace &ws_;
+  cudaStream_t s_;
+  SplitJobs all_{};
+};
 
 // ---------------------------------------------------------------------------
 // Launch
@@ -862,9 +972,11 @@ void run(const Product &g, Workspace &ws, cudaStream_t s) {
     const int64_t tn = (g.N + (g.dual ? bn / 2 : bn) - 1) / (g.dual ? bn / 2 : bn);
     return (g.M + BM - 1) / BM * tn * p.batch;
   };
-  // 256-wide tiles read a third less shared memory for a product, as long as
-  // they still give every SM a tile
-  const int bn = !f32 && count(256) >= sms ? 256 : 128;
+  // tiles of 256 columns need less shared-memory traffic for a product
+  // (128-wide ones take 0.6 of their time each, not half), but come in
+  // coarser waves: whichever finishes first
+  auto waves = [&](int bn) { return static_cast<double>((count(bn) + sms - 1) / sms); };
+  const int bn = !f32 && waves(256) <= 0.6 * waves(128) ? 256 : 128;
   const int64_t tiles = count(bn);
   p.tiles_m = static_cast<int>((g.M + BM - 1) / BM);
   p.tiles_n = static_cast<int>(tiles / p.tiles_m / p.batch);
@@ -894,7 +1006,9 @@ void run(const Product &g, Workspace &ws, cudaStream_t s) {
     maps.b[i] = map_of(b, bf, g.b_mn ? 64 : bn / 2);
     q.sc[i] = a.sc;
     q.scld[i] = a.scld;
-    q.bs[i] = b.bs;
+    q.bs[i] = b.sc;
+    q.bsn[i] = g.b_mn ? 1 : b.scld;
+    q.bsk[i] = g.b_mn ? b.scld : 1;
     q.bsc[i] = b.bsc;
   }
   if (splits > 1) {
@@ -977,6 +1091,18 @@ Operand split_weight(const GatedLinear::SplitWeight &w, int64_t rows, int64_t co
   o.bsc = std::ldexp(1.f, -w.scale);
   return o;
 }
+
+// Column sums of dz: f32 from the sums of its blocks (part), 16-bit by a pass
+// of its own.
+void bias_grad(const Mat &dz, int64_t M, int64_t N, float scale, int dt, const float *part, void *db, Workspace &ws,
+               cudaStream_t s) {
+  if (dt == DT_F32) {
+    if (!ws.sizing()) column_join(part, ceil_div(M, 128), N, scale, db, dt, s);
+    return;
+  }
+  float *mine = static_cast<float *>(ws.take(4 * column_sum_floats(M, N)));
+  if (!ws.sizing()) column_sum(dz.p, dt, dz.ld, M, N, scale, db, dt, mine, s);
+}
 }  // namespace
 
 void gated_linear_fwd(const GatedLinear &a, Workspace &ws, cudaStream_t s) {
@@ -988,6 +1114,7 @@ void gated_linear_fwd(const GatedLinear &a, Workspace &ws, cudaStream_t s) {
     few_rows(f, s);
     return;
   }
+  Operands prep(a.dtype, ws, s);
   Product g;
   g.dt = a.dtype;
   g.epi = E_GATED;
@@ -996,13 +1123,14 @@ void gated_linear_fwd(const GatedLinear &a, Workspace &ws, cudaStream_t s) {
   g.N = a.F;
   g.K = a.K;
   g.dual = true;
-  g.a[0] = a.x_split ? from_split(*a.x_split) : operand_a(a.x, a.M, a.K, a.dtype, false, ws, s);
-  g.b[0] = a.wg_split.hi ? split_weight(a.wg_split, a.F, a.K) : operand_b(a.wg, a.F, a.K, a.dtype, ws, s);
-  g.b[1] = a.wv_split.hi ? split_weight(a.wv_split, a.F, a.K) : operand_b(a.wv, a.F, a.K, a.dtype, ws, s);
+  g.a[0] = a.x_split ? from_split(*a.x_split) : prep.add(a.x, a.M, a.K, FORM_ROWS);
+  g.b[0] = a.wg_split.hi ? split_weight(a.wg_split, a.F, a.K) : prep.add(a.wg, a.F, a.K, FORM_BLOCKS);
+  g.b[1] = a.wv_split.hi ? split_weight(a.wv_split, a.F, a.K) : prep.add(a.wv, a.F, a.K, FORM_BLOCKS);
   g.e = plain_out(a.h);
   g.e.act = a.act;
   g.e.b0 = a.bg;
   g.e.b1 = a.bv;
+  prep.go();
   run(g, ws, s);
 }
 
@@ -1019,82 +1147,93 @@ void gated_linear_bwd(const GatedLinear &a, Workspace &ws, cudaStream_t s) {
     zero_rows(a.dbv, a.F, 1, a.F, a.dtype, s);
     return;
   }
-  if (!a.dx.p && !a.dwg.p && !a.dwv.p && !a.dbg && !a.dbv) return;
+  const bool weights = a.dwg.p || a.dwv.p;
+  if (!a.dx.p && !weights && !a.dbg && !a.dbv) return;
+  const bool f32 = a.dtype == DT_F32;
   const size_t es = dtype_size(a.dtype);
   const int64_t fp = (a.F + 7) / 8 * 8;
-  MutMat dz{ws.take(2 * a.M * fp * es), fp}, dzv{ws.sizing() ? nullptr : static_cast<char *>(dz.p) + a.M * fp * es, fp};
-  const Operand wg = a.wg_split.hi ? split_weight(a.wg_split, a.F, a.K) : operand_b(a.wg, a.F, a.K, a.dtype, ws, s);
-  const Operand wv = a.wv_split.hi ? split_weight(a.wv_split, a.F, a.K) : operand_b(a.wv, a.F, a.K, a.dtype, ws, s);
-  {
-    Product g;
-    g.dt = a.dtype;
-    g.epi = E_GATED_BWD;
-    g.products = a.products;
-    g.M = a.M;
-    g.N = a.F;
-    g.K = a.K;
-    g.dual = true;
-    g.a[0] = a.x_split ? from_split(*a.x_split) : operand_a(a.x, a.M, a.K, a.dtype, false, ws, s);
-    g.b[0] = wg;
-    g.b[1] = wv;
-    g.e = plain_out(dz);
-    g.e.out1 = dzv.p;
-    g.e.act = a.act;
-    g.e.b0 = a.bg;
-    g.e.b1 = a.bv;
-    g.e.in = a.dh.p;
-    g.e.ldin = a.dh.ld;
-    run(g, ws, s);
+  char *buf = static_cast<char *>(ws.take(2 * a.M * fp * es));
+  const MutMat dz[2] = {{buf, fp}, {ws.sizing() ? nullptr : buf + a.M * fp * es, fp}};
+  Operands prep(a.dtype, ws, s);
+  Operand w[2], xb;
+  w[0] = a.wg_split.hi ? split_weight(a.wg_split, a.F, a.K) : prep.add(a.wg, a.F, a.K, FORM_BLOCKS);
+  w[1] = a.wv_split.hi ? split_weight(a.wv_split, a.F, a.K) : prep.add(a.wv, a.F, a.K, FORM_BLOCKS);
+  Product g;
+  g.dt = a.dtype;
+  g.products = a.products;
+  g.a[0] = a.x_split ? from_split(*a.x_split) : prep.add(a.x, a.M, a.K, FORM_ROWS);
+  if (weights) xb = f32 ? prep.add(a.x, a.M, a.K, FORM_BLOCKS) : g.a[0];
+  g.epi = E_GATED_BWD;
+  g.M = a.M;
+  g.N = a.F;
+  g.K = a.K;
+  g.dual = true;
+  g.b[0] = w[0];
+  g.b[1] = w[1];
+  g.e = plain_out(dz[0]);
+  g.e.out1 = dz[1].p;
+  g.e.act = a.act;
+  g.e.b0 = a.bg;
+  g.e.b1 = a.bv;
+  g.e.in = a.dh.p;
+  g.e.ldin = a.dh.ld;
+  prep.go();
+  run(g, ws, s);
+
+  const Mat m[2] = {{dz[0].p, fp}, {dz[1].p, fp}};
+  void *const dw[2] = {a.dwg.p, a.dwv.p}, *const db[2] = {a.dbg, a.dbv};
+  const int64_t lddw[2] = {a.dwg.ld, a.dwv.ld};
+  Operand rows[2], cols[2];
+  float *part[2] = {nullptr, nullptr};
+  for (int i = 0; i < 2; ++i) {
+    if (a.dx.p) rows[i] = prep.add(m[i], a.M, a.F, FORM_ROWS);
+    if (dw[i]) cols[i] = f32 || !a.dx.p ? prep.add(m[i], a.M, a.F, FORM_COLS) : rows[i];
+    if (db[i] && f32) part[i] = prep.sums(m[i], a.M, a.F);
   }
-  const Mat mg{dz.p, fp}, mv{dzv.p, fp};
+  prep.go();
   if (a.dx.p) {
-    Product g;
-    g.dt = a.dtype;
-    g.products = a.products;
-    g.M = a.M;
-    g.N = a.K;
-    g.K = a.F;
-    g.kcat = true;
-    g.b_mn = true;
-    g.a[0] = operand_a(mg, a.M, a.F, a.dtype, false, ws, s);
-    g.a[1] = operand_a(mv, a.M, a.F, a.dtype, false, ws, s);
-    g.b[0] = wg;
-    g.b[1] = wv;
-    g.e = plain_out(a.dx);
-    run(g, ws, s);
+    Product q;
+    q.dt = a.dtype;
+    q.products = a.products;
+    q.M = a.M;
+    q.N = a.K;
+    q.K = a.F;
+    q.kcat = true;
+    q.b_mn = true;
+    for (int i = 0; i < 2; ++i) {
+      q.a[i] = rows[i];
+      q.b[i] = w[i];
+    }
+    q.e = plain_out(a.dx);
+    run(q, ws, s);
   }
-  if (a.dwg.p || a.dwv.p) {
-    Product g;
-    g.dt = a.dtype;
-    g.products = a.products;
-    g.M = a.F;
-    g.N = a.K;
-    g.K = a.M;
-    g.a_mn = g.b_mn = true;
-    g.b[0] = operand_b(a.x, a.M, a.K, a.dtype, ws, s);
-    const bool both = a.dwg.p && a.dwv.p;
-    g.a[0] = operand_a(a.dwg.p ? mg : mv, a.M, a.F, a.dtype, true, ws, s);
-    g.e = plain_out(a.dwg.p ? a.dwg : a.dwv);
-    if (both && a.dwg.ld == a.dwv.ld) {
-      g.batch2 = true;
-      g.a[1] = operand_a(mv, a.M, a.F, a.dtype, true, ws, s);
-      g.e.out1 = a.dwv.p;
-      run(g, ws, s);
+  if (weights) {
+    Product q;
+    q.dt = a.dtype;
+    q.products = a.products;
+    q.M = a.F;
+    q.N = a.K;
+    q.K = a.M;
+    q.a_mn = q.b_mn = true;
+    q.b[0] = xb;
+    if (dw[0] && dw[1] && lddw[0] == lddw[1]) {
+      q.batch2 = true;
+      q.a[0] = cols[0];
+      q.a[1] = cols[1];
+      q.e = plain_out(a.dwg);
+      q.e.out1 = dw[1];
+      run(q, ws, s);
     } else {
-      run(g, ws, s);
-      if (both) {
-        g.a[0] = operand_a(mv, a.M, a.F, a.dtype, true, ws, s);
-        g.e = plain_out(a.dwv);
-        run(g, ws, s);
+      for (int i = 0; i < 2; ++i) {
+        if (!dw[i]) continue;
+        q.a[0] = cols[i];
+        q.e = plain_out(MutMat{dw[i], lddw[i]});
+        run(q, ws, s);
       }
     }
   }
-  for (int i = 0; i < 2; ++i) {
-    void *db = i ? a.dbv : a.dbg;
-    if (!db) continue;
-    float *part = static_cast<float *>(ws.take(4 * column_sum_floats(a.M, a.F)));
-    if (!ws.sizing()) column_sum(i ? mv.p : mg.p, a.dtype, fp, a.M, a.F, 1.f, db, a.dtype, part, s);
-  }
+  for (int i = 0; i < 2; ++i)
+    if (db[i]) bias_grad(m[i], a.M, a.F, 1.f, a.dtype, part[i], db[i], ws, s);
 }
 
 void linear_fwd(const Linear &a, Workspace &ws, cudaStream_t s) {
@@ -1106,19 +1245,21 @@ void linear_fwd(const Linear &a, Workspace &ws, cudaStream_t s) {
     few_rows(f, s);
     return;
   }
+  Operands prep(a.dtype, ws, s);
   Product g;
   g.dt = a.dtype;
   g.M = a.M;
   g.N = a.N;
   g.K = a.K;
-  g.a[0] = operand_a(a.x, a.M, a.K, a.dtype, false, ws, s);
-  g.b[0] = operand_b(a.w, a.N, a.K, a.dtype, ws, s);
+  g.a[0] = prep.add(a.x, a.M, a.K, FORM_ROWS);
+  g.b[0] = prep.add(a.w, a.N, a.K, FORM_BLOCKS);
   g.e = plain_out(a.y);
   g.e.act = a.act;
   g.e.scale = a.scale;
   g.e.b0 = a.b;
   g.e.in = a.residual.p;
   g.e.ldin = a.residual.ld;
+  prep.go();
   run(g, ws, s);
 }
 
@@ -1132,20 +1273,23 @@ void linear_bwd(const Linear &a, Workspace &ws, cudaStream_t s) {
     return;
   }
   if (!a.dx.p && !a.dw.p && !a.db) return;
-  const bool id = a.act == ACT_IDENTITY;
-  Operand w;
-  if (!id || a.dx.p) w = operand_b(a.w, a.N, a.K, a.dtype, ws, s);
+  const bool id = a.act == ACT_IDENTITY, f32 = a.dtype == DT_F32;
+  Operands prep(a.dtype, ws, s);
+  Operand w, xr, xb;
+  if (!id || a.dx.p) w = prep.add(a.w, a.N, a.K, FORM_BLOCKS);
+  if (!id) xr = prep.add(a.x, a.M, a.K, FORM_ROWS);
+  if (a.dw.p) xb = f32 || id ? prep.add(a.x, a.M, a.K, FORM_BLOCKS) : xr;
   Mat dz = a.dy;
   if (!id) {
     const int64_t np = (a.N + 7) / 8 * 8;
-    MutMat out{ws.take(a.M * np * dtype_size(a.dtype)), np};
+    const MutMat out{ws.take(a.M * np * dtype_size(a.dtype)), np};
     Product g;
     g.dt = a.dtype;
     g.epi = E_LINEAR_BWD;
     g.M = a.M;
     g.N = a.N;
     g.K = a.K;
-    g.a[0] = operand_a(a.x, a.M, a.K, a.dtype, false, ws, s);
+    g.a[0] = xr;
     g.b[0] = w;
     g.e = plain_out(out);
     g.e.act = a.act;
@@ -1153,10 +1297,17 @@ void linear_bwd(const Linear &a, Workspace &ws, cudaStream_t s) {
     g.e.b0 = a.b;
     g.e.in = a.dy.p;
     g.e.ldin = a.dy.ld;
+    prep.go();
     run(g, ws, s);
     dz = Mat{out.p, np};
   }
   const float scale = id ? a.scale : 1.f;
+  Operand rows, cols;
+  float *part = nullptr;
+  if (a.dx.p) rows = prep.add(dz, a.M, a.N, FORM_ROWS);
+  if (a.dw.p) cols = f32 || !a.dx.p ? prep.add(dz, a.M, a.N, FORM_COLS) : rows;
+  if (a.db && f32) part = prep.sums(dz, a.M, a.N);
+  prep.go();
   if (a.dx.p) {
     Product g;
     g.dt = a.dtype;
@@ -1164,7 +1315,7 @@ void linear_bwd(const Linear &a, Workspace &ws, cudaStream_t s) {
     g.N = a.K;
     g.K = a.N;
     g.b_mn = true;
-    g.a[0] = operand_a(dz, a.M, a.N, a.dtype, false, ws, s);
+    g.a[0] = rows;
     g.b[0] = w;
     g.e = plain_out(a.dx);
     g.e.scale = scale;
@@ -1177,16 +1328,13 @@ void linear_bwd(const Linear &a, Workspace &ws, cudaStream_t s) {
     g.N = a.K;
     g.K = a.M;
     g.a_mn = g.b_mn = true;
-    g.a[0] = operand_a(dz, a.M, a.N, a.dtype, true, ws, s);
-    g.b[0] = operand_b(a.x, a.M, a.K, a.dtype, ws, s);
+    g.a[0] = cols;
+    g.b[0] = xb;
     g.e = plain_out(a.dw);
     g.e.scale = scale;
     run(g, ws, s);
   }
-  if (a.db) {
-    float *part = static_cast<float *>(ws.take(4 * column_sum_floats(a.M, a.N)));
-    if (!ws.sizing()) column_sum(dz.p, a.dtype, dz.ld, a.M, a.N, scale, a.db, a.dtype, part, s);
-  }
+  if (a.db) bias_grad(dz, a.M, a.N, scale, a.dtype, part, a.db, ws, s);
 }
 
 }  // namespace pet

@@ -149,11 +149,12 @@ struct Row {
   }
   // zeros into the columns past d
   static __device__ __forceinline__ void trim(int t, int d, float2 (&x)[P]) {
-    if (FULL) return;
+    if constexpr (!FULL) {
 #pragma unroll
-    for (int k = 0; k < P; ++k) {
-      if (col(2 * k / V, t) >= d) x[k].x = 0.f;
-      if (col((2 * k + 1) / V, t) >= d) x[k].y = 0.f;
+      for (int k = 0; k < P; ++k) {
+        if (col(2 * k / V, t) >= d) x[k].x = 0.f;
+        if (col((2 * k + 1) / V, t) >= d) x[k].y = 0.f;
+      }
     }
   }
 };

@@ -109,7 +109,10 @@ __global__ void __launch_bounds__(256) k_few_rows(const FewRows a, int wpr) {
   if (n >= a.N || lane >= a.M) return;
   if (a.b0) v += to_f(static_cast<const T *>(a.b0)[n]);
   if (DUAL && a.b1) w += to_f(static_cast<const T *>(a.b1)[n]);
-  with_act(a.act, [&](auto A) { v = act_only<decltype(A)::value, sizeof(T) == 2>(v); });
+  with_act(a.act, [&](auto A) {
+    float da;
+    act_pair<decltype(A)::value>(v, v, da);
+  });
   if (DUAL) v *= w;
   else v = v * a.scale + (a.res ? to_f(static_cast<const T *>(a.res)[lane * a.ldr + n]) : 0.f);
   static_cast<T *>(a.out)[lane * a.ldo + n] = from_f<T>(v);

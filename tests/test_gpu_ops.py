@@ -347,6 +347,19 @@ def test_expanded_gradient_and_leading_dimensions(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("m", [3, 64])
+def test_same_tensor_twice(dtype, m):
+    """One weight for both projections, and x as its own residual."""
+    g = gen(5)
+    x, w = rand(g, m, 96, dtype=dtype), rand(g, 96, 96, dtype=dtype, std=0.1)
+    check_gated(x, w, w, None, None, "silu", rand(g, m, 96, dtype=dtype))
+    check_linear(x, w, None, "identity", x, 1.0, x)
+    a = ops.residual_norm(x, x, w[0], w[0])
+    b = ops.residual_norm(x, x.clone(), w[0].clone(), w[0].clone())
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 def test_no_rows(dtype):
     x, w = torch.empty(0, 64, dtype=dtype, device="cuda"), torch.ones(32, 64, dtype=dtype, device="cuda")
     b = torch.ones(32, dtype=dtype, device="cuda")
