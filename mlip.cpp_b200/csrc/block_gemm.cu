@@ -21,6 +21,12 @@
 //    accumulator warps add the partial sum to fp32 registers with
 //    round-to-nearest.
 //
+// Pairs (16-bit): where there are enough rows, two SMs take a tile of 256 x 256
+// together (cta_group::2).  Each loads its own 128 rows of A and half of B's
+// rows, the leader issues M = 256 MMAs that read both halves and leave each SM
+// its own rows' accumulator: a third fewer bytes in and out of shared memory
+// for a product.
+//
 // Forms of a launch: `dual` (the gated projections: a tile's accumulator
 // holds BN / 2 columns of x Wg^T beside the same columns of x Wv^T, so the
 // epilogue has both in one thread), `kcat` (two pairs of operands along the
@@ -52,25 +58,29 @@ namespace {
 
 constexpr int BM = 128, BK = 64;
 constexpr int kTile = BM * 128;  // bytes of 128 rows x 64 16-bit elements
-constexpr int kAccWarps = 8;
+
+constexpr int kAccWarps = 8;  // two per quarter of the tensor-memory lanes
 constexpr int kThreads = 64 + 32 * kAccWarps;
-constexpr int kStageFloats = 32 * 32;  // staging of one accumulator warp
+constexpr int kStageFloats = 32 * 32;  // turning block of one accumulator warp
 
 enum Epi : int { E_LINEAR = 0, E_LINEAR_BWD = 1, E_GATED = 2, E_GATED_BWD = 3, E_PARTIAL = 4 };
 
 // MODE: 16-bit operands (one product, planes = 1) or split-fp16 (planes = 2).
-template <bool F32, int BN>
+template <bool F32, int BN, bool PAIR>
 struct Cfg {
   static constexpr int Planes = F32 ? 2 : 1;
-  static constexpr int BTile = BN * 128;
+  static constexpr int BRows = PAIR ? BN / 2 : BN;  // rows of B that one CTA loads
+  static constexpr int BTile = BRows * 128;
   static constexpr int StageBytes = Planes * (kTile + BTile);
-  static constexpr int Stages = F32 ? 3 : (BN == 256 ? 4 : 6);
+  static constexpr int Stages = 192 * 1024 / StageBytes;
+
   static constexpr int Bufs = 512 / BN;
   static constexpr int Chunk = F32 ? 2 : 1 << 30;  // k tiles per accumulator pass
   static constexpr int BarBytes = 256;
   static constexpr int Smem = 1024 + Stages * StageBytes + kAccWarps * kStageFloats * 4 + BarBytes;
 };
-static_assert(Cfg<false, 256>::Smem <= 232448 && Cfg<false, 128>::Smem <= 232448 && Cfg<true, 128>::Smem <= 232448,
+static_assert(Cfg<false, 256, false>::Smem <= 232448 && Cfg<false, 128, false>::Smem <= 232448 &&
+                  Cfg<true, 128, false>::Smem <= 232448 && Cfg<false, 256, true>::Smem <= 232448,
               "shared memory of one CTA");
 
 struct EpiArgs {
@@ -105,41 +115,31 @@ struct Maps {
 
 __device__ int g_block_err = 0;
 
+// One thread of the warp, in the form that lets the compiler keep what it
+// issues to the tensor core and to TMA in uniform registers (a test of the
+// lane left the MMA issue, not the MMAs, as the limit: 60 against 68 us for
+// 8192 x 4096 x 1024 in bf16).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e != 0;
+}
+
 __device__ __forceinline__ void tma3(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
+// into this CTA's shared memory, completing on a barrier of the pair's leader
+__device__ __forceinline__ void tma3_pair(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
 __device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-
-// MN-major operand of 64-row chunks, each [64 k][64 rows] in 128-byte rows:
-// 8 KB between chunks, 1 KB between groups of 8 k.
-__device__ __forceinline__ uint64_t mn_desc(uint32_t start) {
-  return static_cast<uint64_t>((start >> 4) & 0x3FFFu) | (static_cast<uint64_t>(8192 >> 4) << 16) |
-         (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
-
-// Two blocks of 32 lanes x 32 consecutive fp32 columns -> 32 registers each;
-// the wait names every register, so no use of one can move before it.
-__device__ __forceinline__ void tmem_ld2x32(uint32_t ta, uint32_t tb, float (&a)[32], float (&b)[32]) {
-#define PET_R8(x, k) "=f"(x[k]), "=f"(x[k + 1]), "=f"(x[k + 2]), "=f"(x[k + 3]), "=f"(x[k + 4]), "=f"(x[k + 5]), "=f"(x[k + 6]), "=f"(x[k + 7])
-#define PET_LD32(x, addr)                                                                          \
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "                                           \
-               "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"                           \
-               "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"          \
-               : PET_R8(x, 0), PET_R8(x, 8), PET_R8(x, 16), PET_R8(x, 24)                          \
-               : "r"(addr))
-#define PET_W8(x, k) "+f"(x[k]), "+f"(x[k + 1]), "+f"(x[k + 2]), "+f"(x[k + 3]), "+f"(x[k + 4]), "+f"(x[k + 5]), "+f"(x[k + 6]), "+f"(x[k + 7])
-  PET_LD32(a, ta);
-  PET_LD32(b, tb);
-  asm volatile("tcgen05.wait::ld.sync.aligned;" : PET_W8(a, 0), PET_W8(a, 8), PET_W8(a, 16), PET_W8(a, 24)::"memory");
-  asm volatile("" : PET_W8(b, 0), PET_W8(b, 8), PET_W8(b, 16), PET_W8(b, 24)::"memory");
-#undef PET_R8
-#undef PET_LD32
-#undef PET_W8
 }
 
 // One tile's coordinates from its number: groups of 8 row tiles, columns
@@ -167,13 +167,13 @@ __device__ __forceinline__ Item item_of(const Params &p, int it) {
 // lane has V consecutive columns (16 bytes of T) of row i * 32 / L + lane / L,
 // i < L.  16-byte piece k of row r lies at place k ^ (r % 8), which keeps both
 // accesses free of bank conflicts.
-__device__ __forceinline__ float4 *piece(float *st, int r, int k) {
-  return reinterpret_cast<float4 *>(st + r * 32 + ((k ^ (r & 7)) << 2));
-}
 template <typename T>
 struct Turned {
   static constexpr int V = 16 / static_cast<int>(sizeof(T)), L = 32 / V;
   float x[L][V];
+  static __device__ __forceinline__ float4 *piece(float *st, int r, int k) {
+    return reinterpret_cast<float4 *>(st + r * 32 + ((k ^ (r & 7)) << 2));
+  }
   static __device__ __forceinline__ int row(int i, int lane) { return i * (32 / L) + lane / L; }
   static __device__ __forceinline__ int col(int lane) { return (lane % L) * V; }
   __device__ __forceinline__ void turn(float *st, int lane, const float (&v)[32]) {
@@ -228,17 +228,34 @@ struct Input {
   }
 };
 
+// Rows that are not 16-byte aligned go out a row at a time, a column a lane,
+// after another turn through `st`.
 template <typename T>
-__device__ __forceinline__ void block_store(const Turned<T> &b, T *out, int64_t ldo, bool vec, int lane, int row0,
-                                            int col0, int M, int N) {
+__device__ __forceinline__ void block_store(const Turned<T> &b, T *out, int64_t ldo, bool vec, float *st, int lane,
+                                            int row0, int col0, int M, int N) {
   using U = Turned<T>;
   const int c = col0 + U::col(lane);
+  if (!vec) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < U::L; ++i)
+#pragma unroll
+      for (int j = 0; j < U::V; j += 4)
+        *U::piece(st, U::row(i, lane), (U::col(lane) + j) / 4) =
+            make_float4(b.x[i][j], b.x[i][j + 1], b.x[i][j + 2], b.x[i][j + 3]);
+    __syncwarp();
+    if (col0 + lane < N)
+      for (int r = 0; r < 32 && row0 + r < M; ++r)
+        out[static_cast<size_t>(row0 + r) * ldo + col0 + lane] =
+            from_f<T>(reinterpret_cast<const float *>(U::piece(st, r, lane / 4))[lane % 4]);
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < U::L; ++i) {
     const int r = row0 + U::row(i, lane);
     if (r >= M || c >= N) continue;
     T *q = out + static_cast<size_t>(r) * ldo + c;
-    if (vec && c + U::V <= N) {
+    if (c + U::V <= N) {
       *reinterpret_cast<uint4 *>(q) = pack<T>(b.x[i]);
     } else {
 #pragma unroll
@@ -299,13 +316,13 @@ __device__ __forceinline__ void epilogue(const Params &p, int batch, float *st, 
       }
     }
   });
-  block_store<T>(a, static_cast<T *>(batch ? e.out1 : e.out0), e.ldo, e.vout, lane, row0, col0, p.M, p.N);
-  if (EPI == E_GATED_BWD) block_store<T>(b, static_cast<T *>(e.out1), e.ldo, e.vout, lane, row0, col0, p.M, p.N);
+  block_store<T>(a, static_cast<T *>(batch ? e.out1 : e.out0), e.ldo, e.vout, st, lane, row0, col0, p.M, p.N);
+  if (EPI == E_GATED_BWD) block_store<T>(b, static_cast<T *>(e.out1), e.ldo, e.vout, st, lane, row0, col0, p.M, p.N);
 }
 
-template <bool F32, int BN, int EPI, typename T>
+template <bool F32, int BN, bool PAIR, int EPI, typename T>
 __global__ void __launch_bounds__(kThreads, 1) k_block_gemm(const __grid_constant__ Maps maps, const Params p) {
-  using C = Cfg<F32, BN>;
+  using C = Cfg<F32, BN, PAIR>;
   constexpr bool kDual = EPI == E_GATED || EPI == E_GATED_BWD;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
@@ -320,10 +337,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_block_gemm(const __grid_constan
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tail + 232);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = PAIR ? static_cast<int>(cluster_rank()) : 0;
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"(512));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    if (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                   "r"(512));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                   "r"(512));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
   }
   if (tid == 0) {
     for (int s = 0; s < C::Stages; ++s) {
@@ -332,16 +356,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_block_gemm(const __grid_constan
     }
     for (int b = 0; b < C::Bufs; ++b) {
       mbar_init(accf0 + 8 * b, 1);
-      mbar_init(acce0 + 8 * b, 32 * kAccWarps);
+      mbar_init(acce0 + 8 * b, (PAIR ? 2 : 1) * kAccWarps);  // of the pair, at the leader
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   tc_fence_before();
-  __syncthreads();
+  if (PAIR) cluster_sync();  // both CTAs' barriers and tensor memory exist
+  else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  const int first = PAIR ? static_cast<int>(cluster_id_x()) : static_cast<int>(blockIdx.x);
+  const int step = PAIR ? static_cast<int>(num_clusters_x()) : static_cast<int>(gridDim.x);
+  constexpr int TM = PAIR ? 2 * BM : BM;  // rows of a tile
   const int items = p.batch * p.splits * p.tiles_m * p.tiles_n;
   const int out_n = p.dual ? BN / 2 : BN;  // output columns of a tile
   const int planes = F32 ? (p.products == 1 ? 1 : 2) : 1;
@@ -349,12 +377,49 @@ __global__ void __launch_bounds__(kThreads, 1) k_block_gemm(const __grid_constan
 
   if (warp == 0) {
     // ---------------- TMA producer ----------------
-    if (lane == 0) {
+    if (elect_one()) {
       int it = 0;
       bool ok = true;
-      for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+      // one k tile of an item: the pair of operands and the place in them
+      struct At {
+        const CUtensorMap *a, *b0, *b1;
+        int x, m0, nb0, nb1;
+      };
+      auto locate = [&](const Item &t, int kt) {
+        const int m0 = t.tm * TM + rank * BM, n0 = t.tn * out_n;
+        const int seg = kt >= p.kt0 ? 1 : 0;
+        At o;
+        o.x = (kt - (seg ? p.kt0 : 0)) * BK;
+        o.m0 = m0;
+        // this CTA's rows of B: two boxes of BRows / 2, in the dual form one of
+        // each weight, or (pair) both of this CTA's weight
+        o.nb0 = n0 + (PAIR && !p.dual ? rank * C::BRows : 0);
+        o.nb1 = p.dual && !PAIR ? n0 : o.nb0 + C::BRows / 2;
+        o.a = &maps.a[t.batch | seg];
+        o.b0 = &maps.b[PAIR && p.dual ? rank : seg];
+        o.b1 = &maps.b[p.dual ? (PAIR ? rank : 1) : seg];
+        return o;
+      };
+      // every box of the tile, in the order of shared memory
+      auto boxes = [&](const At &o, auto &&load) {
+        for (int z = 0; z < planes; ++z) {
+          const uint32_t sa = z * kTile, sb = C::Planes * kTile + z * C::BTile;
+          if (p.a_mn) {
+            load(sa, o.a, o.m0, o.x, z);
+            load(sa + 8192, o.a, o.m0 + 64, o.x, z);
+          } else {
+            load(sa, o.a, o.x, o.m0, z);
+          }
+          if (p.b_mn) {
+            for (int c = 0; c < C::BRows / 64; ++c) load(sb + 8192 * c, o.b0, o.nb0 + 64 * c, o.x, z);
+          } else {
+            load(sb, o.b0, o.x, o.nb0, z);
+            load(sb + C::BTile / 2, o.b1, o.x, o.nb1, z);
+          }
+        }
+      };
+      for (int item = first; item < items && ok; item += step) {
         const Item t = item_of(p, item);
-        const int m0 = t.tm * BM, n0 = t.tn * out_n;
         const int k_end = min(p.kt, (t.split + 1) * p.kt_split);
         for (int kt = t.split * p.kt_split; kt < k_end; ++kt, ++it) {
           const int s = it % C::Stages;
@@ -362,46 +427,55 @@ __global__ void __launch_bounds__(kThreads, 1) k_block_gemm(const __grid_constan
             ok = false;
             break;
           }
-          const int seg = kt >= p.kt0 ? 1 : 0, x = (kt - (seg ? p.kt0 : 0)) * BK;
-          const CUtensorMap *ma = &maps.a[t.batch | seg];
-          const uint32_t fb = full0 + 8 * s, st = base + s * C::StageBytes;
-          expect_tx(fb, planes * (kTile + C::BTile));
-          for (int z = 0; z < planes; ++z) {
-            const uint32_t sa = st + z * kTile, sb = st + C::Planes * kTile + z * C::BTile;
-            if (p.a_mn) {
-              tma3(sa, ma, fb, m0, x, z);
-              tma3(sa + 8192, ma, fb, m0 + 64, x, z);
-            } else {
-              tma3(sa, ma, fb, x, m0, z);
-            }
-            if (p.b_mn) {
-              for (int c = 0; c < BN / 64; ++c) tma3(sb + 8192 * c, &maps.b[seg], fb, n0 + 64 * c, x, z);
-            } else {
-              // two halves of BN / 2 rows: both weights' rows n0.. (dual), or
-              // 2 x BN / 2 consecutive rows
-              tma3(sb, &maps.b[seg], fb, x, n0, z);
-              tma3(sb + C::BTile / 2, &maps.b[p.dual ? 1 : seg], fb, x, p.dual ? n0 : n0 + BN / 2, z);
-            }
-          }
+          const uint32_t st = base + s * C::StageBytes;
+          const uint32_t fb = PAIR ? map_to_rank(full0 + 8 * s, 0) : full0 + 8 * s;
+          if (rank == 0) expect_tx(full0 + 8 * s, (PAIR ? 2 : 1) * planes * (kTile + C::BTile));
+          boxes(locate(t, kt), [&](uint32_t off, const CUtensorMap *map, int cx, int cy, int cz) {
+            if (PAIR) tma3_pair(st + off, map, fb, cx, cy, cz);
+            else tma3(st + off, map, fb, cx, cy, cz);
+          });
         }
       }
+      // (pair) the commits that free the last stages have arrived here before
+      // this CTA ends
+      if (PAIR)
+        for (int i = it; ok && i < it + C::Stages; ++i)
+          ok = wait_or_abort(empty0 + 8 * (i % C::Stages), ((i / C::Stages) & 1) ^ 1, abort_flag);
       issued = it;
     }
     __syncwarp();
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
-    if (lane == 0) {
+    if (rank == 0 && elect_one()) {
       const uint32_t fmt = (!F32 && p.bf16) ? (1u << 7) | (1u << 10) : 0u;
-      const uint32_t idesc = idesc_f16(BM, BN) | fmt | (static_cast<uint32_t>(p.a_mn) << 15) |
+      const uint32_t idesc = idesc_f16(TM, BN) | fmt | (static_cast<uint32_t>(p.a_mn) << 15) |
                              (static_cast<uint32_t>(p.b_mn) << 16);
-      // one MMA step is 16 k: 32 bytes along a K-major row, 16 rows of 128
-      // bytes of an MN-major chunk
-      const uint32_t ka = p.a_mn ? 2048u : 32u, kb = p.b_mn ? 2048u : 32u;
-      auto desc_a = [&](uint32_t a) { return p.a_mn ? mn_desc(a) : sw128_desc(a); };
-      auto desc_b = [&](uint32_t a) { return p.b_mn ? mn_desc(a) : sw128_desc(a); };
+      // Operand descriptors (tc_common.cuh: kmajor_desc): the upper word is the
+      // same for both ways round; the lower one is the address / 16 and, for
+      // an MN-major tile of 64-row chunks ([64 k][64 rows], 128-byte rows), the
+      // 8 KB between chunks.  Addresses stay below 2^18, so stages and steps
+      // are plain additions to it.  One MMA step is 16 k: 32 bytes along a
+      // K-major row, 16 rows of 128 bytes of an MN-major chunk.
+      const uint32_t lo_a = (base >> 4) | (p.a_mn ? (8192u >> 4) << 16 : 1u << 16);
+      const uint32_t lo_b = ((base + C::Planes * kTile) >> 4) | (p.b_mn ? (8192u >> 4) << 16 : 1u << 16);
+      const uint32_t ka = p.a_mn ? 2048u >> 4 : 32u >> 4, kb = p.b_mn ? 2048u >> 4 : 32u >> 4;
+      auto desc = [](uint32_t lo) {
+        constexpr uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+        uint64_t d;
+        asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "n"(hi));
+        return d;
+      };
+      auto mma = [&](uint32_t d, uint64_t a, uint64_t b, uint32_t acc) {
+        if (PAIR) mma_f16_pair(d, a, b, idesc, acc);
+        else mma_f16(d, a, b, idesc, acc);
+      };
+      auto commit = [&](uint32_t bar) {
+        if (PAIR) mma_commit_pair(bar);
+        else mma_commit(bar);
+      };
       int it = 0, pass = 0;
       bool ok = true;
-      for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+      for (int item = first; item < items && ok; item += step) {
         const Item t = item_of(p, item);
         const int k_end = min(p.kt, (t.split + 1) * p.kt_split);
         for (int kt0 = t.split * p.kt_split; kt0 < k_end && ok; ++pass) {
@@ -420,41 +494,49 @@ __global__ void __launch_bounds__(kThreads, 1) k_block_gemm(const __grid_constan
               break;
             }
             tc_fence_after();
-            const uint32_t sa = base + s * C::StageBytes, sb = sa + C::Planes * kTile;
+            const uint32_t da = lo_a + s * (C::StageBytes >> 4), db = lo_b + s * (C::StageBytes >> 4);
 #pragma unroll
             for (int kk = 0; kk < BK / 16; ++kk) {
-              const uint32_t first = (kt > kt0 || kk > 0) ? 1u : 0u;
-              const uint64_t ah = desc_a(sa + kk * ka), bh = desc_b(sb + kk * kb);
+              const uint32_t more = (kt > kt0 || kk > 0) ? 1u : 0u;
+              const uint64_t ah = desc(da + kk * ka), bh = desc(db + kk * kb);
               if (F32 && p.products == 3) {
-                mma_f16(d, desc_a(sa + kTile + kk * ka), bh, idesc, first);
-                mma_f16(d, ah, desc_b(sb + C::BTile + kk * kb), idesc, 1u);
-                mma_f16(d, ah, bh, idesc, 1u);
+                mma(d, desc(da + (kTile >> 4) + kk * ka), bh, more);
+                mma(d, ah, desc(db + (C::BTile >> 4) + kk * kb), 1u);
+                mma(d, ah, bh, 1u);
               } else {
-                mma_f16(d, ah, bh, idesc, first);
+                mma(d, ah, bh, more);
               }
             }
-            mma_commit(empty0 + 8 * s);
+            commit(empty0 + 8 * s);
           }
-          if (ok) mma_commit(accf0 + 8 * b);
+          if (ok) commit(accf0 + 8 * b);
           kt0 = p_end;
         }
       }
     }
     __syncwarp();
   } else {
-    // ------- accumulators and epilogue: warp -> (lane quarter q, half h) -------
-    // A warp's columns are two groups of BN / 4 of the accumulator: in the
-    // gated forms the gate and the value of the same outputs.
+    // ------- accumulators and epilogue: warp -> (lane quarter q, share h) -------
+    // A warp's columns are two groups of G of the accumulator: in the gated
+    // forms the gate and the value of the same outputs.
     constexpr int G = BN / 4;
     const int q = warp & 3, h = (warp - 2) / 4;
     const int cb[2] = {kDual ? h * G : h * 2 * G, kDual ? BN / 2 + h * G : h * 2 * G + G};
     float *st = staging + (warp - 2) * kStageFloats;
     const uint32_t tq = tmem + (static_cast<uint32_t>(q * 32) << 16);
+    // this warp has read accumulator b
+    auto release = [&](int b) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane) return;
+      if (PAIR) mbar_arrive_cluster(map_to_rank(acce0 + 8 * b, 0));
+      else mbar_arrive(acce0 + 8 * b);
+    };
     int pass = 0;
     bool ok = true;
-    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+    for (int item = first; item < items && ok; item += step) {
       const Item t = item_of(p, item);
-      const int row0 = t.tm * BM + q * 32, row = row0 + lane, n0 = t.tn * out_n;
+      const int row0 = t.tm * TM + rank * BM + q * 32, row = row0 + lane, n0 = t.tn * out_n;
       const int k0 = t.split * p.kt_split, k_end = min(p.kt, k0 + p.kt_split);
       constexpr int GA = F32 ? G : 1;
       // output columns a warp finishes, in blocks of 32; column of block i / 32
@@ -480,22 +562,28 @@ __global__ void __launch_bounds__(kThreads, 1) k_block_gemm(const __grid_constan
         for (int gi = 0; gi < 2; ++gi)
 #pragma unroll
           for (int j = 0; j < GA; ++j) acc[gi][j] = 0.f;
-        // 2^-(s + t) of this thread's row and each group's columns in one
-        // pass, requested a pass ahead
-        float sa_next, sb_next[2];
+        // scale exponents of this thread's row and of each group's columns in
+        // one pass, requested a pass ahead and not touched before it
+        int sa = 0, sb[2] = {0, 0};
         auto scales = [&](int kt) {
           const int seg = kt >= p.kt0 ? 1 : 0, o = t.batch | seg;
           const int blk = (kt - (seg ? p.kt0 : 0)) / C::Chunk;
-          sa_next = row < p.M ? pow2f(-static_cast<int>(p.sc[o][static_cast<size_t>(blk) * p.scld[o] + row])) : 0.f;
+          if (row < p.M) sa = p.sc[o][static_cast<size_t>(blk) * p.scld[o] + row];
 #pragma unroll
           for (int gi = 0; gi < 2; ++gi) {
             const int bi = p.dual ? (cb[gi] >= BN / 2 ? 1 : 0) : seg;
-            sb_next[gi] = p.bs[bi] ? pow2f(-static_cast<int>(__ldg(p.bs[bi] + (n0 / 128) * p.bsn[bi] + blk * p.bsk[bi]))) : p.bsc[bi];
+            if (p.bs[bi]) sb[gi] = p.bs[bi][((n0 + (p.dual ? 0 : cb[gi])) / 128) * p.bsn[bi] + blk * p.bsk[bi]];
           }
         };
         scales(k0);
         for (int kt = k0; kt < k_end; kt += C::Chunk, ++pass) {
-          const float f[2] = {sa_next * sb_next[0], sa_next * sb_next[1]};
+          const float fa = pow2f(-sa);
+          float f[2];
+#pragma unroll
+          for (int gi = 0; gi < 2; ++gi) {
+            const int bi = p.dual ? (cb[gi] >= BN / 2 ? 1 : 0) : (kt >= p.kt0 ? 1 : 0);
+            f[gi] = fa * (p.bs[bi] ? pow2f(-sb[gi]) : p.bsc[bi]);
+          }
           if (kt + C::Chunk < k_end) scales(kt + C::Chunk);
           b = pass % C::Bufs;
           if (!__all_sync(0xffffffffu, wait_or_abort(accf0 + 8 * b, (pass / C::Bufs) & 1, abort_flag))) {
@@ -503,14 +591,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_block_gemm(const __grid_constan
             break;
           }
           tc_fence_after();
-          float v[2][32];
-          tmem_ld2x32(tq + static_cast<uint32_t>(b * BN + cb[0]), tq + static_cast<uint32_t>(b * BN + cb[1]), v[0], v[1]);
-          tc_fence_before();
-          mbar_arrive(acce0 + 8 * b);
+          static_assert(!F32 || G == 32, "a group is 32 columns");
 #pragma unroll
-          for (int gi = 0; gi < 2; ++gi)
+          for (int gi = 0; gi < 2; ++gi) {
+            float v[32];
+            tmem_ld32(tq + static_cast<uint32_t>(b * BN + cb[gi]), v);
+            if (gi) release(b);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) acc[gi][F32 ? j : 0] = __fmaf_rn(v[gi][j], f[gi], acc[gi][F32 ? j : 0]);
+            for (int j = 0; j < 32; ++j) acc[gi][F32 ? j : 0] = __fmaf_rn(v[j], f[gi], acc[gi][F32 ? j : 0]);
+          }
         }
         if (!ok) break;
       } else {
@@ -523,9 +612,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_block_gemm(const __grid_constan
         ++pass;
       }
       auto get = [&](int gi, int c, float(&v)[32]) {
-        if (F32) {
+        if constexpr (F32) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = acc[gi][F32 ? c + j : 0];
+          for (int j = 0; j < 32; ++j) v[j] = acc[gi][c + j];
         } else {
           tmem_ld32(tq + static_cast<uint32_t>(b * BN + cb[gi] + c), v);
         }
@@ -536,13 +625,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_block_gemm(const __grid_constan
         get(gi, c, v);
         if (kDual) get(1, c, w);
         const int col = col_of(i);
-        if (EPI == E_PARTIAL) {
+        if constexpr (EPI == E_PARTIAL) {
           if (col >= p.N || row0 >= p.M) return;
           Turned<float> o;
           o.turn(st, lane, v);
           float *dst = p.e.part + (static_cast<size_t>(t.batch) * p.splits + t.split) * p.M * p.e.nacc +
                        (p.dual ? h * p.N : 0);
-          block_store<float>(o, dst, p.e.nacc, p.e.vout, lane, row0, col, p.M, p.N);
+          block_store<float>(o, dst, p.e.nacc, p.e.vout, st, lane, row0, col, p.M, p.N);
         } else {
           const Input<T> cur = next;
           if (kIn && p.e.in && i + 32 < kCols) next.fetch(p, lane, row0, col_of(i + 32));
@@ -556,8 +645,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block_gemm(const __grid_constan
       } else {
 #pragma unroll 1
         for (int i = 0; i < kCols; i += 32) chunk(i);
-        tc_fence_before();
-        mbar_arrive(acce0 + 8 * b);
+        release(b);
       }
     }
   }
@@ -565,18 +653,31 @@ __global__ void __launch_bounds__(kThreads, 1) k_block_gemm(const __grid_constan
   tc_fence_before();
   __syncthreads();
   if (*abort_flag) {
-    // this CTA's own loads and MMAs complete before it ends
-    if (warp == 0 && lane == 0)
+    // this CTA's own loads and MMAs complete before it ends; a pair's loads
+    // report to the leader's barriers, so both CTAs allow them 10 ms instead
+    if (PAIR) {
+      const uint64_t t0 = globaltimer();
+      while (tid == 0 && globaltimer() - t0 < 10000000ull) {
+      }
+    } else if (warp == 0 && issued) {
       for (int j = issued > C::Stages ? issued - C::Stages : 0; j < issued; ++j)
         wait_bounded(full0 + 8 * (j % C::Stages), (j / C::Stages) & 1);
-    if (warp == 1 && lane == 0) {
-      mma_commit(drain);
+    }
+    if (warp == 1 && rank == 0 && elect_one()) {
+      if (PAIR) mma_commit_pair(drain);
+      else mma_commit(drain);
       wait_bounded(drain, 0);
     }
     __syncthreads();
     if (tid == 0) atomicExch(&g_block_err, 1);
   }
-  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  if (PAIR) {
+    cluster_sync();  // neither CTA leaves while the other may still signal it
+    tc_fence_after();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  } else if (warp == 1) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
 }
 
 // Sums the partial products of a split launch in order and runs the epilogue.
@@ -926,21 +1027,48 @@ struct Product {
   EpiArgs e{};
 };
 
-template <bool F32, int BN, int EPI, typename T>
+template <bool F32, int BN, bool PAIR, int EPI, typename T>
 void launch(const Maps &maps, const Params &p, cudaStream_t s) {
-  constexpr int smem = Cfg<F32, BN>::Smem;
-  CUDA_CHECK(cudaFuncSetAttribute(k_block_gemm<F32, BN, EPI, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  constexpr int smem = Cfg<F32, BN, PAIR>::Smem;
+  auto *kernel = k_block_gemm<F32, BN, PAIR, EPI, T>;
+  CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   const int items = p.batch * p.splits * p.tiles_m * p.tiles_n;
-  k_block_gemm<F32, BN, EPI, T><<<std::min(items, sm_count()), kThreads, smem, s>>>(maps, p);
-  CUDA_LAUNCH_CHECK();
+  if (!PAIR) {
+    kernel<<<std::min(items, sm_count()), kThreads, smem, s>>>(maps, p);
+    CUDA_LAUNCH_CHECK();
+    return;
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * std::min(items, sm_count() / 2));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, maps, p));
+  ::pet::g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
+}
+// How a product is tiled.
+struct Tiling {
+  int bn;
+  bool pair;
+};
+template <int EPI, typename T>
+void launch_16(Tiling t, const Maps &maps, const Params &p, cudaStream_t s) {
+  if (t.pair) launch<false, 256, true, EPI, T>(maps, p, s);
+  else if (t.bn == 256) launch<false, 256, false, EPI, T>(maps, p, s);
+  else launch<false, 128, false, EPI, T>(maps, p, s);
 }
 template <int EPI>
-void launch_epi(int dt, int bn, const Maps &maps, const Params &p, cudaStream_t s) {
-  if (dt == DT_F32) launch<true, 128, EPI, float>(maps, p, s);
-  else if (dt == DT_F16 && bn == 256) launch<false, 256, EPI, __half>(maps, p, s);
-  else if (dt == DT_F16) launch<false, 128, EPI, __half>(maps, p, s);
-  else if (bn == 256) launch<false, 256, EPI, __nv_bfloat16>(maps, p, s);
-  else launch<false, 128, EPI, __nv_bfloat16>(maps, p, s);
+void launch_epi(int dt, Tiling t, const Maps &maps, const Params &p, cudaStream_t s) {
+  if (dt == DT_F16) launch_16<EPI, __half>(t, maps, p, s);
+  else if (dt == DT_BF16) launch_16<EPI, __nv_bfloat16>(t, maps, p, s);
+  else launch<true, 128, false, EPI, float>(maps, p, s);
 }
 template <int EPI>
 void join_epi(int dt, const Params &p, cudaStream_t s) {
@@ -968,22 +1096,35 @@ void run(const Product &g, Workspace &ws, cudaStream_t s) {
   p.products = g.products;
   p.e = g.e;
   p.e.dt = g.dt;
-  auto count = [&](int bn) {
-    const int64_t tn = (g.N + (g.dual ? bn / 2 : bn) - 1) / (g.dual ? bn / 2 : bn);
-    return (g.M + BM - 1) / BM * tn * p.batch;
+  // tiles of bm rows of `bn` accumulator columns
+  auto count = [&](int bm, int bn) {
+    const int on = g.dual ? bn / 2 : bn;
+    return (g.M + bm - 1) / bm * ((g.N + on - 1) / on) * p.batch;
   };
-  // tiles of 256 columns need less shared-memory traffic for a product
-  // (128-wide ones take 0.6 of their time each, not half), but come in
-  // coarser waves: whichever finishes first
-  auto waves = [&](int bn) { return static_cast<double>((count(bn) + sms - 1) / sms); };
-  const int bn = !f32 && waves(256) <= 0.6 * waves(128) ? 256 : 128;
-  const int64_t tiles = count(bn);
-  p.tiles_m = static_cast<int>((g.M + BM - 1) / BM);
+  // f32 takes 128 x 128 tiles of one SM (256-wide ones leave no registers for
+  // the epilogue beside the running sums).  16-bit: time in waves over the
+  // SMs, in units of one SM's 128 x 256 tile; a pair's 256 x 256 tile takes
+  // kPair of one, a 128-wide one kNarrow, not half (it needs more
+  // shared-memory traffic for a product).  Measured in bf16: 8192 x 1024 x 8192
+  // in 100 (pair), 107 and 145 us, 1024 x 4096 x 8192 in 56, 59 and 76.
+  constexpr double kPair = 0.93, kNarrow = 0.66;
+  auto waves = [&](int64_t tiles, int at_once) { return static_cast<double>((tiles + at_once - 1) / at_once); };
+  Tiling tile{128, false};
+  if (!f32) {
+    const double narrow = kNarrow * waves(count(BM, 128), sms), wide = waves(count(BM, 256), sms),
+                 pair = kPair * waves(count(2 * BM, 256), sms / 2);
+    if (g.M > BM && pair < narrow && pair < wide) tile = {256, true};
+    else if (wide < narrow) tile = {256, false};
+  }
+  const int bm = tile.pair ? 2 * BM : BM, bn = tile.bn;
+  const int64_t tiles = count(bm, bn);
+  p.tiles_m = static_cast<int>((g.M + bm - 1) / bm);
   p.tiles_n = static_cast<int>(tiles / p.tiles_m / p.batch);
   // few tiles and a long contraction: divided over the SMs, at least four k
   // tiles each
+  const int at_once = tile.pair ? sms / 2 : sms;
   int splits = 1;
-  if (tiles * 2 <= sms && p.kt >= 8) splits = static_cast<int>(std::min<int64_t>(sms / tiles, p.kt / 4));
+  if (tiles * 2 <= at_once && p.kt >= 8) splits = static_cast<int>(std::min<int64_t>(at_once / tiles, p.kt / 4));
   p.kt_split = (p.kt + splits - 1) / splits;
   p.kt_split = (p.kt_split + unit - 1) / unit * unit;
   p.splits = splits = (p.kt + p.kt_split - 1) / p.kt_split;
@@ -1003,7 +1144,7 @@ void run(const Product &g, Workspace &ws, cudaStream_t s) {
   for (int i = 0; i < 2; ++i) {
     const Operand &a = g.a[i].p ? g.a[i] : g.a[0], &b = g.b[i].p ? g.b[i] : g.b[0];
     maps.a[i] = map_of(a, bf, g.a_mn ? 64 : BM);
-    maps.b[i] = map_of(b, bf, g.b_mn ? 64 : bn / 2);
+    maps.b[i] = map_of(b, bf, g.b_mn ? 64 : (tile.pair ? bn / 4 : bn / 2));
     q.sc[i] = a.sc;
     q.scld[i] = a.scld;
     q.bs[i] = b.sc;
@@ -1012,7 +1153,7 @@ void run(const Product &g, Workspace &ws, cudaStream_t s) {
     q.bsc[i] = b.bsc;
   }
   if (splits > 1) {
-    launch_epi<E_PARTIAL>(g.dt, bn, maps, q, s);
+    launch_epi<E_PARTIAL>(g.dt, tile, maps, q, s);
     switch (g.epi) {
       case E_LINEAR: join_epi<E_LINEAR>(g.dt, p, s); break;
       case E_LINEAR_BWD: join_epi<E_LINEAR_BWD>(g.dt, p, s); break;
@@ -1022,10 +1163,10 @@ void run(const Product &g, Workspace &ws, cudaStream_t s) {
     return;
   }
   switch (g.epi) {
-    case E_LINEAR: launch_epi<E_LINEAR>(g.dt, bn, maps, q, s); break;
-    case E_LINEAR_BWD: launch_epi<E_LINEAR_BWD>(g.dt, bn, maps, q, s); break;
-    case E_GATED: launch_epi<E_GATED>(g.dt, bn, maps, q, s); break;
-    default: launch_epi<E_GATED_BWD>(g.dt, bn, maps, q, s); break;
+    case E_LINEAR: launch_epi<E_LINEAR>(g.dt, tile, maps, q, s); break;
+    case E_LINEAR_BWD: launch_epi<E_LINEAR_BWD>(g.dt, tile, maps, q, s); break;
+    case E_GATED: launch_epi<E_GATED>(g.dt, tile, maps, q, s); break;
+    default: launch_epi<E_GATED_BWD>(g.dt, tile, maps, q, s); break;
   }
 }
 

@@ -16,7 +16,7 @@ namespace blk {
 
 namespace {
 
-constexpr int kDepth = 4;  // 16-byte loads in flight per lane and weight
+constexpr int kDepth = 4;  // loads in flight per lane and weight (8 cost more in resident warps)
 
 template <typename T, int MR, bool DUAL, bool VEC>
 __global__ void __launch_bounds__(256) k_few_rows(const FewRows a, int wpr) {
@@ -124,9 +124,10 @@ void launch_rows(const FewRows &a, cudaStream_t s) {
   const bool vec = a.K % V == 0 && rows16(a.x, a.ldx, a.dt) && rows16(a.w0, a.ldw0, a.dt) &&
                    (!DUAL || rows16(a.w1, a.ldw1, a.dt));
   // warps per output feature: enough of them for every SM to have 16, as
-  // long as each still has a full load of its own
+  // long as each has a full load of its own
   int wpr = 1;
-  while (wpr < 8 && a.N * wpr < 16LL * sm_count() && a.K > 64LL * wpr * (vec ? V : 1)) wpr *= 2;
+  const int64_t step = 32LL * (vec ? V : 1);
+  while (wpr < 8 && a.N * wpr < 16LL * sm_count() && a.K > 2 * step * wpr) wpr *= 2;
   const unsigned grid = static_cast<unsigned>((a.N + 8 / wpr - 1) / (8 / wpr));
   if (vec) k_few_rows<T, MR, DUAL, true><<<grid, 256, 0, s>>>(a, wpr);
   else k_few_rows<T, MR, DUAL, false><<<grid, 256, 0, s>>>(a, wpr);

@@ -109,15 +109,19 @@ def _call(name: str, args: bytes, index: int, backward: bool):
 _FORMS: dict = {}
 
 
-def _recorded(*tensors) -> bool:
-    return any(t is not None and t.requires_grad for t in tensors)
+def _wants(t) -> bool:
+    return t is not None and t.requires_grad
+
+
+def _result(x, m: int, n: int):
+    """Uninitialised [..., n] of x's rows, type and device."""
+    return x.new_empty((m, n) if x.dim() == 2 else x.shape[:-1] + (n,))
 
 
 def _grads(inputs, needs):
     """Uninitialised gradients of the inputs that are there and needed, and
     their addresses."""
-    out = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and need else None
-                for t, need in zip(inputs, needs))
+    out = tuple([t.new_empty(t.shape) if t is not None and need else None for t, need in zip(inputs, needs)])
     return out, [0 if t is None else t.data_ptr() for t in out]
 
 
@@ -159,11 +163,12 @@ def gated_linear(x, w_gate, w_value, b_gate=None, b_value=None, activation="silu
     """act(x w_gate^T + b_gate) * (x w_value^T + b_value): x [..., K], weights
     [F, K], biases [F] -> [..., F].  Both projections, the activation and the
     product are one kernel."""
-    if torch.is_grad_enabled() and _recorded(x, w_gate, w_value, b_gate, b_value):
+    if ((x.requires_grad or w_gate.requires_grad or w_value.requires_grad or _wants(b_gate) or _wants(b_value))
+            and torch.is_grad_enabled()):
         return _GatedLinear.apply(x, w_gate, w_value, b_gate, b_value, activation)
     keep: list = []
     m, k, f, fields = _gated_inputs(x, w_gate, w_value, b_gate, b_value, activation, keep)
-    h = torch.empty(x.shape[:-1] + (f,), dtype=x.dtype, device=x.device)
+    h = _result(x, m, f)
     _call("gated_linear", _GATED.pack(*fields, h.data_ptr(), f, 0, f, 0, 0, 0, 0, 0, k, k, k), x.get_device(), False)
     return h
 
@@ -194,7 +199,7 @@ def _linear_inputs(x, w, bias, activation, residual, scale, keep):
     px, lx = _take(x, x, x.shape, k, keep, "x")
     pw, lw = _take(w, x, w.shape, k, keep, "w")
     pb, _ = _take(bias, x, (n,), n, keep, "bias")
-    pr, lr = _take(residual, x, x.shape[:-1] + (n,), n, keep, "residual")
+    pr, lr = (0, n) if residual is None else _take(residual, x, x.shape[:-1] + (n,), n, keep, "residual")
     m = x.numel() // k
     return m, k, n, (dt, act, m, k, n, scale, px, pw, pb, pr, lx, lw, lr)
 
@@ -216,11 +221,11 @@ class _Linear(torch.autograd.Function):
 def linear(x, w, bias=None, activation="identity", residual=None, scale=1.0):
     """residual + scale act(x w^T + bias): x [..., K], w [N, K], bias [N],
     residual [..., N] -> [..., N], in one kernel."""
-    if torch.is_grad_enabled() and _recorded(x, w, bias, residual):
+    if ((x.requires_grad or w.requires_grad or _wants(bias) or _wants(residual)) and torch.is_grad_enabled()):
         return _Linear.apply(x, w, bias, activation, residual, scale)
     keep: list = []
     m, k, n, fields = _linear_inputs(x, w, bias, activation, residual, scale, keep)
-    y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
+    y = _result(x, m, n)
     _call("linear", _LINEAR.pack(*fields, y.data_ptr(), n, 0, n, 0, 0, 0, k, k), x.get_device(), False)
     return y
 
@@ -253,8 +258,9 @@ def _norm_inputs(residual, y, weight, bias, post_weight, post_bias, gate, scale,
         _refuse("a post norm or a gate needs y")
     pr, lr = _take(residual, residual, shape, d, keep, "residual")
     py, ly = _take(y, residual, shape, d, keep, "y")
-    vec = [_take(t, residual, (d,), d, keep, name)[0]
-           for name, t in (("weight", weight), ("bias", bias), ("post_weight", post_weight), ("post_bias", post_bias))]
+    vec = (_take(weight, residual, (d,), d, keep, "weight")[0], _take(bias, residual, (d,), d, keep, "bias")[0],
+           _take(post_weight, residual, (d,), d, keep, "post_weight")[0],
+           _take(post_bias, residual, (d,), d, keep, "post_bias")[0])
     channel = gate is not None and gate.dim() == 1
     pg, lg = _take(gate, residual, (d,) if channel else shape, d, keep, "gate")
     if channel or gate is None:
@@ -285,13 +291,13 @@ def residual_norm(residual, y=None, weight=None, bias=None, post_weight=None, po
     norm(stream), over the last dimension (at most 16384): norms "none", "rms"
     or "layer" with optional weight and bias, a gate [d] for all rows or one
     of the residual's shape.  y None: stream = scale residual."""
-    if torch.is_grad_enabled() and _recorded(residual, y, weight, bias, post_weight, post_bias, gate):
+    if ((residual.requires_grad or _wants(y) or _wants(weight) or _wants(bias) or _wants(post_weight)
+            or _wants(post_bias) or _wants(gate)) and torch.is_grad_enabled()):
         return _ResidualNorm.apply(residual, y, weight, bias, post_weight, post_bias, gate, scale, norm, post_norm,
                                    eps)
     keep: list = []
     d, fields = _norm_inputs(residual, y, weight, bias, post_weight, post_bias, gate, scale, norm, post_norm, eps, keep)
-    stream = torch.empty(residual.shape, dtype=residual.dtype, device=residual.device)
-    out = torch.empty_like(stream)
+    stream, out = residual.new_empty(residual.shape), residual.new_empty(residual.shape)
     _call("residual_norm", _NORM.pack(*fields, stream.data_ptr(), out.data_ptr(), d, d, 0, 0, d, d,
                                       0, 0, 0, 0, 0, 0, 0, d, d, d), residual.get_device(), False)
     return stream, out

@@ -101,7 +101,8 @@ def d_of(*ts):
 # (rows, in, out): one row, the few-row kernel and its end, one past a tile,
 # odd sizes, widths of one, several tiles of every kind
 SHAPES = [(1, 64, 64), (1, 1, 1), (3, 257, 130), (8, 1000, 96), (9, 64, 64), (31, 129, 65), (128, 128, 128),
-          (129, 192, 257), (200, 1, 7), (257, 333, 1), (300, 2050, 136), (1000, 512, 520)]
+          (129, 192, 257), (200, 1, 7), (257, 333, 1), (300, 2050, 136), (1000, 512, 520), (4101, 136, 1100),
+          (2500, 1030, 600)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
