@@ -69,6 +69,7 @@ struct GatedLinear {
     int scale = 0;
   } wg_split, wv_split;
   int products = 3;
+  int *err = nullptr;  // device error word (null: the one of block_status)
 };
 void gated_linear_fwd(const GatedLinear &a, Workspace &ws, cudaStream_t s);
 void gated_linear_bwd(const GatedLinear &a, Workspace &ws, cudaStream_t s);

@@ -101,6 +101,7 @@ struct Params {
   int kt0, kt;                     // k tiles of the first pair of operands, of all
   int tiles_m, tiles_n, splits, kt_split, batch;
   int a_mn, b_mn, dual, bf16, products;
+  int *err;                        // error word, or null for the file's own
   const int8_t *sc[2];             // f32: scale exponents of A, [block][row]
   int64_t scld[2];
   const int8_t *bs[2];             // f32: scale exponents of B's blocks, or null
@@ -669,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block_gemm(const __grid_constan
       wait_bounded(drain, 0);
     }
     __syncthreads();
-    if (tid == 0) atomicExch(&g_block_err, 1);
+    if (tid == 0) atomicExch(p.err ? p.err : &g_block_err, 1);
   }
   if (PAIR) {
     cluster_sync();  // neither CTA leaves while the other may still signal it
@@ -1021,6 +1022,7 @@ CUtensorMap map_of(const Operand &o, bool bf16, int box_rows) {
 
 struct Product {
   int dt = DT_F32, epi = E_LINEAR, products = 3;
+  int *err = nullptr;
   int64_t M = 0, N = 0, K = 0;  // K: contraction of each pair of operands
   Operand a[2], b[2];
   bool a_mn = false, b_mn = false, dual = false, kcat = false, batch2 = false;
@@ -1094,6 +1096,7 @@ void run(const Product &g, Workspace &ws, cudaStream_t s) {
   p.dual = g.dual;
   p.bf16 = g.dt == DT_BF16;
   p.products = g.products;
+  p.err = g.err;
   p.e = g.e;
   p.e.dt = g.dt;
   // tiles of bm rows of `bn` accumulator columns
@@ -1260,6 +1263,7 @@ void gated_linear_fwd(const GatedLinear &a, Workspace &ws, cudaStream_t s) {
   g.dt = a.dtype;
   g.epi = E_GATED;
   g.products = a.products;
+  g.err = a.err;
   g.M = a.M;
   g.N = a.F;
   g.K = a.K;
@@ -1302,6 +1306,7 @@ void gated_linear_bwd(const GatedLinear &a, Workspace &ws, cudaStream_t s) {
   Product g;
   g.dt = a.dtype;
   g.products = a.products;
+  g.err = a.err;
   g.a[0] = a.x_split ? from_split(*a.x_split) : prep.add(a.x, a.M, a.K, FORM_ROWS);
   if (weights) xb = f32 ? prep.add(a.x, a.M, a.K, FORM_BLOCKS) : g.a[0];
   g.epi = E_GATED_BWD;
@@ -1336,6 +1341,7 @@ void gated_linear_bwd(const GatedLinear &a, Workspace &ws, cudaStream_t s) {
     Product q;
     q.dt = a.dtype;
     q.products = a.products;
+    q.err = a.err;
     q.M = a.M;
     q.N = a.K;
     q.K = a.F;
@@ -1352,6 +1358,7 @@ void gated_linear_bwd(const GatedLinear &a, Workspace &ws, cudaStream_t s) {
     Product q;
     q.dt = a.dtype;
     q.products = a.products;
+    q.err = a.err;
     q.M = a.F;
     q.N = a.K;
     q.K = a.M;

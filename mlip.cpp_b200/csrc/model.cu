@@ -11,7 +11,9 @@
 // LN-normalised inputs and 1/sigma of both layer norms, the FFN
 // pre-activation [T,f]; per GNN layer the compress pre-activation [E,H] and
 // the readout pre-activations.  Nothing else: no dW is needed, so GEMM
-// inputs of linear layers are never kept.
+// inputs of linear layers are never kept.  Pre-norm models keep QKV and the
+// stream at each norm; their norms and gated projections (block.h) are
+// recomputed.
 #include "model.h"
 
 #include <algorithm>
@@ -21,6 +23,7 @@
 
 #include <cuda_fp16.h>
 
+#include "block.h"
 #include "gemm_tc.cuh"
 #include "gguf.h"
 #include "kernels.cuh"
@@ -172,7 +175,7 @@ const float *PETModel::w(const std::string &name) const {
 const float *PETModel::device_forces() const { return in_->a.F; }
 
 size_t PETModel::device_bytes() const {
-  return wbuf_.cap + persist_.cap + scratch_.cap + sp_[0].cap + sp_[1].cap + sp_[2].cap + nl_.center.cap * 10;
+  return wbuf_.cap + persist_.cap + scratch_.cap + opws_.cap + sp_[0].cap + sp_[1].cap + sp_[2].cap + nl_.center.cap * 10;
 }
 
 // ---------------------------------------------------------------------------
@@ -232,8 +235,39 @@ void PETModel::load(const std::string &path, float cutoff_override) {
   const auto *c0 = f.tensor("model.gnn.0.compress.0.weight");
   if (!c0) throw Error(kErrIO, "Required tensor 'model.gnn.0.compress.0.weight' not found");
   h.hid = static_cast<int>(c0->ne[1]);
+  // Pre-norm blocks (x + attn(norm_a(x)), then x + mlp(norm_m(x))) with a
+  // gated feed-forward part: mlp.0 holds the gate's rows, then the value's,
+  // and mlp(v) = mlp.3 (silu(gate v) * (value v)); their norms divide by
+  // sqrt(var + eps) or, RMS norms, sqrt(mean square + eps).  The reference's
+  // files carry none of these keys.
+  {
+    const std::string type = f.get_string("pet.transformer_type", "postln"),
+                      act = f.get_string("pet.activation", "silu"),
+                      norm = f.get_string("pet.normalization", "layernorm");
+    h.prenorm = type == "preln";
+    h.norm = norm == "rmsnorm" ? NORM_RMS : NORM_LAYER;
+    h.norm_eps = f.get_f32("pet.norm_eps", 1e-5f);
+    const bool plain = type == "postln" && act == "silu" && norm == "layernorm";
+    const bool gated = h.prenorm && act == "swiglu" && (norm == "rmsnorm" || norm == "layernorm");
+    if (!plain && !gated)
+      throw Error(kErrUnsupported, "transformer type '" + type + "' with activation '" + act + "' and normalization '" +
+                                       norm + "' is not supported (postln with silu and layernorm, or preln with "
+                                       "swiglu and layernorm or rmsnorm)");
+    if (!std::isfinite(h.norm_eps) || h.norm_eps <= 0.0f) throw Error(kErrIO, "pet.norm_eps must be finite and positive");
+  }
   const auto *w0 = f.tensor("model.gnn.0.tl.0.mlp.0.weight");
-  if (w0) h.ff = static_cast<int>(w0->ne[1]);
+  if (w0) h.ff = static_cast<int>(w0->ne[1]) / (h.prenorm ? 2 : 1);
+  if (h.prenorm) {
+    for (int l = 0; l < 2; ++l)
+      for (int t = 0; t < 2; ++t) {
+        const std::string q = "model.gnn." + std::to_string(l) + ".tl." + std::to_string(t) + ".mlp.";
+        const auto *w = f.tensor(q + "0.weight"), *b = f.tensor(q + "0.bias"), *o = f.tensor(q + "3.weight");
+        if (!w || !b || !o || w->type != 0 || w->ne.size() != 2 || w->ne[0] != h.d || w->ne[1] != 2 * h.ff ||
+            b->numel() != 2 * h.ff || o->ne.size() != 2 || o->ne[0] != h.ff || o->ne[1] != h.d)
+          throw Error(kErrIO, "gated feed-forward tensors '" + q + "*' are missing or of an unexpected shape");
+      }
+    if (h.d > kMaxNormDim) throw Error(kErrUnsupported, "pre-norm models support d_pet up to " + std::to_string(kMaxNormDim));
+  }
   const auto *hd = f.tensor("model.node_heads.energy.0.0.weight");
   if (hd) h.dh = static_cast<int>(hd->ne[1]);
 
@@ -265,7 +299,7 @@ void PETModel::load(const std::string &path, float cutoff_override) {
       const std::string q = p + "tl." + std::to_string(t) + ".";
       transpose_of(q + "attn.in.weight");
       transpose_of(q + "attn.out.weight");
-      transpose_of(q + "mlp.0.weight");
+      if (!h.prenorm) transpose_of(q + "mlp.0.weight");
       transpose_of(q + "mlp.3.weight");
     }
     for (const char *kind : {"node", "edge"}) {
@@ -385,7 +419,7 @@ void PETModel::load(const std::string &path, float cutoff_override) {
     chain_ok_ = use_f16_ && m128 && 3 * h.d <= 2048 && h.ff <= 2048 && h.hid <= 2048 && h.d <= 1024 &&
                 hd > 0 && 128 % hd == 0 && h.heads % (128 / hd) == 0;
     const char *c = std::getenv("MLIPCPP_B200_CHAIN");
-    if (c && std::string(c) == "0") chain_ok_ = false;
+    if ((c && std::string(c) == "0") || h.prenorm) chain_ok_ = false;
   }
 
   // composition map and species index (pet.cpp:1280-1303)
@@ -427,12 +461,17 @@ void PETModel::load(const std::string &path, float cutoff_override) {
       BlockW &B = L.blk[t];
       B.Win = w(q + "attn.in.weight"); B.bin = w(q + "attn.in.bias");
       B.Wout = w(q + "attn.out.weight"); B.bout = w(q + "attn.out.bias");
-      B.ga = w(q + "norm_a.weight"); B.ba = w(q + "norm_a.bias");
-      B.gm = w(q + "norm_m.weight"); B.bm = w(q + "norm_m.bias");
+      B.ga = w(q + "norm_a.weight");
+      B.gm = w(q + "norm_m.weight");
+      // RMS norms need no shift
+      auto shift = [&](const std::string &name) -> const float * {
+        return h.prenorm && !f.tensor(name) ? nullptr : w(name);
+      };
+      B.ba = shift(q + "norm_a.bias"); B.bm = shift(q + "norm_m.bias");
       B.W0 = w(q + "mlp.0.weight"); B.b0 = w(q + "mlp.0.bias");
       B.W3 = w(q + "mlp.3.weight"); B.b3 = w(q + "mlp.3.bias");
       B.WinT = w(q + "attn.in.weight.T"); B.WoutT = w(q + "attn.out.weight.T");
-      B.W0T = w(q + "mlp.0.weight.T"); B.W3T = w(q + "mlp.3.weight.T");
+      B.W0T = h.prenorm ? nullptr : w(q + "mlp.0.weight.T"); B.W3T = w(q + "mlp.3.weight.T");
     }
     for (int k = 0; k < 2; ++k) {
       const std::string kind = k == 0 ? "node" : "edge";
@@ -513,9 +552,11 @@ static void plan_memory(Plan &P, Plan &S, Acts &a, const Hypers &h, const Counts
     a.lse[b] = P.take<float>(T * h.heads);
     // LN inputs (the residual sums) and their per-row mean and 1 / sd,
     // from which the backward recomputes the normalised rows
-    a.xa[b] = P.take<float>(T * d); a.ra[b] = P.take<float>(2 * T);
-    a.zf[b] = P.take<float>(T * f);
-    a.xm[b] = P.take<float>(T * d); a.rm[b] = P.take<float>(2 * T);
+    // (pre-norm: the stream at each norm; everything else is recomputed)
+    const bool post = !h.prenorm;
+    a.xa[b] = P.take<float>(T * d); a.ra[b] = post ? P.take<float>(2 * T) : nullptr;
+    a.zf[b] = post ? P.take<float>(T * f) : nullptr;
+    a.xm[b] = P.take<float>(T * d); a.rm[b] = post ? P.take<float>(2 * T) : nullptr;
   }
   for (int l = 0; l < 2; ++l) {
     a.zc[l] = P.take<float>((l == 0 ? E0 : E1) * H);
@@ -688,6 +729,83 @@ void PETModel::forward_backward(bool grad) {
     if (ch && sout) *sout = take_split(T, d);
     layer_norm_fwd(a.xm[b], B.gm, B.bm, out, a.rm[b], T, d, s, ch ? sout : nullptr);
   };
+  // The block's norm (attention's or the feed-forward part's) of a pre-norm
+  // model, and its feed-forward projection, on T rows.
+  auto norm_of = [&](const float *g, const float *b) {
+    ResidualNorm n;
+    n.norm = h.norm;
+    n.eps = h.norm_eps;
+    n.M = T;
+    n.d = d;
+    n.w = g;
+    n.b = b;
+    return n;
+  };
+  auto block_ws = [&]() {
+    Workspace ws;
+    ws.base = opws_.as<char>();
+    ws.cap = opws_.cap;
+    return ws;
+  };
+  auto gated_of = [&](const BlockW &B, const float *v) {
+    const float *wb = wbuf_.as<float>();
+    const uint16_t *h16 = reinterpret_cast<const uint16_t *>(wb + 3 * wspan_);
+    const size_t off = static_cast<size_t>(B.W0 - wb), half = static_cast<size_t>(f) * d;
+    GatedLinear g;
+    g.M = T;
+    g.K = d;
+    g.F = f;
+    g.x = {v, d};
+    g.wg = {B.W0, d};
+    g.wv = {B.W0 + half, d};
+    g.bg = B.b0;
+    g.bv = B.b0 + f;
+    if (half % 8 == 0 && d % 8 == 0) {  // the split copies, where TMA can read them
+      const int sc = weight_scale(off);
+      g.wg_split = {h16 + off, h16 + wspan_ + off, sc};
+      g.wv_split = {h16 + off + half, h16 + wspan_ + off + half, sc};
+    }
+    g.products = reduced_ ? 1 : 3;
+    g.err = d_err_.as<int>();
+    return g;
+  };
+  // the products of a gated projection, for the profile
+  auto gated_run = [&](const GatedLinear &g, bool backward) {
+    cudaEvent_t e0 = nullptr;
+    if (kprof_) mark_begin(e0);
+    Workspace ws = block_ws();
+    if (backward) gated_linear_bwd(g, ws, s);
+    else gated_linear_fwd(g, ws, s);
+    if (kprof_)
+      mark_end(KC_GEMM_F16, e0, (backward ? 8.0 : 4.0) * T * d * f,
+               4.0 * (static_cast<double>(T) * ((backward ? 2 : 1) * d + f) + 2.0 * d * f));
+  };
+  // Pre-norm block b on the stream a.xa[b]; the stream after it goes to out.
+  auto block_pre = [&](int b, float *out) {
+    const BlockW &B = g_lw[b / 2].blk[b % 2];
+    Workspace ws = block_ws();
+    const float *x = a.xa[b];
+    ResidualNorm n = norm_of(B.ga, B.ba);
+    n.residual = {x, d};
+    n.out = {a.x1, d};
+    residual_norm_fwd(n, ws, s);
+    gemm(a.x1, d, nullptr, B.Win, d, a.qkv[b], 3 * d, nullptr, T, 3 * d, d, B.bin, EPI_STORE, s);
+    at.qkv = a.qkv[b];
+    at.lse = a.lse[b];
+    at.out = a.o;
+    attn(false, at);
+    gemm(a.o, d, nullptr, B.Wout, d, a.xmid, d, nullptr, T, d, d, B.bout, EPI_STORE, s);
+    n = norm_of(B.gm, B.bm);
+    n.residual = {x, d};
+    n.y = {a.xmid, d};
+    n.stream = {a.xm[b], d};
+    n.out = {a.x1, d};
+    residual_norm_fwd(n, ws, s);
+    GatedLinear g = gated_of(B, a.x1);
+    g.h = {a.hf, f};
+    gated_run(g, false);
+    gemm(a.hf, f, nullptr, B.W3, f, out, d, nullptr, T, d, f, B.b3, EPI_RESID, s, nullptr, 0, a.xm[b], d);
+  };
   // Energy head (node or edge) on rows [row0, row0 + M) of the layer output:
   // x in fp32, or in chain mode its split form sxl (in split buffer fin_sp;
   // the head's hidden layer takes the other buffer).
@@ -718,6 +836,8 @@ void PETModel::forward_backward(bool grad) {
     at.n_atoms = N;
     at.edge_base = N;
     Split16View sx;
+    // the layer's tokens (pre-norm: the stream of its first block)
+    float *const xin = h.prenorm ? a.xa[2 * l] : a.xin;
     // layer-0 tokens of reverse edges held by other domains (collective)
     if (l == 1 && rm_) rm_->exchange_tokens(a.xl[0], Nl_[0], Tl_[0], d, s);
     if (E > 0) {
@@ -743,17 +863,22 @@ void PETModel::forward_backward(bool grad) {
         sx = take_split(T, d);
         sxe = split_rows(sx, N, E);
       }
-      gemm(a.hc, H, nullptr, L.C2, H, ch ? nullptr : a.xin + static_cast<size_t>(N) * d, d, nullptr, E, d, H, L.c2,
+      gemm(a.hc, H, nullptr, L.C2, H, ch ? nullptr : xin + static_cast<size_t>(N) * d, d, nullptr, E, d, H, L.c2,
            EPI_STORE, s, nullptr, 0, nullptr, 0, SplitIO{ch ? &shc : nullptr, true, ch ? &sxe : nullptr});
     } else if (ch) {
       sx = take_split(T, d);
     }
-    node_tokens(L.node_emb, species, ch ? nullptr : a.xin, N, d, s, ch ? &sx : nullptr);
+    node_tokens(L.node_emb, species, ch ? nullptr : xin, N, d, s, ch ? &sx : nullptr);
     Split16View smid;
-    block_fwd(2 * l, a.xin, ch ? &sx : nullptr, ch ? nullptr : a.xmid, ch ? &smid : nullptr);
-    // layer output: fp32 for the next layer's messages (layer 0) and the
-    // fp32 path; in chain mode the readout reads its split form
-    block_fwd(2 * l + 1, a.xmid, ch ? &smid : nullptr, (ch && l > 0) ? nullptr : a.xl[l], ch ? &sxl : nullptr);
+    if (h.prenorm) {
+      block_pre(2 * l, a.xa[2 * l + 1]);
+      block_pre(2 * l + 1, a.xl[l]);
+    } else {
+      block_fwd(2 * l, a.xin, ch ? &sx : nullptr, ch ? nullptr : a.xmid, ch ? &smid : nullptr);
+      // layer output: fp32 for the next layer's messages (layer 0) and the
+      // fp32 path; in chain mode the readout reads its split form
+      block_fwd(2 * l + 1, a.xmid, ch ? &smid : nullptr, (ch && l > 0) ? nullptr : a.xl[l], ch ? &sxl : nullptr);
+    }
     fin_sp = last_sp;
     const float *xo = ch ? nullptr : a.xl[l];
     // readout (pet_layers.cpp:920-1015) of the N1 atoms whose energy counts:
@@ -800,7 +925,44 @@ void PETModel::forward_backward(bool grad) {
   };
   // dxin: the block input's gradient in fp32; in chain mode it goes instead
   // to *sdxin in split form when that is given
+  // Pre-norm block: the stream's gradient dy goes around each part and through
+  // its norm.  The feed-forward part's input is recomputed from the stream.
+  auto block_pre_bwd = [&](int b, const float *dy, float *dxin) {
+    const BlockW &B = g_lw[b / 2].blk[b % 2];
+    Workspace ws = block_ws();
+    gemm(dy, d, nullptr, B.W3T, d, a.dhf, f, nullptr, T, f, d, nullptr, EPI_STORE, s);
+    ResidualNorm n = norm_of(B.gm, B.bm);
+    n.residual = {a.xm[b], d};
+    n.out = {a.dout, d};
+    residual_norm_fwd(n, ws, s);
+    GatedLinear g = gated_of(B, a.dout);
+    g.dh = {a.dhf, f};
+    g.dx = {a.du, d};
+    gated_run(g, true);
+    n.out = {};
+    n.dstream = {dy, d};
+    n.dout = {a.du, d};
+    n.dresidual = {a.dx1, d};
+    residual_norm_bwd(n, ws, s);
+    gemm(a.dx1, d, nullptr, B.WoutT, d, a.dout, d, nullptr, T, d, d, nullptr, EPI_STORE, s);
+    at.qkv = a.qkv[b];
+    at.lse = a.lse[b];
+    at.d_out = a.dout;
+    at.d_qkv = a.dqkv;
+    attn(true, at);
+    gemm(a.dqkv, 3 * d, nullptr, B.WinT, 3 * d, a.du, d, nullptr, T, d, 3 * d, nullptr, EPI_STORE, s);
+    n = norm_of(B.ga, B.ba);
+    n.residual = {a.xa[b], d};
+    n.dstream = {a.dx1, d};
+    n.dout = {a.du, d};
+    n.dresidual = {dxin, d};
+    residual_norm_bwd(n, ws, s);
+  };
   auto block_bwd = [&](int b, const float *dy, float *dxin, const Split16View *sdxin = nullptr) {
+    if (h.prenorm) {
+      block_pre_bwd(b, dy, dxin);
+      return;
+    }
     const BlockW &B = g_lw[b / 2].blk[b % 2];
     Split16View sdu, sdhf, sdu2, sdq;
     if (ch) sdu = take_split(T, d);
@@ -895,7 +1057,7 @@ std::vector<uintptr_t> PETModel::graph_key(bool grad) const {
               (timing_ ? 32u : 0u),
           p(persist_.ptr), p(scratch_.ptr), p(sp_[0].ptr), p(sp_[1].ptr), p(sp_[2].ptr), p(wbuf_.ptr),
           p(nl_.offset.ptr), p(nl_.center.ptr), p(nl_.nbr.ptr), p(nl_.shift.ptr), p(nl_.vec.ptr), p(nl_.dist.ptr),
-          p(species_), p(d_err_.ptr), static_cast<uintptr_t>(n_short_), p(attn_cls_.ptr)};
+          p(species_), p(d_err_.ptr), static_cast<uintptr_t>(n_short_), p(attn_cls_.ptr), p(opws_.ptr)};
 }
 
 // Phase boundary i of the step's timing.  Inside a capture the record
@@ -1010,6 +1172,24 @@ void PETModel::setup_graph(int n_local, int N0, int E0, int N1, int E1, const in
     if (chain_) sp_[1].ensure(mk * 4 + mk / 128 + 256);
     const size_t md = static_cast<size_t>(std::max(Tl_[0], Tl_[1])) * h_.d;
     if (chain_ && grad) sp_[2].ensure(md * 4 + md / 128 + 256);
+  }
+  if (h_.prenorm) {
+    // working memory of the block operators: the largest of their calls (an
+    // operator sizes by shape; any pointer stands for a wanted gradient)
+    size_t need = 0;
+    for (int l = 0; l < 2; ++l) {
+      float any = 0.f;
+      GatedLinear g;
+      g.M = Tl_[l];
+      g.K = h_.d;
+      g.F = h_.ff;
+      Workspace fw, bw;
+      gated_linear_fwd(g, fw, stream_);
+      g.dx = {&any, h_.d};
+      gated_linear_bwd(g, bw, stream_);
+      need = std::max({need, fw.off, grad ? bw.off : 0});
+    }
+    opws_.ensure(need + 256);
   }
   P = Plan{persist_.as<char>(), 0};
   S = Plan{scratch_.as<char>(), 0};

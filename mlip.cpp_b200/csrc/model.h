@@ -23,6 +23,11 @@ struct Hypers {
   // per embedding row, rounded up to 128): see FeaturizeArgs
   int aux = 128;
   float cutoff = 4.5f, width = 0.5f;
+  // Pre-norm blocks with a gated feed-forward part (no counterpart in the
+  // reference's "pet" layout): the kind of norm (NormKind) and its eps.
+  bool prenorm = false;
+  int norm = 2;
+  float norm_eps = 1e-5f;
 };
 
 // One structure as the C API receives it (host pointers, not owned).
@@ -224,6 +229,7 @@ class PETModel {
   Split16View split_view(int i, int rows, int cols);
   int weight_scale(size_t elem) const;
   DevBuf d_err_;         // device error word written by bounded waits
+  DevBuf opws_;          // working memory of the block operators (pre-norm models)
   std::map<std::string, const float *> wptr_;
   std::map<int, int> species_index_;
   std::map<int, float> composition_;

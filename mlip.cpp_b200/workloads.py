@@ -19,7 +19,7 @@ composition energies ~ N(-3, 1).
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass, asdict
+from dataclasses import dataclass, asdict, replace
 
 import numpy as np
 
@@ -38,6 +38,12 @@ class PETHypers:
     cutoff_width: float = 0.2
     num_gnn_layers: int = 2
     num_attention_layers: int = 2
+    # block form: "postln" with "silu" and "layernorm" (the reference's), or
+    # "preln" with the gated "swiglu" and "layernorm" or "rmsnorm"
+    transformer_type: str = "postln"
+    activation: str = "silu"
+    normalization: str = "layernorm"
+    norm_eps: float = 1e-5
 
 
 #: Stand-in for pet-mad-s (its GGUF is not available): PET-MAD's published
@@ -49,7 +55,11 @@ PET_OAM_L = PETHypers(d_pet=512, num_heads=16, d_feedforward=1024, d_head=256)
 #: Small hypers for fast tests.
 PET_TINY = PETHypers(d_pet=64, num_heads=4, d_feedforward=128, d_head=32)
 
-HYPERS = {"pet-mad-s": PET_MAD_S, "pet-oam-l": PET_OAM_L, "tiny": PET_TINY}
+_GATED = dict(transformer_type="preln", activation="swiglu", normalization="rmsnorm")
+#: The same sizes with pre-norm blocks, RMS norms and gated feed-forward parts.
+HYPERS = {"pet-mad-s": PET_MAD_S, "pet-oam-l": PET_OAM_L, "tiny": PET_TINY,
+          "pet-mad-s-gated": replace(PET_MAD_S, **_GATED), "pet-oam-l-gated": replace(PET_OAM_L, **_GATED),
+          "tiny-gated": replace(PET_TINY, **_GATED)}
 
 
 # --------------------------------------------------------------------------
@@ -79,9 +89,12 @@ def pet_tensor_shapes(h: PETHypers, n_species: int) -> dict[str, tuple[int, ...]
             s[q + "attn.out.bias"] = (d,)
             for nrm in ("norm_a", "norm_m"):
                 s[q + nrm + ".weight"] = (d,)
-                s[q + nrm + ".bias"] = (d,)
-            s[q + "mlp.0.weight"] = (f, d)
-            s[q + "mlp.0.bias"] = (f,)
+                if h.normalization != "rmsnorm":
+                    s[q + nrm + ".bias"] = (d,)
+            # gated: the gate's rows, then the value's
+            f0 = 2 * f if h.activation == "swiglu" else f
+            s[q + "mlp.0.weight"] = (f0, d)
+            s[q + "mlp.0.bias"] = (f0,)
             s[q + "mlp.3.weight"] = (d, f)
             s[q + "mlp.3.bias"] = (d,)
         for kind in ("node", "edge"):
@@ -190,6 +203,11 @@ def write_pet_gguf(path: str, h: PETHypers, atomic_numbers=None, seed: int = 0,
     w.add_int32("pet.num_gnn_layers", int(h.num_gnn_layers))
     w.add_int32("pet.d_feedforward", int(h.d_feedforward))
     w.add_int32("pet.num_attention_layers", int(h.num_attention_layers))
+    if h.transformer_type != "postln":
+        w.add_string("pet.transformer_type", h.transformer_type)
+        w.add_string("pet.activation", h.activation)
+        w.add_string("pet.normalization", h.normalization)
+        w.add_float32("pet.norm_eps", float(h.norm_eps))
     for name, arr in weights.items():
         w.add_tensor(name, arr)
     w.write_header_to_file()
@@ -207,7 +225,8 @@ def read_pet_gguf(path: str) -> tuple[PETHypers, dict[str, np.ndarray]]:
     meta = {}
     for f in r.fields.values():
         if f.name.startswith("pet.") and f.types and len(f.data) == 1:
-            meta[f.name] = f.parts[f.data[0]][0]
+            part = f.parts[f.data[0]]
+            meta[f.name] = bytes(part).decode() if f.types[0] == gguf.GGUFValueType.STRING else part[0]
     tensors = {}
     for t in r.tensors:
         shape = tuple(int(x) for x in reversed(t.shape.tolist()))
@@ -219,6 +238,10 @@ def read_pet_gguf(path: str) -> tuple[PETHypers, dict[str, np.ndarray]]:
         d_head=int(meta.get("pet.d_head", 128)),
         cutoff=float(meta.get("pet.cutoff", 4.5)),
         cutoff_width=float(meta.get("pet.cutoff_width", 0.5)),
+        transformer_type=meta.get("pet.transformer_type", "postln"),
+        activation=meta.get("pet.activation", "silu"),
+        normalization=meta.get("pet.normalization", "layernorm"),
+        norm_eps=float(meta.get("pet.norm_eps", 1e-5)),
     )
     return h, tensors
 

@@ -162,6 +162,14 @@ class PETOracle:
         var = (xc * xc).mean(-1, keepdim=True)
         return xc / torch.sqrt(var * (1.0 + eps)) * w + b
 
+    # Pre-norm models (no counterpart in mlip.cpp): the textbook norms
+    def _norm(self, x, name):
+        w, b = self.W[name + ".weight"], self.W.get(name + ".bias")
+        if self.h.normalization != "rmsnorm":
+            x = x - x.mean(-1, keepdim=True)
+        y = x / torch.sqrt((x * x).mean(-1, keepdim=True) + self.h.norm_eps) * w
+        return y if b is None else y + b
+
     def _lin(self, x, name):
         return x @ self.W[name + ".weight"].T + self.W[name + ".bias"]
 
@@ -207,11 +215,18 @@ class PETOracle:
             S = M + 1
             for t in range(2):
                 q_ = p + f"tl.{t}."
-                qkv = self._lin(x, q_ + "attn.in").reshape(N, S, 3, nh, hd)
+                pre = h.transformer_type == "preln"
+                u = self._norm(x, q_ + "norm_a") if pre else x
+                qkv = self._lin(u, q_ + "attn.in").reshape(N, S, 3, nh, hd)
                 q, k, v = (qkv[:, :, i].transpose(1, 2) for i in range(3))      # [N,nh,S,hd]
                 s = (q @ k.transpose(-1, -2)) * (1.0 / math.sqrt(hd)) + mask
                 a = torch.softmax(s, -1) @ v                                      # [N,nh,S,hd]
                 a = a.transpose(1, 2).reshape(N, S, d)
+                if pre:  # x + attn(norm(x)), then x + mlp(norm(x)) with mlp.0 = [gate; value]
+                    x = x + self._lin(a, q_ + "attn.out")
+                    gate, value = self._lin(self._norm(x, q_ + "norm_m"), q_ + "mlp.0").chunk(2, -1)
+                    x = x + self._lin(torch.nn.functional.silu(gate) * value, q_ + "mlp.3")
+                    continue
                 x = self._ln(x + self._lin(a, q_ + "attn.out"), W[q_ + "norm_a.weight"], W[q_ + "norm_a.bias"])
                 hmid = torch.nn.functional.silu(self._lin(x, q_ + "mlp.0"))
                 x = self._ln(x + self._lin(hmid, q_ + "mlp.3"), W[q_ + "norm_m.weight"], W[q_ + "norm_m.bias"])

@@ -1,0 +1,82 @@
+"""PET models with pre-norm blocks, RMS or layer norms and gated feed-forward
+parts (pet.transformer_type = preln, pet.activation = swiglu): the library
+against the torch oracle, at the tolerances of the post-norm models' parity
+tests (|dE| / N <= 1e-5 eV, |dF| <= 1e-4 eV / A, |dstress| <= 1e-4 eV / A^3)."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+import mlipcpp_b200 as mb  # noqa: E402
+from mlipcpp_b200 import workloads as wl  # noqa: E402
+from oracle import pet_oracle  # noqa: E402
+
+
+def check(got, ref, n, stress=True, tol=(1e-5, 1e-4, 1e-4)):
+    assert abs(got.energy - ref["energy_f64"]) / n <= tol[0]
+    assert np.abs(got.forces - ref["forces"]).max() <= tol[1]
+    if stress:
+        assert np.abs(got.stress - ref["stress"]).max() <= tol[2]
+
+
+@pytest.mark.parametrize("name", ["tiny-gated", "pet-mad-s-gated"])
+@pytest.mark.parametrize("normalization", ["rmsnorm", "layernorm"])
+def test_periodic(model_file, name, normalization):
+    path = model_file(name, normalization=normalization)
+    s = wl.si_diamond(2, seed=3)
+    p = mb.Predictor(path)
+    ref = pet_oracle.load_oracle(path, torch.float64).predict([s])[0]
+    for _ in range(3):  # eager, captured, replayed
+        check(p.predict(s.positions, s.numbers, s.cell, compute_stress=True), ref, s.n_atoms)
+
+
+def test_oam_width(model_file):
+    path = model_file("pet-oam-l-gated")
+    s = wl.si_diamond(1, seed=5)
+    ref = pet_oracle.load_oracle(path, torch.float64).predict([s])[0]
+    check(mb.Predictor(path).predict(s.positions, s.numbers, s.cell, compute_stress=True), ref, s.n_atoms)
+
+
+def test_odd_widths(model_file):
+    """Widths that no tensor-core layer of the model takes: the gated
+    projection pads them."""
+    path = model_file("tiny-gated", d_pet=48, num_heads=3, d_feedforward=50)
+    s = wl.si_diamond(1, seed=2)
+    ref = pet_oracle.load_oracle(path, torch.float64).predict([s])[0]
+    check(mb.Predictor(path).predict(s.positions, s.numbers, s.cell, compute_stress=True), ref, s.n_atoms)
+
+
+def test_molecules_and_single_atom(model_file):
+    """Non-periodic batch, and an atom without neighbours (one token a layer)."""
+    path = model_file("tiny-gated")
+    p, oracle = mb.Predictor(path), pet_oracle.load_oracle(path, torch.float64)
+    systems = wl.molecules(5, seed=1)
+    for got, ref, s in zip(p.predict_batch(systems), oracle.predict(systems), systems):
+        check(got, ref, s.n_atoms, stress=False)
+    r = p.predict(np.zeros((1, 3), np.float32), [14])
+    assert np.isfinite(r.energy) and np.abs(r.forces).max() == 0.0
+
+
+def test_forces_are_the_energy_gradient(model_file):
+    """Central differences of the energy-only path, which skips the backward."""
+    path = model_file("tiny-gated")
+    s = wl.molecules(1, seed=4)[0]
+    p = mb.Predictor(path)
+    f = p.predict(s.positions, s.numbers).forces
+    oracle = pet_oracle.load_oracle(path, torch.float64)
+    batch = pet_oracle.prepare_batch([s], oracle.h.cutoff, oracle.h.cutoff_width, oracle.species_to_index)
+    ref = oracle.predict([s], key_mask=batch.key_mask)[0]["forces"]
+    assert np.abs(f - ref).max() <= 1e-4
+    e = p.predict(s.positions, s.numbers, compute_forces=False).energy
+    assert abs(e - p.predict(s.positions, s.numbers).energy) <= 1e-5 * s.n_atoms
+
+
+def test_reduced_precision(model_file):
+    """The one-product mode's stated tolerances (|dE| / N <= 2e-3, |dF| <= 1e-2)."""
+    path = model_file("pet-mad-s-gated")
+    s = wl.si_diamond(2, seed=3)
+    full = mb.Predictor(path).predict(s.positions, s.numbers, s.cell, compute_stress=True)
+    half = mb.Predictor(path, mb.ModelOptions(precision=1)).predict(s.positions, s.numbers, s.cell, compute_stress=True)
+    assert abs(full.energy - half.energy) / s.n_atoms <= 2e-3
+    assert np.abs(full.forces - half.forces).max() <= 1e-2

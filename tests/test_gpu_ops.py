@@ -433,3 +433,160 @@ def test_gradients_against_differences(dtype):
         # here a sum of independent ones; 8 standard deviations
         sd = 2 * unit(dtype) * (got[i].double().abs() * step.abs()).pow(2).sum().sqrt().item()
         assert abs((got[i].double() * step).sum().item() - diff) <= 8 * sd + 1e-4 * max(1.0, abs(diff)), i
+
+
+def block(x, r, p, backward=None):
+    """norm -> gated projection -> projection onto the stream, through autograd."""
+    stream, u = ops.residual_norm(r, x, p["n"], post_weight=p["pn"], gate=p["g"], post_norm="rms")
+    return ops.linear(ops.gated_linear(u, p["wg"], p["wv"], p["bg"]), p["wo"], p["bo"], residual=stream)
+
+
+def plain_block(x, r, p):
+    def rms(t, w):
+        return t / (t.pow(2).mean(-1, keepdim=True) + 1e-5).sqrt() * w
+    stream = r + p["g"] * rms(x, p["pn"])
+    u = rms(stream, p["n"])
+    h = torch.nn.functional.silu(u @ p["wg"].T + p["bg"]) * (u @ p["wv"].T)
+    return stream + h @ p["wo"].T + p["bo"]
+
+
+def block_inputs(seed, dtype, rows=(2, 75), d=136, f=200):
+    g = gen(seed)
+    p = {"n": rand(g, d, dtype=dtype, std=0.1, mean=1), "pn": rand(g, d, dtype=dtype, std=0.1, mean=1),
+         "g": rand(g, d, dtype=dtype), "wg": rand(g, f, d, dtype=dtype, std=d ** -0.5),
+         "wv": rand(g, f, d, dtype=dtype, std=d ** -0.5), "bg": rand(g, f, dtype=dtype, std=0.1),
+         "wo": rand(g, d, f, dtype=dtype, std=f ** -0.5), "bo": rand(g, d, dtype=dtype, std=0.1)}
+    return rand(g, *rows, d, dtype=dtype), rand(g, *rows, d, dtype=dtype), p
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_block_and_its_gradients(dtype):
+    """The three together, as a block runs them, against float64 autograd.
+    Each of the five roundings between the operators (u, h, out and the
+    gradients of the same) enters every result once, as do the products'
+    own; relative to the largest result, 16 u covers them."""
+    x, r, p = block_inputs(31, dtype)
+    leaves = [t.clone().requires_grad_() for t in (x, r, *p.values())]
+    y = block(leaves[0], leaves[1], dict(zip(p, leaves[2:])))
+    gy = rand(gen(32), *y.shape, dtype=dtype)
+    grads = torch.autograd.grad(y, leaves, gy)
+    exact = [t.double().requires_grad_() for t in (x, r, *p.values())]
+    y64 = plain_block(exact[0], exact[1], dict(zip(p, exact[2:])))
+    ref = torch.autograd.grad(y64, exact, gy.double())
+    tol = 16 * unit(dtype) + 2.0 ** -18
+    for a, b in zip((y, *grads), (y64, *ref)):
+        assert a.dtype == dtype and a.shape == b.shape
+        assert (a.double() - b).norm() <= tol * b.norm()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_graph_capture(dtype):
+    """Forward and backward captured and replayed on new inputs, beside two
+    graphs that share nothing, equal the eager calls bit for bit."""
+    x, r, p = block_inputs(41, dtype, rows=(150,))
+    gy = rand(gen(42), 150, 136, dtype=dtype)
+
+    def step():
+        stream, u = ops.residual_norm(r, x, p["n"], post_weight=p["pn"], gate=p["g"], post_norm="rms")
+        h = ops.gated_linear(u, p["wg"], p["wv"], p["bg"])
+        dh, dwo, dbo = ops.linear_backward(gy, h, p["wo"], p["bo"])
+        du, *dw = ops.gated_linear_backward(dh, u, p["wg"], p["wv"], p["bg"])
+        g = ops.residual_norm_backward(gy, du, r, x, p["n"], post_weight=p["pn"], gate=p["g"], post_norm="rms")
+        return [stream, u, h, dwo, dbo, *[t for t in dw if t is not None], *[t for t in g if t is not None]]
+
+    step()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step()
+        graphs.append((g, out))
+    for seed in (43, 44):
+        nx, nr, _ = block_inputs(seed, dtype, rows=(150,))
+        x.copy_(nx)
+        r.copy_(nr)
+        want = [t.clone() for t in step()]
+        for g, _ in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            for a, b in zip(out, want):
+                assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_streams(dtype):
+    """Calls on two streams at once, many times over: each has its own
+    workspace, and results do not depend on timing."""
+    x, r, p = block_inputs(51, dtype, rows=(700,))
+    gy = rand(gen(52), 700, 200, dtype=dtype)
+    want = [t for t in ops.gated_linear_backward(gy, x, p["wg"], p["wv"], p["bg"]) if t is not None]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(6):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append([t for t in ops.gated_linear_backward(gy, x, p["wg"], p["wv"], p["bg"]) if t is not None])
+    torch.cuda.synchronize()
+    for res in got:
+        for a, b in zip(res, want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_needs(dtype):
+    """Only the wanted gradients, equal to those of the whole call."""
+    x, r, p = block_inputs(61, dtype, rows=(90,))
+    dh = rand(gen(62), 90, 200, dtype=dtype)
+    full = ops.gated_linear_backward(dh, x, p["wg"], p["wv"], p["bg"], p["bg"])
+    for i in range(5):
+        one = ops.gated_linear_backward(dh, x, p["wg"], p["wv"], p["bg"], p["bg"], needs=[j == i for j in range(5)])
+        assert [t is not None for t in one] == [j == i for j in range(5)]
+        assert torch.equal(one[i], full[i])
+    g = rand(gen(63), 90, 136, dtype=dtype)
+    args = (r, x, p["n"], p["pn"], p["pn"], p["n"], p["g"])
+    whole = ops.residual_norm_backward(g, g, *args, post_norm="layer")
+    for i in range(7):
+        one = ops.residual_norm_backward(g, g, *args, post_norm="layer", needs=[j == i for j in range(7)])
+        assert torch.equal(one[i], whole[i])
+    # a missing upstream gradient is a zero one
+    zero = torch.zeros_like(g)
+    for a, b in ((None, g), (g, None)):
+        x1 = ops.residual_norm_backward(a, b, *args, post_norm="layer")
+        x2 = ops.residual_norm_backward(zero if a is None else a, zero if b is None else b, *args, post_norm="layer")
+        for s, t in zip(x1, x2):
+            assert (s.double() - t.double()).abs().max() <= 4 * unit(dtype) * max(1.0, t.abs().max().item())
+
+
+def test_small_workspace_is_refused():
+    """A workspace a byte too small changes nothing."""
+    x, w = torch.randn(40, 64, device="cuda"), torch.randn(32, 64, device="cuda")
+    h = torch.full((40, 32), 7.0, device="cuda")
+    args = ops._GATED.pack(0, 2, 40, 64, 32, x.data_ptr(), w.data_ptr(), w.data_ptr(), 0, 0, 64, 64, 64, h.data_ptr(),
+                           32, 0, 32, 0, 0, 0, 0, 0, 64, 64, 64)
+    need = mb.lib().mlipcpp_b200_gated_linear_workspace(args, False)
+    assert need > 0
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    assert mb.lib().mlipcpp_b200_gated_linear(args, ws.data_ptr(), need - 1, None) == mb.INVALID_PARAMETER
+    torch.cuda.synchronize()
+    assert (h == 7).all()
+    assert mb.lib().mlipcpp_b200_gated_linear(args, ws.data_ptr(), need, None) == mb.OK
+    ops.check_status()
+    assert not (h == 7).any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_rows_beyond_the_call_stay(dtype):
+    """Output rows and columns around the call's are left as they were."""
+    g = gen(71)
+    x, w = rand(g, 133, 64, dtype=dtype), rand(g, 70, 64, dtype=dtype, std=0.1)
+    for m in (3, 133):
+        for pad in (0, 3, 10):
+            y = torch.full((140, 70 + pad + 3), 5.0, dtype=dtype, device="cuda")
+            ld, es = y.stride(0), y.element_size()
+            args = ops._LINEAR.pack(ops._DTYPES[dtype], 0, m, 64, 70, 1.0, x.data_ptr(), w.data_ptr(), 0, 0, 64, 64, 70,
+                                    y.data_ptr() + pad * es, ld, 0, 70, 0, 0, 0, 64, 64)
+            ops._call("linear", args, 0, False)
+            assert (y[m:] == 5).all() and (y[:, :pad] == 5).all() and (y[:, pad + 70:] == 5).all()
+            assert torch.equal(y[:m, pad:pad + 70], ops.linear(x[:m], w))
