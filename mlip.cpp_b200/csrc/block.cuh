@@ -127,13 +127,12 @@ struct FewRows {
 };
 void few_rows(const FewRows &a, cudaStream_t s);
 
-// Column sums of a [M, N] matrix (fp32 sums in a fixed order), times scale,
-// into out [N]; `part`: column_sum_floats(M, N) floats.
-// out[c] = scale sum over p < P of part[p][c], in a fixed order.
-void column_join(const float *part, int P, int64_t N, float scale, void *out, int dt, cudaStream_t s);
-size_t column_sum_floats(int64_t M, int64_t N);
-void column_sum(const void *p, int dt_in, int64_t ld, int64_t M, int64_t N, float scale, void *out, int dt_out,
-                float *part, cudaStream_t s);
+// Column sums of a 16-bit [M, N] matrix in fp32 over column_strips(M) strips of
+// rows: part [strip][N].
+int column_strips(int64_t M);
+void column_sums(const void *p, int dt, int64_t ld, int64_t M, int64_t N, float *part, cudaStream_t s);
+// out[c] = scale sum over p < P of part[p][c], in a fixed order; part is used up.
+void column_join(float *part, int64_t P, int64_t N, float scale, void *out, int dt, cudaStream_t s);
 
 }  // namespace blk
 }  // namespace pet

@@ -91,6 +91,8 @@ struct EpiArgs {
   int64_t ldo;
   int dt, act;
   float scale;
+  float *sums0, *sums1;   // E_*_BWD, or null: column sums of each 32 rows of the
+                          // results before they are rounded, [row / 32][N]
   bool vin, vout;         // rows movable in 16-byte pieces
   float *part;            // E_PARTIAL: [batch][split][M][nacc]
   int64_t nacc;
@@ -266,6 +268,27 @@ __device__ __forceinline__ void block_store(const Turned<T> &b, T *out, int64_t 
   }
 }
 
+// Sums of the block's columns (bias gradients), in a fixed order: rows past M
+// are zeros.
+template <typename T>
+__device__ __forceinline__ void block_sums(const Turned<T> &b, float *sums, int lane, int row0, int col0, int N) {
+  using U = Turned<T>;
+  float s[U::V];
+#pragma unroll
+  for (int j = 0; j < U::V; ++j) {
+    s[j] = b.x[0][j];
+#pragma unroll
+    for (int i = 1; i < U::L; ++i) s[j] += b.x[i][j];
+#pragma unroll
+    for (int k = U::L; k < 32; k *= 2) s[j] += __shfl_xor_sync(0xffffffffu, s[j], k);
+  }
+  const int c = col0 + U::col(lane);
+  if (lane >= U::L) return;
+#pragma unroll
+  for (int j = 0; j < U::V; ++j)
+    if (c + j < N) sums[static_cast<size_t>(row0 / 32) * N + c + j] = s[j];
+}
+
 // The epilogue of one block: v (and w, the value half of the gated forms) as
 // they come from the accumulator, `in` from the rows' input.
 template <int EPI, typename T>
@@ -317,6 +340,10 @@ __device__ __forceinline__ void epilogue(const Params &p, int batch, float *st, 
       }
     }
   });
+  if (EPI == E_LINEAR_BWD || EPI == E_GATED_BWD) {
+    if (e.sums0) block_sums<T>(a, e.sums0, lane, row0, col0, p.N);
+    if (EPI == E_GATED_BWD && e.sums1) block_sums<T>(b, e.sums1, lane, row0, col0, p.N);
+  }
   block_store<T>(a, static_cast<T *>(batch ? e.out1 : e.out0), e.ldo, e.vout, st, lane, row0, col0, p.M, p.N);
   if (EPI == E_GATED_BWD) block_store<T>(b, static_cast<T *>(e.out1), e.ldo, e.vout, st, lane, row0, col0, p.M, p.N);
 }
@@ -682,35 +709,65 @@ __global__ void __launch_bounds__(kThreads, 1) k_block_gemm(const __grid_constan
 }
 
 // Sums the partial products of a split launch in order and runs the epilogue.
+// Block: 32 columns x 32 rows, four rows a thread.
 template <int EPI, typename T>
 __global__ void __launch_bounds__(256) k_join(const Params p) {
+  __shared__ float part[2][8][32];
   const EpiArgs &e = p.e;
-  const int64_t per = static_cast<int64_t>(p.M) * p.N, all = per * p.batch;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int batch = static_cast<int>(i / per);
-    const int64_t j = i - batch * per, row = j / p.N, col = j - row * p.N;
-    const float *src = e.part + static_cast<size_t>(batch) * p.splits * p.M * e.nacc + row * e.nacc + col;
-    const size_t step = static_cast<size_t>(p.M) * e.nacc;
-    float v = 0.f, w = 0.f;
-    for (int s = 0; s < p.splits; ++s) v += src[s * step];
-    if (p.dual)
-      for (int s = 0; s < p.splits; ++s) w += src[s * step + p.N];
-    if (e.b0) v += to_f(static_cast<const T *>(e.b0)[col]);
-    if (p.dual && e.b1) w += to_f(static_cast<const T *>(e.b1)[col]);
-    const float in = e.in ? to_f(static_cast<const T *>(e.in)[row * e.ldin + col]) : 0.f;
-    T *o = static_cast<T *>(batch ? e.out1 : e.out0) + row * e.ldo + col;
-    with_act(e.act, [&](auto A) {
-      constexpr int ACT = decltype(A)::value;
-      float a, da;
-      act_pair<ACT>(v, a, da);
-      if (EPI == E_LINEAR) *o = from_f<T>(a * e.scale + in);
-      else if (EPI == E_LINEAR_BWD) *o = from_f<T>(da * e.scale * in);
-      else if (EPI == E_GATED) *o = from_f<T>(a * w);
-      else {
-        *o = from_f<T>(da * w * in);
-        static_cast<T *>(e.out1)[row * e.ldo + col] = from_f<T>(a * in);
+  const int lane = threadIdx.x & 31, w8 = threadIdx.x >> 5;
+  const int64_t nb = (p.N + 31) / 32, mb = (p.M + 31) / 32, all = nb * mb * p.batch;
+  for (int64_t id = blockIdx.x; id < all; id += gridDim.x) {
+    const int batch = static_cast<int>(id / (nb * mb));
+    const int64_t strip = (id - batch * nb * mb) / nb, col = (id % nb) * 32 + lane;
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t row = strip * 32 + k * 8 + w8;
+      if (row >= p.M || col >= p.N) continue;
+      const float *src = e.part + static_cast<size_t>(batch) * p.splits * p.M * e.nacc + row * e.nacc + col;
+      const size_t step = static_cast<size_t>(p.M) * e.nacc;
+      float v = 0.f, w = 0.f;
+      for (int s = 0; s < p.splits; ++s) v += src[s * step];
+      if (p.dual)
+        for (int s = 0; s < p.splits; ++s) w += src[s * step + p.N];
+      if (e.b0) v += to_f(static_cast<const T *>(e.b0)[col]);
+      if (p.dual && e.b1) w += to_f(static_cast<const T *>(e.b1)[col]);
+      const float in = e.in ? to_f(static_cast<const T *>(e.in)[row * e.ldin + col]) : 0.f;
+      T *o = static_cast<T *>(batch ? e.out1 : e.out0) + row * e.ldo + col;
+      with_act(e.act, [&](auto A) {
+        constexpr int ACT = decltype(A)::value;
+        float a, da;
+        act_pair<ACT>(v, a, da);
+        if (EPI == E_LINEAR) {
+          *o = from_f<T>(fmaf(a, e.scale, in));
+        } else if (EPI == E_LINEAR_BWD) {
+          const float r = da * e.scale * in;
+          s0 += r;
+          *o = from_f<T>(r);
+        } else if (EPI == E_GATED) {
+          *o = from_f<T>(a * w);
+        } else {
+          const float r = da * w * in, q = a * in;
+          s0 += r;
+          s1 += q;
+          *o = from_f<T>(r);
+          static_cast<T *>(e.out1)[row * e.ldo + col] = from_f<T>(q);
+        }
+      });
+    }
+    if ((EPI == E_LINEAR_BWD || EPI == E_GATED_BWD) && (e.sums0 || e.sums1)) {
+      __syncthreads();
+      part[0][w8][lane] = s0;
+      part[1][w8][lane] = s1;
+      __syncthreads();
+      float *const sums = w8 == 0 ? e.sums0 : w8 == 1 ? e.sums1 : nullptr;
+      if (sums && col < p.N) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t += part[w8][k][lane];
+        sums[strip * p.N + col] = t;
       }
-    });
+    }
   }
 }
 
@@ -924,11 +981,9 @@ class Operands {
     of(job(m, rows, cols, form), form) = SplitForm{d, sc};
     return o;
   }
-  // sums of the columns of `m` (which add() has seen) into part [rows / 128][cols]
-  float *sums(const Mat &m, int64_t rows, int64_t cols) {
-    float *part = static_cast<float *>(ws_.take(4 * ((rows + 127) / 128) * cols));
+  // f32: sums of the columns of each 128 rows of `m` into part [rows / 128][cols]
+  void sums(const Mat &m, int64_t rows, int64_t cols, float *part) {
     if (!ws_.sizing()) job(m, rows, cols, FORM_NONE).sums = part;
-    return part;
   }
   void go() {
     if (!all_.n) return;
@@ -1074,7 +1129,8 @@ void launch_epi(int dt, Tiling t, const Maps &maps, const Params &p, cudaStream_
 }
 template <int EPI>
 void join_epi(int dt, const Params &p, cudaStream_t s) {
-  const int g = grid_for(static_cast<int64_t>(p.M) * p.N * p.batch);
+  const int64_t blocks = static_cast<int64_t>(ceil_div(p.M, 32)) * ceil_div(p.N, 32) * p.batch;
+  const int g = static_cast<int>(std::min<int64_t>(blocks, 8LL * sm_count()));
   if (dt == DT_F32) k_join<EPI, float><<<g, 256, 0, s>>>(p);
   else if (dt == DT_F16) k_join<EPI, __half><<<g, 256, 0, s>>>(p);
   else k_join<EPI, __nv_bfloat16><<<g, 256, 0, s>>>(p);
@@ -1236,17 +1292,6 @@ Operand split_weight(const GatedLinear::SplitWeight &w, int64_t rows, int64_t co
   return o;
 }
 
-// Column sums of dz: f32 from the sums of its blocks (part), 16-bit by a pass
-// of its own.
-void bias_grad(const Mat &dz, int64_t M, int64_t N, float scale, int dt, const float *part, void *db, Workspace &ws,
-               cudaStream_t s) {
-  if (dt == DT_F32) {
-    if (!ws.sizing()) column_join(part, ceil_div(M, 128), N, scale, db, dt, s);
-    return;
-  }
-  float *mine = static_cast<float *>(ws.take(4 * column_sum_floats(M, N)));
-  if (!ws.sizing()) column_sum(dz.p, dt, dz.ld, M, N, scale, db, dt, mine, s);
-}
 }  // namespace
 
 void gated_linear_fwd(const GatedLinear &a, Workspace &ws, cudaStream_t s) {
@@ -1323,18 +1368,28 @@ void gated_linear_bwd(const GatedLinear &a, Workspace &ws, cudaStream_t s) {
   g.e.b1 = a.bv;
   g.e.in = a.dh.p;
   g.e.ldin = a.dh.ld;
+  // bias gradients from the unrounded dz: 16-bit in the epilogue (each 32
+  // rows), f32 where dz is split (each 128)
+  void *const db[2] = {a.dbg, a.dbv};
+  const int64_t strips = ceil_div(a.M, f32 ? 128 : 32);
+  float *part[2] = {nullptr, nullptr};
+  for (int i = 0; i < 2; ++i)
+    if (db[i]) part[i] = static_cast<float *>(ws.take(4 * strips * a.F));
+  if (!f32) {
+    g.e.sums0 = part[0];
+    g.e.sums1 = part[1];
+  }
   prep.go();
   run(g, ws, s);
 
   const Mat m[2] = {{dz[0].p, fp}, {dz[1].p, fp}};
-  void *const dw[2] = {a.dwg.p, a.dwv.p}, *const db[2] = {a.dbg, a.dbv};
+  void *const dw[2] = {a.dwg.p, a.dwv.p};
   const int64_t lddw[2] = {a.dwg.ld, a.dwv.ld};
   Operand rows[2], cols[2];
-  float *part[2] = {nullptr, nullptr};
   for (int i = 0; i < 2; ++i) {
     if (a.dx.p) rows[i] = prep.add(m[i], a.M, a.F, FORM_ROWS);
     if (dw[i]) cols[i] = f32 || !a.dx.p ? prep.add(m[i], a.M, a.F, FORM_COLS) : rows[i];
-    if (db[i] && f32) part[i] = prep.sums(m[i], a.M, a.F);
+    if (db[i] && f32) prep.sums(m[i], a.M, a.F, part[i]);
   }
   prep.go();
   if (a.dx.p) {
@@ -1381,7 +1436,7 @@ void gated_linear_bwd(const GatedLinear &a, Workspace &ws, cudaStream_t s) {
     }
   }
   for (int i = 0; i < 2; ++i)
-    if (db[i]) bias_grad(m[i], a.M, a.F, 1.f, a.dtype, part[i], db[i], ws, s);
+    if (db[i] && !ws.sizing()) column_join(part[i], strips, a.F, 1.f, db[i], a.dtype, s);
 }
 
 void linear_fwd(const Linear &a, Workspace &ws, cudaStream_t s) {
@@ -1428,6 +1483,10 @@ void linear_bwd(const Linear &a, Workspace &ws, cudaStream_t s) {
   if (!id) xr = prep.add(a.x, a.M, a.K, FORM_ROWS);
   if (a.dw.p) xb = f32 || id ? prep.add(a.x, a.M, a.K, FORM_BLOCKS) : xr;
   Mat dz = a.dy;
+  // bias gradient: without an activation the sums of dy itself, else as in
+  // gated_linear_bwd
+  const int64_t strips = id && !f32 ? column_strips(a.M) : ceil_div(a.M, f32 ? 128 : 32);
+  float *part = a.db ? static_cast<float *>(ws.take(4 * strips * a.N)) : nullptr;
   if (!id) {
     const int64_t np = (a.N + 7) / 8 * 8;
     const MutMat out{ws.take(a.M * np * dtype_size(a.dtype)), np};
@@ -1445,16 +1504,16 @@ void linear_bwd(const Linear &a, Workspace &ws, cudaStream_t s) {
     g.e.b0 = a.b;
     g.e.in = a.dy.p;
     g.e.ldin = a.dy.ld;
+    if (!f32) g.e.sums0 = part;
     prep.go();
     run(g, ws, s);
     dz = Mat{out.p, np};
   }
   const float scale = id ? a.scale : 1.f;
   Operand rows, cols;
-  float *part = nullptr;
   if (a.dx.p) rows = prep.add(dz, a.M, a.N, FORM_ROWS);
   if (a.dw.p) cols = f32 || !a.dx.p ? prep.add(dz, a.M, a.N, FORM_COLS) : rows;
-  if (a.db && f32) part = prep.sums(dz, a.M, a.N);
+  if (a.db && f32) prep.sums(dz, a.M, a.N, part);
   prep.go();
   if (a.dx.p) {
     Product g;
@@ -1482,7 +1541,10 @@ void linear_bwd(const Linear &a, Workspace &ws, cudaStream_t s) {
     g.e.scale = scale;
     run(g, ws, s);
   }
-  if (a.db) bias_grad(dz, a.M, a.N, scale, a.dtype, part, a.db, ws, s);
+  if (a.db && !ws.sizing()) {
+    if (id && !f32) column_sums(dz.p, a.dtype, dz.ld, a.M, a.N, part, s);
+    column_join(part, strips, a.N, scale, a.db, a.dtype, s);
+  }
 }
 
 }  // namespace pet

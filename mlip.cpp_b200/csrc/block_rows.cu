@@ -178,15 +178,44 @@ __global__ void __launch_bounds__(256) k_column_part(const T *__restrict__ p, in
   }
 }
 
-// out[c] = scale sum_p part[p][c], the parts in 8 interleaved shares.
-__global__ void __launch_bounds__(256) k_column_join(const float *__restrict__ part, int P, int64_t N, float scale,
-                                                     void *out, int dt) {
+// Sums rows p, p + stride, .. of each group of kFold into the group's first.
+constexpr int kFold = 64;
+__global__ void __launch_bounds__(256) k_column_fold(float *part, int64_t P, int64_t stride, int64_t N) {
+  __shared__ float sums[8][33];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  for (int64_t g = blockIdx.y; g * kFold < P; g += gridDim.y) {
+    float acc = 0.f;
+    if (c < N) {
+#pragma unroll
+      for (int i = 0; i < kFold / 8; ++i) {
+        const int64_t q = g * kFold + i * 8 + warp;
+        if (q < P) acc += part[q * stride * N + c];
+      }
+    }
+    __syncthreads();
+    sums[warp][lane] = acc;
+    __syncthreads();
+    if (warp == 0 && c < N) {
+      float t = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) t += sums[w][lane];
+      part[g * kFold * stride * N + c] = t;
+    }
+  }
+}
+
+// out[c] = scale sum over p < P of part[p stride][c], in 8 interleaved shares.
+__global__ void __launch_bounds__(256) k_column_join(const float *__restrict__ part, int64_t P, int64_t stride, int64_t N,
+                                                     float scale, void *out, int dt) {
   __shared__ float sums[8][33];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   float acc = 0.f;
-  if (c < N)
-    for (int q = warp; q < P; q += 8) acc += part[q * N + c];
+  if (c < N) {
+#pragma unroll 8
+    for (int64_t q = warp; q < P; q += 8) acc += part[q * stride * N + c];
+  }
   sums[warp][lane] = acc;
   __syncthreads();
   if (warp == 0 && c < N) {
@@ -196,9 +225,6 @@ __global__ void __launch_bounds__(256) k_column_join(const float *__restrict__ p
     store_dt(out, dt, c, t * scale);
   }
 }
-
-constexpr int kStrips = 128;
-int strips(int64_t M) { return static_cast<int>(std::min<int64_t>(kStrips, (M + 63) / 64)); }
 
 template <typename T>
 void column_parts(const void *p, int dt, int64_t ld, int64_t M, int64_t N, int y, float *part, cudaStream_t s) {
@@ -223,20 +249,24 @@ void few_rows(const FewRows &a, cudaStream_t s) {
   else a.w1 ? rows_of<__nv_bfloat16, true>(a, s) : rows_of<__nv_bfloat16, false>(a, s);
 }
 
-size_t column_sum_floats(int64_t M, int64_t N) { return static_cast<size_t>(strips(M)) * N; }
+int column_strips(int64_t M) { return static_cast<int>(std::min<int64_t>(128, (M + 63) / 64)); }
 
-void column_join(const float *part, int P, int64_t N, float scale, void *out, int dt, cudaStream_t s) {
-  k_column_join<<<static_cast<unsigned>((N + 31) / 32), 256, 0, s>>>(part, P, N, scale, out, dt);
+void column_join(float *part, int64_t P, int64_t N, float scale, void *out, int dt, cudaStream_t s) {
+  const unsigned gx = static_cast<unsigned>((N + 31) / 32);
+  int64_t stride = 1;
+  for (; P > 2 * kFold; P = (P + kFold - 1) / kFold, stride *= kFold) {
+    k_column_fold<<<dim3(gx, static_cast<unsigned>(std::min<int64_t>((P + kFold - 1) / kFold, 65535))), 256, 0, s>>>(
+        part, P, stride, N);
+    CUDA_LAUNCH_CHECK();
+  }
+  k_column_join<<<gx, 256, 0, s>>>(part, P, stride, N, scale, out, dt);
   CUDA_LAUNCH_CHECK();
 }
 
-void column_sum(const void *p, int dt_in, int64_t ld, int64_t M, int64_t N, float scale, void *out, int dt_out,
-                float *part, cudaStream_t s) {
-  const int y = strips(M);
-  if (dt_in == DT_F32) column_parts<float>(p, dt_in, ld, M, N, y, part, s);
-  else if (dt_in == DT_F16) column_parts<__half>(p, dt_in, ld, M, N, y, part, s);
-  else column_parts<__nv_bfloat16>(p, dt_in, ld, M, N, y, part, s);
-  column_join(part, y, N, scale, out, dt_out, s);
+void column_sums(const void *p, int dt, int64_t ld, int64_t M, int64_t N, float *part, cudaStream_t s) {
+  const int y = column_strips(M);
+  if (dt == DT_F16) column_parts<__half>(p, dt, ld, M, N, y, part, s);
+  else column_parts<__nv_bfloat16>(p, dt, ld, M, N, y, part, s);
 }
 
 }  // namespace blk
