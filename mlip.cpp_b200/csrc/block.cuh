@@ -112,20 +112,28 @@ __device__ __forceinline__ void store_dt(void *p, int dt, int64_t j, float v) {
 }
 
 // ---- few rows (block_rows.cu) ---------------------------------------------
-// Forward of at most kFewRows rows: reads each weight once with plain loads.
+// At most kFewRows rows: each weight read once with plain loads, every sum and
+// gradient in fp32.
 constexpr int kFewRows = 8;
 struct FewRows {
   int dt, act, M;
   int64_t K, N;
   const void *x, *w0, *w1;  // w1 null: linear
   int64_t ldx, ldw0, ldw1;
-  const void *b0, *b1, *res;
-  int64_t ldr;
+  const void *b0, *b1;
   float scale;
-  void *out;
+  const void *in;           // residual (linear forward) or upstream gradient (backward)
+  int64_t ldin;
+  void *out;                // forward: the result; null in a backward
   int64_t ldo;
+  // backward: gradients out unless null; dz: few_rows_floats() floats
+  void *dx, *dw0, *dw1, *db0, *db1;
+  int64_t lddx, lddw0, lddw1;
+  float *dz;
 };
 void few_rows(const FewRows &a, cudaStream_t s);
+size_t few_rows_floats(const FewRows &a);
+void few_rows_bwd(const FewRows &a, cudaStream_t s);
 
 // Column sums of a 16-bit [M, N] matrix in fp32 over column_strips(M) strips of
 // rows: part [strip][N].

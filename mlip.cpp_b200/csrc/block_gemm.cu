@@ -526,14 +526,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_block_gemm(const __grid_constan
 #pragma unroll
             for (int kk = 0; kk < BK / 16; ++kk) {
               const uint32_t more = (kt > kt0 || kk > 0) ? 1u : 0u;
-              const uint64_t ah = desc(da + kk * ka), bh = desc(db + kk * kb);
               if (F32 && p.products == 3) {
-                mma(d, desc(da + (kTile >> 4) + kk * ka), bh, more);
-                mma(d, ah, desc(db + (C::BTile >> 4) + kk * kb), 1u);
-                mma(d, ah, bh, 1u);
+                mma(d, desc(da + (kTile >> 4) + kk * ka), desc(db + kk * kb), more);
+                mma(d, desc(da + kk * ka), desc(db + (C::BTile >> 4) + kk * kb), 1u);
               } else {
-                mma(d, ah, bh, more);
+                mma(d, desc(da + kk * ka), desc(db + kk * kb), more);
               }
+            }
+            // the large products after the small ones, so that fewer additions
+            // are truncated at the sum's full size
+            if (F32 && p.products == 3) {
+#pragma unroll
+              for (int kk = 0; kk < BK / 16; ++kk) mma(d, desc(da + kk * ka), desc(db + kk * kb), 1u);
             }
             commit(empty0 + 8 * s);
           }
@@ -1294,12 +1298,53 @@ Operand split_weight(const GatedLinear::SplitWeight &w, int64_t rows, int64_t co
 
 }  // namespace
 
+namespace {
+FewRows few_of(const GatedLinear &a) {
+  FewRows f{};
+  f.dt = a.dtype;
+  f.act = a.act;
+  f.M = static_cast<int>(a.M);
+  f.K = a.K;
+  f.N = a.F;
+  f.x = a.x.p;
+  f.ldx = a.x.ld;
+  f.w0 = a.wg.p;
+  f.w1 = a.wv.p;
+  f.ldw0 = a.wg.ld;
+  f.ldw1 = a.wv.ld;
+  f.b0 = a.bg;
+  f.b1 = a.bv;
+  f.scale = 1.f;
+  return f;
+}
+FewRows few_of(const Linear &a) {
+  FewRows f{};
+  f.dt = a.dtype;
+  f.act = a.act;
+  f.M = static_cast<int>(a.M);
+  f.K = a.K;
+  f.N = a.N;
+  f.x = a.x.p;
+  f.ldx = a.x.ld;
+  f.w0 = a.w.p;
+  f.ldw0 = a.w.ld;
+  f.b0 = a.b;
+  f.scale = a.scale;
+  return f;
+}
+void few_bwd(FewRows &f, Workspace &ws, cudaStream_t s) {
+  f.dz = static_cast<float *>(ws.take(4 * few_rows_floats(f)));
+  if (!ws.sizing()) few_rows_bwd(f, s);
+}
+}  // namespace
+
 void gated_linear_fwd(const GatedLinear &a, Workspace &ws, cudaStream_t s) {
   if (a.M == 0) return;
   if (a.M <= kFewRows && !a.x_split) {
     if (ws.sizing()) return;
-    FewRows f{a.dtype, a.act, static_cast<int>(a.M), a.K, a.F, a.x.p, a.wg.p, a.wv.p, a.x.ld, a.wg.ld, a.wv.ld,
-              a.bg, a.bv, nullptr, 0, 1.f, a.h.p, a.h.ld};
+    FewRows f = few_of(a);
+    f.out = a.h.p;
+    f.ldo = a.h.ld;
     few_rows(f, s);
     return;
   }
@@ -1339,6 +1384,21 @@ void gated_linear_bwd(const GatedLinear &a, Workspace &ws, cudaStream_t s) {
   }
   const bool weights = a.dwg.p || a.dwv.p;
   if (!a.dx.p && !weights && !a.dbg && !a.dbv) return;
+  if (a.M <= kFewRows && !a.x_split) {
+    FewRows f = few_of(a);
+    f.in = a.dh.p;
+    f.ldin = a.dh.ld;
+    f.dx = a.dx.p;
+    f.lddx = a.dx.ld;
+    f.dw0 = a.dwg.p;
+    f.dw1 = a.dwv.p;
+    f.lddw0 = a.dwg.ld;
+    f.lddw1 = a.dwv.ld;
+    f.db0 = a.dbg;
+    f.db1 = a.dbv;
+    few_bwd(f, ws, s);
+    return;
+  }
   const bool f32 = a.dtype == DT_F32;
   const size_t es = dtype_size(a.dtype);
   const int64_t fp = (a.F + 7) / 8 * 8;
@@ -1443,8 +1503,11 @@ void linear_fwd(const Linear &a, Workspace &ws, cudaStream_t s) {
   if (a.M == 0) return;
   if (a.M <= kFewRows) {
     if (ws.sizing()) return;
-    FewRows f{a.dtype, a.act, static_cast<int>(a.M), a.K, a.N, a.x.p, a.w.p, nullptr, a.x.ld, a.w.ld, 0, a.b, nullptr,
-              a.residual.p, a.residual.ld, a.scale, a.y.p, a.y.ld};
+    FewRows f = few_of(a);
+    f.in = a.residual.p;
+    f.ldin = a.residual.ld;
+    f.out = a.y.p;
+    f.ldo = a.y.ld;
     few_rows(f, s);
     return;
   }
@@ -1476,6 +1539,18 @@ void linear_bwd(const Linear &a, Workspace &ws, cudaStream_t s) {
     return;
   }
   if (!a.dx.p && !a.dw.p && !a.db) return;
+  if (a.M <= kFewRows) {
+    FewRows f = few_of(a);
+    f.in = a.dy.p;
+    f.ldin = a.dy.ld;
+    f.dx = a.dx.p;
+    f.lddx = a.dx.ld;
+    f.dw0 = a.dw.p;
+    f.lddw0 = a.dw.ld;
+    f.db0 = a.db;
+    few_bwd(f, ws, s);
+    return;
+  }
   const bool id = a.act == ACT_IDENTITY, f32 = a.dtype == DT_F32;
   Operands prep(a.dtype, ws, s);
   Operand w, xr, xb;

@@ -7,6 +7,11 @@
 // row of x, which stays in L1.  The sums run in fp32 FMAs; the tensor cores
 // would idle behind the same loads, and a 128-row tile would leave most SMs
 // without work.
+//
+// The backward of so few rows is the same for the weights (read once for dz,
+// once for dx, and their gradients written once): dz in fp32 by the forward's
+// kernel, dW = dz^T x and db as one pass of stores, dx = dz W in strips of W's
+// rows whose fp32 sums a last kernel adds in order.
 #include <algorithm>
 
 #include "block.cuh"
@@ -109,12 +114,16 @@ __global__ void __launch_bounds__(256) k_few_rows(const FewRows a, int wpr) {
   if (n >= a.N || lane >= a.M) return;
   if (a.b0) v += to_f(static_cast<const T *>(a.b0)[n]);
   if (DUAL && a.b1) w += to_f(static_cast<const T *>(a.b1)[n]);
-  with_act(a.act, [&](auto A) {
-    float da;
-    act_pair<decltype(A)::value>(v, v, da);
-  });
+  const float in = a.in ? to_f(static_cast<const T *>(a.in)[lane * a.ldin + n]) : 0.f;
+  float da;
+  with_act(a.act, [&](auto A) { act_pair<decltype(A)::value>(v, v, da); });
+  if (!a.out) {  // backward: [product][row][feature]
+    a.dz[lane * a.N + n] = DUAL ? da * w * in : da * a.scale * in;
+    if (DUAL) a.dz[(a.M + lane) * a.N + n] = v * in;
+    return;
+  }
   if (DUAL) v *= w;
-  else v = v * a.scale + (a.res ? to_f(static_cast<const T *>(a.res)[lane * a.ldr + n]) : 0.f);
+  else v = v * a.scale + in;
   static_cast<T *>(a.out)[lane * a.ldo + n] = from_f<T>(v);
 }
 
@@ -138,6 +147,176 @@ void rows_of(const FewRows &a, cudaStream_t s) {
   if (a.M == 1) launch_rows<T, 1, DUAL>(a, s);
   else if (a.M <= 4) launch_rows<T, 4, DUAL>(a, s);
   else launch_rows<T, kFewRows, DUAL>(a, s);
+}
+
+// dz of a linear layer without an activation.
+template <typename T>
+__global__ void __launch_bounds__(256) k_rows_dz(const FewRows a) {
+  const int64_t all = a.M * a.N;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t m = i / a.N;
+    a.dz[i] = a.scale * to_f(static_cast<const T *>(a.in)[m * a.ldin + (i - m * a.N)]);
+  }
+}
+
+// dW[n][k] = sum over m of dz[m][n] x[m][k]; db[n] = sum of dz[m][n].  Block:
+// kStrip features n, 32 V columns k a warp and 8 of those; blockIdx.z: product.
+constexpr int kStrip = 16;
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) k_rows_dw(const FewRows a) {
+  constexpr int V = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  T *dw = static_cast<T *>(blockIdx.z ? a.dw1 : a.dw0);
+  T *db = static_cast<T *>(blockIdx.z ? a.db1 : a.db0);
+  const int64_t ld = blockIdx.z ? a.lddw1 : a.lddw0;
+  const float *dz = a.dz + blockIdx.z * a.M * a.N;
+  if (db && blockIdx.x == 0)
+    for (int64_t n = static_cast<int64_t>(blockIdx.y) * 256 + threadIdx.x; n < a.N; n += static_cast<int64_t>(gridDim.y) * 256) {
+      float t = 0.f;
+      for (int m = 0; m < a.M; ++m) t += dz[m * a.N + n];
+      db[n] = from_f<T>(t);
+    }
+  const int64_t k = ((static_cast<int64_t>(blockIdx.x) * 8 + warp) * 32 + lane) * V;
+  if (!dw || k >= a.K) return;
+  float x[kFewRows][V];
+#pragma unroll
+  for (int m = 0; m < kFewRows; ++m) {
+    const T *p = static_cast<const T *>(a.x) + m * a.ldx + k;
+#pragma unroll
+    for (int j = 0; j < V; ++j) x[m][j] = 0.f;
+    if (m >= a.M) continue;
+    if constexpr (VEC) {
+      float f[16 / sizeof(T)];
+      unpack<T>(__ldg(reinterpret_cast<const uint4 *>(p)), f);
+#pragma unroll
+      for (int j = 0; j < V; ++j) x[m][j] = f[j];
+    } else {
+      x[m][0] = to_f(*p);
+    }
+  }
+  for (int64_t n0 = static_cast<int64_t>(blockIdx.y) * kStrip; n0 < a.N; n0 += static_cast<int64_t>(gridDim.y) * kStrip)
+  for (int64_t n = n0; n < min(a.N, n0 + kStrip); ++n) {
+    float v[VEC ? 16 / sizeof(T) : 1];
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = 0.f;
+#pragma unroll
+    for (int m = 0; m < kFewRows; ++m) {
+      if (m >= a.M) break;
+      const float g = __ldg(dz + m * a.N + n);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = fmaf(g, x[m][j], v[j]);
+    }
+    if constexpr (VEC) *reinterpret_cast<uint4 *>(dw + n * ld + k) = pack<T>(v);
+    else dw[n * ld + k] = from_f<T>(v[0]);
+  }
+}
+
+// part[strip][m][k] = sum over the strip's features n of dz[m][n] W[n][k], over
+// both products; a strip of W's rows in eight interleaved shares, one a warp.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) k_rows_dx(const FewRows a, int64_t strip, float *part) {
+  constexpr int V = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
+  __shared__ float sums[8][32 * V];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t k0 = static_cast<int64_t>(blockIdx.x) * 32 * V, k = k0 + lane * V;
+  const int64_t n0 = blockIdx.y * strip, n1 = min(a.N, n0 + strip);
+  float acc[kFewRows][V];
+#pragma unroll
+  for (int m = 0; m < kFewRows; ++m)
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[m][j] = 0.f;
+  for (int q = 0; q < (a.w1 ? 2 : 1); ++q) {
+    const T *w = static_cast<const T *>(q ? a.w1 : a.w0) + k;
+    const int64_t ld = q ? a.ldw1 : a.ldw0;
+    const float *dz = a.dz + q * a.M * a.N;
+    if (k < a.K) {
+#pragma unroll 4
+      for (int64_t n = n0 + warp; n < n1; n += 8) {
+        float f[VEC ? 16 / sizeof(T) : 1];
+        if constexpr (VEC) unpack<T>(__ldg(reinterpret_cast<const uint4 *>(w + n * ld)), f);
+        else f[0] = to_f(w[n * ld]);
+#pragma unroll
+        for (int m = 0; m < kFewRows; ++m) {
+          if (m >= a.M) break;
+          const float g = __ldg(dz + m * a.N + n);
+#pragma unroll
+          for (int j = 0; j < V; ++j) acc[m][j] = fmaf(g, f[j], acc[m][j]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < kFewRows; ++m) {
+    if (m >= a.M) break;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < V; ++j) sums[warp][lane * V + j] = acc[m][j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * V; i += 256) {
+      if (k0 + i >= a.K) continue;
+      float t = 0.f;
+#pragma unroll
+      for (int w8 = 0; w8 < 8; ++w8) t += sums[w8][i];
+      part[(static_cast<int64_t>(blockIdx.y) * a.M + m) * a.K + k0 + i] = t;
+    }
+  }
+}
+template <typename T>
+__global__ void __launch_bounds__(256) k_rows_join(const FewRows a, int strips, const float *part) {
+  const int64_t all = a.M * a.K;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * 256) {
+    float t = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < strips; ++s) t += part[s * all + i];
+    const int64_t m = i / a.K;
+    static_cast<T *>(a.dx)[m * a.lddx + (i - m * a.K)] = from_f<T>(t);
+  }
+}
+
+// Strips of W's rows for dx: enough blocks for every SM to have four, at least
+// 32 rows each.
+int dx_strips(const FewRows &a) {
+  const int64_t cols = (a.K + 255) / 256;  // blocks of 32 16-byte pieces, about
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((a.N + 31) / 32, (4LL * sm_count() + cols - 1) / cols)));
+}
+
+int blocks_for(int64_t threads) {
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((threads + 255) / 256, 8LL * sm_count())));
+}
+
+template <typename T>
+void bwd_of(const FewRows &a, cudaStream_t s) {
+  constexpr int V = 16 / static_cast<int>(sizeof(T));
+  if (a.w1 || a.act != ACT_IDENTITY) {
+    FewRows z = a;
+    z.out = nullptr;
+    a.w1 ? rows_of<T, true>(z, s) : rows_of<T, false>(z, s);
+  } else {
+    k_rows_dz<T><<<blocks_for(a.M * a.N), 256, 0, s>>>(a);
+    CUDA_LAUNCH_CHECK();
+  }
+  if (a.dw0 || a.dw1 || a.db0 || a.db1) {
+    const bool vec = a.K % V == 0 && rows16(a.x, a.ldx, a.dt) && (!a.dw0 || rows16(a.dw0, a.lddw0, a.dt)) &&
+                     (!a.dw1 || rows16(a.dw1, a.lddw1, a.dt));
+    const int64_t span = 256LL * (vec ? V : 1);
+    const int64_t strips = (a.N + kStrip - 1) / kStrip;
+    const dim3 g(static_cast<unsigned>((a.K + span - 1) / span), static_cast<unsigned>(std::min<int64_t>(strips, 65535)),
+                 a.w1 ? 2 : 1);
+    if (vec) k_rows_dw<T, true><<<g, 256, 0, s>>>(a);
+    else k_rows_dw<T, false><<<g, 256, 0, s>>>(a);
+    CUDA_LAUNCH_CHECK();
+  }
+  if (!a.dx) return;
+  const bool vec = a.K % V == 0 && rows16(a.w0, a.ldw0, a.dt) && (!a.w1 || rows16(a.w1, a.ldw1, a.dt));
+  const int y = dx_strips(a);
+  const int64_t strip = (a.N + y - 1) / y, span = 32LL * (vec ? V : 1);
+  float *part = a.dz + (a.w1 ? 2 : 1) * a.M * a.N;
+  const dim3 g(static_cast<unsigned>((a.K + span - 1) / span), y);
+  if (vec) k_rows_dx<T, true><<<g, 256, 0, s>>>(a, strip, part);
+  else k_rows_dx<T, false><<<g, 256, 0, s>>>(a, strip, part);
+  CUDA_LAUNCH_CHECK();
+  k_rows_join<T><<<blocks_for(a.M * a.K), 256, 0, s>>>(a, y, part);
+  CUDA_LAUNCH_CHECK();
 }
 
 // Sums of columns over a strip of rows, a fixed share of it per warp.
@@ -247,6 +426,16 @@ void few_rows(const FewRows &a, cudaStream_t s) {
   if (a.dt == DT_F32) a.w1 ? rows_of<float, true>(a, s) : rows_of<float, false>(a, s);
   else if (a.dt == DT_F16) a.w1 ? rows_of<__half, true>(a, s) : rows_of<__half, false>(a, s);
   else a.w1 ? rows_of<__nv_bfloat16, true>(a, s) : rows_of<__nv_bfloat16, false>(a, s);
+}
+
+size_t few_rows_floats(const FewRows &a) {
+  return static_cast<size_t>(a.M) * ((a.w1 ? 2 : 1) * a.N + dx_strips(a) * a.K);
+}
+
+void few_rows_bwd(const FewRows &a, cudaStream_t s) {
+  if (a.dt == DT_F32) bwd_of<float>(a, s);
+  else if (a.dt == DT_F16) bwd_of<__half>(a, s);
+  else bwd_of<__nv_bfloat16>(a, s);
 }
 
 int column_strips(int64_t M) { return static_cast<int>(std::min<int64_t>(128, (M + 63) / 64)); }

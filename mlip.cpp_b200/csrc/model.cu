@@ -1175,7 +1175,7 @@ void PETModel::setup_graph(int n_local, int N0, int E0, int N1, int E1, const in
   }
   if (h_.prenorm) {
     // working memory of the block operators: the largest of their calls (an
-    // operator sizes by shape; any pointer stands for a wanted gradient)
+    // operator sizes by shape and by which tensors there are)
     size_t need = 0;
     for (int l = 0; l < 2; ++l) {
       float any = 0.f;
@@ -1183,6 +1183,7 @@ void PETModel::setup_graph(int n_local, int N0, int E0, int N1, int E1, const in
       g.M = Tl_[l];
       g.K = h_.d;
       g.F = h_.ff;
+      g.wg = g.wv = {&any, h_.d};
       Workspace fw, bw;
       gated_linear_fwd(g, fw, stream_);
       g.dx = {&any, h_.d};
