@@ -112,8 +112,8 @@ __device__ __forceinline__ void store_dt(void *p, int dt, int64_t j, float v) {
 }
 
 // ---- few rows (block_rows.cu) ---------------------------------------------
-// At most kFewRows rows: each weight read once with plain loads, every sum and
-// gradient in fp32.
+// At most kFewRows rows (forward of 16-bit aligned ones: 16): each weight read
+// once with plain loads, every sum and gradient in fp32.
 constexpr int kFewRows = 8;
 struct FewRows {
   int dt, act, M;
@@ -131,6 +131,7 @@ struct FewRows {
   int64_t lddx, lddw0, lddw1;
   float *dz;
 };
+bool few_rows_fit(const FewRows &a);  // forward
 void few_rows(const FewRows &a, cudaStream_t s);
 size_t few_rows_floats(const FewRows &a);
 void few_rows_bwd(const FewRows &a, cudaStream_t s);

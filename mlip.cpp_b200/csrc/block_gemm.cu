@@ -918,15 +918,32 @@ __global__ void __launch_bounds__(256) k_split(const SplitJobs all) {
   }
 }
 
-// 16-bit rows whose address or stride TMA cannot take -> rows of cp elements.
-__global__ void __launch_bounds__(256) k_pack(const uint16_t *__restrict__ src, int64_t ld, int64_t R, int C, int cp,
-                                              uint16_t *dst) {
-  const int64_t nc = cp / 2, n = R * nc;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t r = i / nc;
-    const int c = static_cast<int>(i - r * nc) * 2;
-    const uint32_t a = c < C ? src[r * ld + c] : 0u, b = c + 1 < C ? src[r * ld + c + 1] : 0u;
-    *reinterpret_cast<uint32_t *>(dst + r * cp + c) = a | (b << 16);
+// 16-bit matrices whose address or stride TMA cannot take -> rows of cp
+// elements, all of a step in one launch; eight elements a thread.
+struct PackJob {
+  const uint16_t *src;
+  uint16_t *dst;
+  int64_t ld, rows, first;  // first: number of the job's first piece
+  int C, cp;
+};
+struct PackJobs {
+  PackJob job[4];
+  int n;
+  int64_t total;
+};
+__global__ void __launch_bounds__(256) k_pack(const PackJobs all) {
+  for (int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; id < all.total; id += static_cast<int64_t>(gridDim.x) * 256) {
+    int ji = 0;
+    while (ji + 1 < all.n && id >= all.job[ji + 1].first) ++ji;
+    const PackJob &q = all.job[ji];
+    const int64_t i = id - q.first, nc = q.cp / 8, r = i / nc;
+    const int c = static_cast<int>(i - r * nc) * 8;
+    const uint16_t *p = q.src + r * q.ld + c;
+    uint32_t v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < q.C ? p[j] : 0u;
+    *reinterpret_cast<uint4 *>(q.dst + r * q.cp + c) =
+        make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
   }
 }
 
@@ -958,8 +975,8 @@ Operand from_split(const Split16View &v) {
   return o;
 }
 
-// Prepares operands: 16-bit ones where they lie (or packed), f32 ones as jobs
-// of one launch of k_split, issued by go().
+// Prepares operands: 16-bit ones where they lie (or packed), f32 ones in split
+// form, by one launch each, issued by go().
 enum Form { FORM_NONE, FORM_ROWS, FORM_COLS, FORM_BLOCKS };
 class Operands {
  public:
@@ -990,6 +1007,11 @@ class Operands {
     if (!ws_.sizing()) job(m, rows, cols, FORM_NONE).sums = part;
   }
   void go() {
+    if (pack_.n) {
+      k_pack<<<grid_for(pack_.total), 256, 0, s_>>>(pack_);
+      CUDA_LAUNCH_CHECK();
+      pack_ = PackJobs{};
+    }
     if (!all_.n) return;
     all_.total = 0;
     for (int i = 0; i < all_.n; ++i) {
@@ -1037,9 +1059,10 @@ class Operands {
     uint16_t *d = static_cast<uint16_t *>(ws_.take(2 * rows * o.ld));
     o.p = d;
     if (!ws_.sizing()) {
-      k_pack<<<grid_for(rows * o.ld / 2), 256, 0, s_>>>(static_cast<const uint16_t *>(m.p), m.ld, rows,
-                                                        static_cast<int>(cols), static_cast<int>(o.ld), d);
-      CUDA_LAUNCH_CHECK();
+      if (pack_.n == 4) throw Error(kErrInternal, "too many operands in one step");
+      pack_.job[pack_.n++] = PackJob{static_cast<const uint16_t *>(m.p), d, m.ld, rows, pack_.total,
+                                     static_cast<int>(cols), static_cast<int>(o.ld)};
+      pack_.total += rows * (o.ld / 8);
     }
     return o;
   }
@@ -1047,6 +1070,7 @@ class Operands {
   Workspace &ws_;
   cudaStream_t s_;
   SplitJobs all_{};
+  PackJobs pack_{};
 };
 
 // ---------------------------------------------------------------------------
@@ -1183,11 +1207,14 @@ void run(const Product &g, Workspace &ws, cudaStream_t s) {
   const int64_t tiles = count(bm, bn);
   p.tiles_m = static_cast<int>((g.M + bm - 1) / bm);
   p.tiles_n = static_cast<int>(tiles / p.tiles_m / p.batch);
-  // few tiles and a long contraction: divided over the SMs, at least four k
-  // tiles each
+  // few tiles and a long contraction: divided over the SMs, where that saves
+  // more k tiles (about 0.35 us each) than the second kernel costs (6 us)
   const int at_once = tile.pair ? sms / 2 : sms;
   int splits = 1;
-  if (tiles * 2 <= at_once && p.kt >= 8) splits = static_cast<int>(std::min<int64_t>(at_once / tiles, p.kt / 4));
+  if (tiles * 2 <= at_once && p.kt >= 16) {
+    splits = static_cast<int>(std::min<int64_t>(at_once / tiles, p.kt / 4));
+    if (p.kt - (p.kt + splits - 1) / splits < 20) splits = 1;
+  }
   p.kt_split = (p.kt + splits - 1) / splits;
   p.kt_split = (p.kt_split + unit - 1) / unit * unit;
   p.splits = splits = (p.kt + p.kt_split - 1) / p.kt_split;
@@ -1303,7 +1330,7 @@ FewRows few_of(const GatedLinear &a) {
   FewRows f{};
   f.dt = a.dtype;
   f.act = a.act;
-  f.M = static_cast<int>(a.M);
+  f.M = static_cast<int>(std::min<int64_t>(a.M, INT32_MAX));
   f.K = a.K;
   f.N = a.F;
   f.x = a.x.p;
@@ -1321,7 +1348,7 @@ FewRows few_of(const Linear &a) {
   FewRows f{};
   f.dt = a.dtype;
   f.act = a.act;
-  f.M = static_cast<int>(a.M);
+  f.M = static_cast<int>(std::min<int64_t>(a.M, INT32_MAX));
   f.K = a.K;
   f.N = a.N;
   f.x = a.x.p;
@@ -1340,9 +1367,8 @@ void few_bwd(FewRows &f, Workspace &ws, cudaStream_t s) {
 
 void gated_linear_fwd(const GatedLinear &a, Workspace &ws, cudaStream_t s) {
   if (a.M == 0) return;
-  if (a.M <= kFewRows && !a.x_split) {
+  if (FewRows f = few_of(a); !a.x_split && few_rows_fit(f)) {
     if (ws.sizing()) return;
-    FewRows f = few_of(a);
     f.out = a.h.p;
     f.ldo = a.h.ld;
     few_rows(f, s);
@@ -1501,9 +1527,8 @@ void gated_linear_bwd(const GatedLinear &a, Workspace &ws, cudaStream_t s) {
 
 void linear_fwd(const Linear &a, Workspace &ws, cudaStream_t s) {
   if (a.M == 0) return;
-  if (a.M <= kFewRows) {
+  if (FewRows f = few_of(a); few_rows_fit(f)) {
     if (ws.sizing()) return;
-    FewRows f = few_of(a);
     f.in = a.residual.p;
     f.ldin = a.residual.ld;
     f.out = a.y.p;

@@ -1,18 +1,26 @@
 // Transformer-block operators for a handful of rows (single tokens), and the
 // column sums of the bias gradients.
 //
-// With at most 8 rows the dense forward is the time it takes to read the
-// weights once: one to eight warps per output feature stream its weight rows
-// with 16-byte loads, several in flight per lane, and multiply them with every
-// row of x, which stays in L1.  The sums run in fp32 FMAs; the tensor cores
-// would idle behind the same loads, and a 128-row tile would leave most SMs
-// without work.
+// With a handful of rows a dense layer is the time it takes to read the weights
+// once, so everything is arranged around 16-byte weight loads, several in flight
+// per lane.
+//
+//  * 16-bit: one CTA per 16 output features, its eight warps along K.  A warp
+//    multiplies a 16 x 16 piece of the weight with up to 8 (16) rows of x by one
+//    (two) mma.sync: a lane's 16 bytes of a weight row and of a row of x are the
+//    fragments as they come, with the contraction index permuted alike on both
+//    sides.  With FMAs the same loads cost 130 instructions for 32 bytes of
+//    weight at 8 rows, and took 33 us where this takes 11 (two 5632 x 2048
+//    weights); a tcgen05 tile of 128 rows took 18.
+//  * f32, and rows that are not 16-byte aligned: one to eight warps per output
+//    feature, fp32 FMAs.
 //
 // The backward of so few rows is the same for the weights (read once for dz,
 // once for dx, and their gradients written once): dz in fp32 by the forward's
-// kernel, dW = dz^T x and db as one pass of stores, dx = dz W in strips of W's
+// kernels, dW = dz^T x and db as one pass of stores, dx = dz W in strips of W's
 // rows whose fp32 sums a last kernel adds in order.
 #include <algorithm>
+#include <type_traits>
 
 #include "block.cuh"
 
@@ -22,6 +30,118 @@ namespace blk {
 namespace {
 
 constexpr int kDepth = 4;  // loads in flight per lane and weight (8 cost more in resident warps)
+
+// The epilogue of one result: row m, feature n, both products.  dz of a backward
+// goes out as [product][feature][8 rows], the rows past M zeros.
+constexpr int kRowPad = 8;
+template <typename T, bool DUAL>
+__device__ __forceinline__ void finish(const FewRows &a, int m, int64_t n, float v, float w) {
+  if (a.b0) v += to_f(static_cast<const T *>(a.b0)[n]);
+  if (DUAL && a.b1) w += to_f(static_cast<const T *>(a.b1)[n]);
+  const float in = a.in ? to_f(static_cast<const T *>(a.in)[m * a.ldin + n]) : 0.f;
+  float da;
+  with_act(a.act, [&](auto A) { act_pair<decltype(A)::value>(v, v, da); });
+  if (a.out) {
+    if (DUAL) v *= w;
+    else v = v * a.scale + in;
+    static_cast<T *>(a.out)[m * a.ldo + n] = from_f<T>(v);
+  } else {
+    a.dz[n * kRowPad + m] = DUAL ? da * w * in : da * a.scale * in;
+    if (DUAL) a.dz[(a.N + n) * kRowPad + m] = v * in;
+  }
+}
+
+// D += A B with A 16 x 16 (four registers a lane), B 16 x 8 (two).
+template <typename T>
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                      uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 16-bit rows, 16-byte aligned, K a multiple of 8; M <= 8 NT.  Lane (g, t) of a
+// warp holds weight rows g and g + 8 and rows g (and g + 8) of x, eight elements
+// at 8 t of each 32: two MMAs, of its first and its last four.
+template <typename T, int NT, bool DUAL>
+__global__ void __launch_bounds__(256) k_few_mma(const FewRows a) {
+  constexpr int NP = DUAL ? 2 : 1;
+  constexpr int U = DUAL || NT > 1 ? 2 : 4;  // 32-element steps in flight
+  __shared__ float part[8][NP][NT][16 * 8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
+  const T *w[NP][2], *x[NT];
+#pragma unroll
+  for (int q = 0; q < NP; ++q)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int64_t n = min(n0 + g + 8 * r, a.N - 1);  // (rows past N are computed and not stored)
+      w[q][r] = static_cast<const T *>(q ? a.w1 : a.w0) + n * (q ? a.ldw1 : a.ldw0);
+    }
+#pragma unroll
+  for (int i = 0; i < NT; ++i) x[i] = g + 8 * i < a.M ? static_cast<const T *>(a.x) + (g + 8 * i) * a.ldx : nullptr;
+  float d[NP][NT][4];
+#pragma unroll
+  for (int q = 0; q < NP; ++q)
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) d[q][i][j] = 0.f;
+  for (int64_t k0 = warp * 32 + t * 8; k0 - t * 8 < a.K; k0 += U * 256) {
+    uint4 wr[U][NP][2], xr[U][NT];
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t k = k0 + u * 256;
+      const bool in = k < a.K;
+#pragma unroll
+      for (int q = 0; q < NP; ++q)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) wr[u][q][r] = in ? __ldg(reinterpret_cast<const uint4 *>(w[q][r] + k)) : zero;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) xr[u][i] = in && x[i] ? __ldg(reinterpret_cast<const uint4 *>(x[i] + k)) : zero;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int q = 0; q < NP; ++q)
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          mma16<T>(d[q][i], wr[u][q][0].x, wr[u][q][1].x, wr[u][q][0].y, wr[u][q][1].y, xr[u][i].x, xr[u][i].y);
+          mma16<T>(d[q][i], wr[u][q][0].z, wr[u][q][1].z, wr[u][q][0].w, wr[u][q][1].w, xr[u][i].z, xr[u][i].w);
+        }
+  }
+  // d[.][i][j]: feature g + 8 (j / 2), row 8 i + 2 t + j % 2; the warps' shares
+  // are added in order
+#pragma unroll
+  for (int q = 0; q < NP; ++q)
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) part[warp][q][i][(2 * t + j % 2) * 16 + g + 8 * (j / 2)] = d[q][i][j];
+  __syncthreads();
+  for (int i = threadIdx.x; i < NT * 128; i += 256) {
+    const int m = i / 16;
+    const int64_t n = n0 + i % 16;
+    if (n >= a.N) continue;
+    if (m >= a.M) {
+      if (!a.out && m < kRowPad) {
+        a.dz[n * kRowPad + m] = 0.f;
+        if (DUAL) a.dz[(a.N + n) * kRowPad + m] = 0.f;
+      }
+      continue;
+    }
+    float v[2] = {0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < NP; ++q)
+#pragma unroll
+      for (int s = 0; s < 8; ++s) v[q] += part[s][q][m / 8][(m % 8) * 16 + i % 16];
+    finish<T, DUAL>(a, m, n, v[0], v[1]);
+  }
+}
 
 template <typename T, int MR, bool DUAL, bool VEC>
 __global__ void __launch_bounds__(256) k_few_rows(const FewRows a, int wpr) {
@@ -111,20 +231,18 @@ __global__ void __launch_bounds__(256) k_few_rows(const FewRows a, int wpr) {
       v = sum[m];
       if (DUAL) w = sum[MR * (DUAL ? 1 : 0) + m];
     }
-  if (n >= a.N || lane >= a.M) return;
-  if (a.b0) v += to_f(static_cast<const T *>(a.b0)[n]);
-  if (DUAL && a.b1) w += to_f(static_cast<const T *>(a.b1)[n]);
-  const float in = a.in ? to_f(static_cast<const T *>(a.in)[lane * a.ldin + n]) : 0.f;
-  float da;
-  with_act(a.act, [&](auto A) { act_pair<decltype(A)::value>(v, v, da); });
-  if (!a.out) {  // backward: [product][row][feature]
-    a.dz[lane * a.N + n] = DUAL ? da * w * in : da * a.scale * in;
-    if (DUAL) a.dz[(a.M + lane) * a.N + n] = v * in;
-    return;
+  if (n >= a.N) return;
+  if (!a.out && lane >= a.M && lane < kRowPad) {
+    a.dz[n * kRowPad + lane] = 0.f;
+    if (DUAL) a.dz[(a.N + n) * kRowPad + lane] = 0.f;
   }
-  if (DUAL) v *= w;
-  else v = v * a.scale + in;
-  static_cast<T *>(a.out)[lane * a.ldo + n] = from_f<T>(v);
+  if (lane >= a.M) return;
+  finish<T, DUAL>(a, lane, n, v, w);
+}
+
+bool few_mma(const FewRows &a) {
+  return a.dt != DT_F32 && a.K % 8 == 0 && rows16(a.x, a.ldx, a.dt) && rows16(a.w0, a.ldw0, a.dt) &&
+         (!a.w1 || rows16(a.w1, a.ldw1, a.dt));
 }
 
 template <typename T, int MR, bool DUAL>
@@ -144,18 +262,40 @@ void launch_rows(const FewRows &a, cudaStream_t s) {
 }
 template <typename T, bool DUAL>
 void rows_of(const FewRows &a, cudaStream_t s) {
+  if constexpr (sizeof(T) == 2) {
+    if (few_mma(a)) {
+      const unsigned grid = static_cast<unsigned>((a.N + 15) / 16);
+      if (a.M <= 8) k_few_mma<T, 1, DUAL><<<grid, 256, 0, s>>>(a);
+      else k_few_mma<T, 2, DUAL><<<grid, 256, 0, s>>>(a);
+      CUDA_LAUNCH_CHECK();
+      return;
+    }
+  }
   if (a.M == 1) launch_rows<T, 1, DUAL>(a, s);
   else if (a.M <= 4) launch_rows<T, 4, DUAL>(a, s);
   else launch_rows<T, kFewRows, DUAL>(a, s);
 }
 
+__device__ __forceinline__ void load_dz(const float *dz, int64_t n, float (&z)[kRowPad]) {
+  const float4 a = __ldg(reinterpret_cast<const float4 *>(dz + n * kRowPad)),
+               b = __ldg(reinterpret_cast<const float4 *>(dz + n * kRowPad) + 1);
+  z[0] = a.x;
+  z[1] = a.y;
+  z[2] = a.z;
+  z[3] = a.w;
+  z[4] = b.x;
+  z[5] = b.y;
+  z[6] = b.z;
+  z[7] = b.w;
+}
+
 // dz of a linear layer without an activation.
 template <typename T>
 __global__ void __launch_bounds__(256) k_rows_dz(const FewRows a) {
-  const int64_t all = a.M * a.N;
+  const int64_t all = kRowPad * a.N;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t m = i / a.N;
-    a.dz[i] = a.scale * to_f(static_cast<const T *>(a.in)[m * a.ldin + (i - m * a.N)]);
+    const int64_t n = i / kRowPad, m = i % kRowPad;
+    a.dz[i] = m < a.M ? a.scale * to_f(static_cast<const T *>(a.in)[m * a.ldin + n]) : 0.f;
   }
 }
 
@@ -169,45 +309,57 @@ __global__ void __launch_bounds__(256) k_rows_dw(const FewRows a) {
   T *dw = static_cast<T *>(blockIdx.z ? a.dw1 : a.dw0);
   T *db = static_cast<T *>(blockIdx.z ? a.db1 : a.db0);
   const int64_t ld = blockIdx.z ? a.lddw1 : a.lddw0;
-  const float *dz = a.dz + blockIdx.z * a.M * a.N;
+  const float *dz = a.dz + blockIdx.z * a.N * kRowPad;
   if (db && blockIdx.x == 0)
     for (int64_t n = static_cast<int64_t>(blockIdx.y) * 256 + threadIdx.x; n < a.N; n += static_cast<int64_t>(gridDim.y) * 256) {
       float t = 0.f;
-      for (int m = 0; m < a.M; ++m) t += dz[m * a.N + n];
+      for (int m = 0; m < a.M; ++m) t += dz[n * kRowPad + m];
       db[n] = from_f<T>(t);
     }
   const int64_t k = ((static_cast<int64_t>(blockIdx.x) * 8 + warp) * 32 + lane) * V;
   if (!dw || k >= a.K) return;
-  float x[kFewRows][V];
+  constexpr int P = V > 1 ? V / 2 : 1;  // pairs of columns (V = 1: .y unused)
+  float2 x[kRowPad][P];
 #pragma unroll
-  for (int m = 0; m < kFewRows; ++m) {
-    const T *p = static_cast<const T *>(a.x) + m * a.ldx + k;
+  for (int m = 0; m < kRowPad; ++m) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) x[m][j] = 0.f;
+    for (int j = 0; j < P; ++j) x[m][j] = make_float2(0.f, 0.f);
     if (m >= a.M) continue;
+    const T *p = static_cast<const T *>(a.x) + m * a.ldx + k;
     if constexpr (VEC) {
       float f[16 / sizeof(T)];
       unpack<T>(__ldg(reinterpret_cast<const uint4 *>(p)), f);
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[m][j] = f[j];
+      for (int j = 0; j < P; ++j) x[m][j] = make_float2(f[2 * j], f[2 * j + 1]);
     } else {
-      x[m][0] = to_f(*p);
+      x[m][0].x = to_f(*p);
     }
   }
-  for (int64_t n0 = static_cast<int64_t>(blockIdx.y) * kStrip; n0 < a.N; n0 += static_cast<int64_t>(gridDim.y) * kStrip)
-  for (int64_t n = n0; n < min(a.N, n0 + kStrip); ++n) {
-    float v[VEC ? 16 / sizeof(T) : 1];
+  for (int64_t s0 = static_cast<int64_t>(blockIdx.y) * kStrip; s0 < a.N; s0 += static_cast<int64_t>(gridDim.y) * kStrip) {
+    const int64_t s1 = min(a.N, s0 + kStrip);
+#pragma unroll 4
+    for (int64_t n = s0; n < s1; ++n) {
+      float z[kRowPad];
+      load_dz(dz, n, z);
+      float2 v[P];
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = 0.f;
+      for (int j = 0; j < P; ++j) v[j] = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int m = 0; m < kFewRows; ++m) {
-      if (m >= a.M) break;
-      const float g = __ldg(dz + m * a.N + n);
+      for (int m = 0; m < kRowPad; ++m)
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = fmaf(g, x[m][j], v[j]);
+        for (int j = 0; j < P; ++j) v[j] = __ffma2_rn(make_float2(z[m], z[m]), x[m][j], v[j]);
+      if constexpr (VEC) {
+        float f[16 / sizeof(T)];
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+          f[2 * j] = v[j].x;
+          f[2 * j + 1] = v[j].y;
+        }
+        *reinterpret_cast<uint4 *>(dw + n * ld + k) = pack<T>(f);
+      } else {
+        dw[n * ld + k] = from_f<T>(v[0].x);
+      }
     }
-    if constexpr (VEC) *reinterpret_cast<uint4 *>(dw + n * ld + k) = pack<T>(v);
-    else dw[n * ld + k] = from_f<T>(v[0]);
   }
 }
 
@@ -220,37 +372,43 @@ __global__ void __launch_bounds__(256) k_rows_dx(const FewRows a, int64_t strip,
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t k0 = static_cast<int64_t>(blockIdx.x) * 32 * V, k = k0 + lane * V;
   const int64_t n0 = blockIdx.y * strip, n1 = min(a.N, n0 + strip);
-  float acc[kFewRows][V];
+  constexpr int P = V > 1 ? V / 2 : 1;
+  float2 acc[kRowPad][P];
 #pragma unroll
-  for (int m = 0; m < kFewRows; ++m)
+  for (int m = 0; m < kRowPad; ++m)
 #pragma unroll
-    for (int j = 0; j < V; ++j) acc[m][j] = 0.f;
+    for (int j = 0; j < P; ++j) acc[m][j] = make_float2(0.f, 0.f);
   for (int q = 0; q < (a.w1 ? 2 : 1); ++q) {
     const T *w = static_cast<const T *>(q ? a.w1 : a.w0) + k;
     const int64_t ld = q ? a.ldw1 : a.ldw0;
-    const float *dz = a.dz + q * a.M * a.N;
+    const float *dz = a.dz + q * a.N * kRowPad;
     if (k < a.K) {
 #pragma unroll 4
       for (int64_t n = n0 + warp; n < n1; n += 8) {
-        float f[VEC ? 16 / sizeof(T) : 1];
-        if constexpr (VEC) unpack<T>(__ldg(reinterpret_cast<const uint4 *>(w + n * ld)), f);
-        else f[0] = to_f(w[n * ld]);
+        float2 f[P];
+        if constexpr (VEC) {
+          float u[16 / sizeof(T)];
+          unpack<T>(__ldg(reinterpret_cast<const uint4 *>(w + n * ld)), u);
 #pragma unroll
-        for (int m = 0; m < kFewRows; ++m) {
-          if (m >= a.M) break;
-          const float g = __ldg(dz + m * a.N + n);
-#pragma unroll
-          for (int j = 0; j < V; ++j) acc[m][j] = fmaf(g, f[j], acc[m][j]);
+          for (int j = 0; j < P; ++j) f[j] = make_float2(u[2 * j], u[2 * j + 1]);
+        } else {
+          f[0] = make_float2(to_f(w[n * ld]), 0.f);
         }
+        float z[kRowPad];
+        load_dz(dz, n, z);
+#pragma unroll
+        for (int m = 0; m < kRowPad; ++m)
+#pragma unroll
+          for (int j = 0; j < P; ++j) acc[m][j] = __ffma2_rn(make_float2(z[m], z[m]), f[j], acc[m][j]);
       }
     }
   }
 #pragma unroll
-  for (int m = 0; m < kFewRows; ++m) {
+  for (int m = 0; m < kRowPad; ++m) {
     if (m >= a.M) break;
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < V; ++j) sums[warp][lane * V + j] = acc[m][j];
+    for (int j = 0; j < V; ++j) sums[warp][lane * V + j] = j % 2 ? acc[m][j / 2].y : acc[m][j / 2].x;
     __syncthreads();
     for (int i = threadIdx.x; i < 32 * V; i += 256) {
       if (k0 + i >= a.K) continue;
@@ -292,7 +450,7 @@ void bwd_of(const FewRows &a, cudaStream_t s) {
     z.out = nullptr;
     a.w1 ? rows_of<T, true>(z, s) : rows_of<T, false>(z, s);
   } else {
-    k_rows_dz<T><<<blocks_for(a.M * a.N), 256, 0, s>>>(a);
+    k_rows_dz<T><<<blocks_for(kRowPad * a.N), 256, 0, s>>>(a);
     CUDA_LAUNCH_CHECK();
   }
   if (a.dw0 || a.dw1 || a.db0 || a.db1) {
@@ -310,7 +468,7 @@ void bwd_of(const FewRows &a, cudaStream_t s) {
   const bool vec = a.K % V == 0 && rows16(a.w0, a.ldw0, a.dt) && (!a.w1 || rows16(a.w1, a.ldw1, a.dt));
   const int y = dx_strips(a);
   const int64_t strip = (a.N + y - 1) / y, span = 32LL * (vec ? V : 1);
-  float *part = a.dz + (a.w1 ? 2 : 1) * a.M * a.N;
+  float *part = a.dz + (a.w1 ? 2 : 1) * a.N * kRowPad;
   const dim3 g(static_cast<unsigned>((a.K + span - 1) / span), y);
   if (vec) k_rows_dx<T, true><<<g, 256, 0, s>>>(a, strip, part);
   else k_rows_dx<T, false><<<g, 256, 0, s>>>(a, strip, part);
@@ -422,6 +580,8 @@ void column_parts(const void *p, int dt, int64_t ld, int64_t M, int64_t N, int y
 
 }  // namespace
 
+bool few_rows_fit(const FewRows &a) { return a.M <= (few_mma(a) ? 16 : kFewRows); }
+
 void few_rows(const FewRows &a, cudaStream_t s) {
   if (a.dt == DT_F32) a.w1 ? rows_of<float, true>(a, s) : rows_of<float, false>(a, s);
   else if (a.dt == DT_F16) a.w1 ? rows_of<__half, true>(a, s) : rows_of<__half, false>(a, s);
@@ -429,7 +589,7 @@ void few_rows(const FewRows &a, cudaStream_t s) {
 }
 
 size_t few_rows_floats(const FewRows &a) {
-  return static_cast<size_t>(a.M) * ((a.w1 ? 2 : 1) * a.N + dx_strips(a) * a.K);
+  return static_cast<size_t>(a.w1 ? 2 : 1) * a.N * kRowPad + static_cast<size_t>(a.M) * dx_strips(a) * a.K;
 }
 
 void few_rows_bwd(const FewRows &a, cudaStream_t s) {

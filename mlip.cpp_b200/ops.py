@@ -140,8 +140,8 @@ def _gated_inputs(x, w_gate, w_value, b_gate, b_value, activation, keep):
     px, lx = _take(x, x, x.shape, k, keep, "x")
     pg, lg = _take(w_gate, x, w_gate.shape, k, keep, "w_gate")
     pv, lv = _take(w_value, x, w_gate.shape, k, keep, "w_value")
-    pbg, _ = _take(b_gate, x, (f,), f, keep, "b_gate")
-    pbv, _ = _take(b_value, x, (f,), f, keep, "b_value")
+    pbg = 0 if b_gate is None else _take(b_gate, x, (f,), f, keep, "b_gate")[0]
+    pbv = 0 if b_value is None else _take(b_value, x, (f,), f, keep, "b_value")[0]
     m = x.numel() // k
     return m, k, f, (dt, act, m, k, f, px, pg, pv, pbg, pbv, lx, lg, lv)
 
@@ -198,7 +198,7 @@ def _linear_inputs(x, w, bias, activation, residual, scale, keep):
         _refuse("there must be at least one feature")
     px, lx = _take(x, x, x.shape, k, keep, "x")
     pw, lw = _take(w, x, w.shape, k, keep, "w")
-    pb, _ = _take(bias, x, (n,), n, keep, "bias")
+    pb = 0 if bias is None else _take(bias, x, (n,), n, keep, "bias")[0]
     pr, lr = (0, n) if residual is None else _take(residual, x, x.shape[:-1] + (n,), n, keep, "residual")
     m = x.numel() // k
     return m, k, n, (dt, act, m, k, n, scale, px, pw, pb, pr, lx, lw, lr)
@@ -257,15 +257,18 @@ def _norm_inputs(residual, y, weight, bias, post_weight, post_bias, gate, scale,
     if y is None and (kinds[1] or gate is not None):
         _refuse("a post norm or a gate needs y")
     pr, lr = _take(residual, residual, shape, d, keep, "residual")
-    py, ly = _take(y, residual, shape, d, keep, "y")
-    vec = (_take(weight, residual, (d,), d, keep, "weight")[0], _take(bias, residual, (d,), d, keep, "bias")[0],
-           _take(post_weight, residual, (d,), d, keep, "post_weight")[0],
-           _take(post_bias, residual, (d,), d, keep, "post_bias")[0])
-    channel = gate is not None and gate.dim() == 1
-    pg, lg = _take(gate, residual, (d,) if channel else shape, d, keep, "gate")
-    if channel or gate is None:
-        lg = 0
-    return d, (dt, *kinds, residual.numel() // d, d, scale, eps, pr, py, *vec, pg, lr, ly, lg)
+    py, ly = (0, d) if y is None else _take(y, residual, shape, d, keep, "y")
+    pw = 0 if weight is None else _take(weight, residual, (d,), d, keep, "weight")[0]
+    pb = 0 if bias is None else _take(bias, residual, (d,), d, keep, "bias")[0]
+    ppw = 0 if post_weight is None else _take(post_weight, residual, (d,), d, keep, "post_weight")[0]
+    ppb = 0 if post_bias is None else _take(post_bias, residual, (d,), d, keep, "post_bias")[0]
+    pg = lg = 0
+    if gate is not None:
+        channel = gate.dim() == 1
+        pg, lg = _take(gate, residual, (d,) if channel else shape, d, keep, "gate")
+        if channel:
+            lg = 0
+    return d, (dt, *kinds, residual.numel() // d, d, scale, eps, pr, py, pw, pb, ppw, ppb, pg, lr, ly, lg)
 
 
 class _ResidualNorm(torch.autograd.Function):
@@ -297,7 +300,8 @@ def residual_norm(residual, y=None, weight=None, bias=None, post_weight=None, po
                                    eps)
     keep: list = []
     d, fields = _norm_inputs(residual, y, weight, bias, post_weight, post_bias, gate, scale, norm, post_norm, eps, keep)
-    stream, out = residual.new_empty(residual.shape), residual.new_empty(residual.shape)
+    stream, out = torch.empty_like(residual, memory_format=torch.contiguous_format), torch.empty_like(
+        residual, memory_format=torch.contiguous_format)
     _call("residual_norm", _NORM.pack(*fields, stream.data_ptr(), out.data_ptr(), d, d, 0, 0, d, d,
                                       0, 0, 0, 0, 0, 0, 0, d, d, d), residual.get_device(), False)
     return stream, out
