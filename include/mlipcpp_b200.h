@@ -207,7 +207,7 @@ mlipcpp_error_t mlipcpp_b200_domain_stats(mlipcpp_b200_domain_t domain, double s
  * current device, aligned to their elements; rows whose address and stride
  * are multiples of 16 bytes are read where they lie, others cost a copy.  A
  * call may have no rows (gradients of weights are then zeros); features are
- * at least 1, and rows and features below 2^31.  Outputs must not overlap
+ * at least 1, and both at most 2147482624.  Outputs must not overlap
  * inputs, but for a residual that is also the output with the same stride.
  *
  * Products accumulate in fp32; activations, norms and sums run in fp32 and

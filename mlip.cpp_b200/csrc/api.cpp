@@ -152,7 +152,8 @@ struct OpCheck {
 // At most one row: its stride says nothing; one that keeps 16-byte rows.
 int64_t op_ld(int64_t ld, int64_t rows, int64_t cols) { return rows > 1 ? ld : (cols + 7) / 8 * 8; }
 
-constexpr int64_t kOpMax = 2147483647;
+// (indices within a tile past the last row or feature stay below 2^31)
+constexpr int64_t kOpMax = 2147482624;
 
 mlipcpp_error_t op_args(const mlipcpp_b200_gated_linear_t *a, bool back, pet::GatedLinear &o) {
   OpCheck c;
@@ -1183,6 +1184,7 @@ mlipcpp_error_t mlipcpp_b200_set_wait_bound_ns(uint64_t ns) {
   }
   try {
     pet::set_gemm_wait_bound_ns(ns);
+    pet::set_block_wait_bound_ns(ns);
   } catch (const pet::Error &e) {
     set_error(e.what());
     return static_cast<mlipcpp_error_t>(e.code);

@@ -19,6 +19,19 @@ inline bool rows16(const void *p, int64_t ld, int dt) {
 }
 // SMs of the current device.
 int sm_count();
+// Reads and clears a device error word after the work on s.
+inline int take_error(const int &word, cudaStream_t s) {
+  int v = 0;
+  CUDA_CHECK(cudaMemcpyFromSymbolAsync(&v, word, sizeof(v), 0, cudaMemcpyDeviceToHost, s));
+  CUDA_CHECK(cudaStreamSynchronize(s));
+  if (v) {
+    const int zero = 0;
+    CUDA_CHECK(cudaMemcpyToSymbolAsync(word, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s));
+    CUDA_CHECK(cudaStreamSynchronize(s));
+  }
+  return v;
+}
+int norm_error(cudaStream_t s);  // of the norms' rings (block_norm.cu)
 
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }

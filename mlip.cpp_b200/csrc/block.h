@@ -14,8 +14,6 @@
 #include <cstddef>
 #include <cstdint>
 
-#include "kernels.cuh"
-
 namespace pet {
 
 enum DType : int { DT_F32 = 0, DT_F16 = 1, DT_BF16 = 2 };
@@ -60,10 +58,9 @@ struct GatedLinear {
   Mat dh;
   MutMat dx, dwg, dwv;
   void *dbg = nullptr, *dbv = nullptr;
-  // f32 only, optional: x, and the weights and their transposes, already in
-  // split-fp16 form (one scale exponent per weight matrix).  products 1
-  // multiplies the hi parts alone (the model's reduced-precision mode).
-  const Split16View *x_split = nullptr;
+  // f32 only, optional: the weights already in split-fp16 form (one scale
+  // exponent per matrix).  products 1 multiplies the hi parts alone (the
+  // model's reduced-precision mode).
   struct SplitWeight {
     const uint16_t *hi = nullptr, *lo = nullptr;
     int scale = 0;
@@ -101,8 +98,7 @@ struct ResidualNorm {
   float scale = 1.f, eps = 1e-5f;
   Mat residual, y, gate;
   const void *w = nullptr, *b = nullptr, *pw = nullptr, *pb = nullptr;
-  MutMat stream, out;              // each optional
-  const Split16View *out_split = nullptr;  // f32: also out in split form (d a multiple of 128)
+  MutMat stream, out;  // each optional
   // backward: dstream and dout in (null: zero); gradients out unless null
   Mat dstream, dout;
   MutMat dresidual, dy, dgate;
@@ -112,8 +108,10 @@ void residual_norm_fwd(const ResidualNorm &a, Workspace &ws, cudaStream_t s);
 void residual_norm_bwd(const ResidualNorm &a, Workspace &ws, cudaStream_t s);
 constexpr int kMaxNormDim = 16384;
 
-// Error word of the operators' tensor-core pipelines on the current device:
-// nonzero once a bounded wait ran out.  Synchronises `s`, reads and clears it.
+// Error word of the operators' pipelines on the current device: nonzero once a
+// bounded wait ran out.  Synchronises `s`, reads and clears it.
 int block_status(cudaStream_t s);
+// Bound on the waits of the tensor-core pipelines (0: the default).
+void set_block_wait_bound_ns(uint64_t ns);
 
 }  // namespace pet

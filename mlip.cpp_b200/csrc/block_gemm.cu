@@ -89,7 +89,7 @@ struct EpiArgs {
   int64_t ldin;
   void *out0, *out1;      // out1: E_GATED_BWD's dv, batch2's second product
   int64_t ldo;
-  int dt, act;
+  int act;
   float scale;
   float *sums0, *sums1;   // E_*_BWD, or null: column sums of each 32 rows of the
                           // results before they are rounded, [row / 32][N]
@@ -963,18 +963,6 @@ struct Operand {
   float bsc = 1.f;             // f32 B without sc: one factor
 };
 
-Operand from_split(const Split16View &v) {
-  Operand o;
-  o.p = v.hi;
-  o.rows = v.rows;
-  o.cols = o.ld = v.cols;
-  o.planes = v.lo ? 2 : 1;
-  o.plane = v.lo ? v.lo - v.hi : 0;
-  o.sc = v.sc;
-  o.scld = split_ld(v);
-  return o;
-}
-
 // Prepares operands: 16-bit ones where they lie (or packed), f32 ones in split
 // form, by one launch each, issued by go().
 enum Form { FORM_NONE, FORM_ROWS, FORM_COLS, FORM_BLOCKS };
@@ -1182,7 +1170,6 @@ void run(const Product &g, Workspace &ws, cudaStream_t s) {
   p.products = g.products;
   p.err = g.err;
   p.e = g.e;
-  p.e.dt = g.dt;
   // tiles of bm rows of `bn` accumulator columns
   auto count = [&](int bm, int bn) {
     const int on = g.dual ? bn / 2 : bn;
@@ -1300,15 +1287,13 @@ void *Workspace::take(size_t bytes) {
 }
 
 int block_status(cudaStream_t s) {
-  int v = 0;
-  CUDA_CHECK(cudaMemcpyFromSymbolAsync(&v, g_block_err, sizeof(v), 0, cudaMemcpyDeviceToHost, s));
-  CUDA_CHECK(cudaStreamSynchronize(s));
-  if (v) {
-    const int zero = 0;
-    CUDA_CHECK(cudaMemcpyToSymbolAsync(g_block_err, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s));
-    CUDA_CHECK(cudaStreamSynchronize(s));
-  }
-  return v;
+  const int a = take_error(g_block_err, s), b = norm_error(s);
+  return a | b;
+}
+
+void set_block_wait_bound_ns(uint64_t ns) {
+  const uint64_t v = ns ? ns : tc::kWaitNs;
+  CUDA_CHECK(cudaMemcpyToSymbol(tc::g_wait_ns, &v, sizeof(v)));
 }
 
 namespace {
@@ -1367,7 +1352,7 @@ void few_bwd(FewRows &f, Workspace &ws, cudaStream_t s) {
 
 void gated_linear_fwd(const GatedLinear &a, Workspace &ws, cudaStream_t s) {
   if (a.M == 0) return;
-  if (FewRows f = few_of(a); !a.x_split && few_rows_fit(f)) {
+  if (FewRows f = few_of(a); few_rows_fit(f)) {
     if (ws.sizing()) return;
     f.out = a.h.p;
     f.ldo = a.h.ld;
@@ -1384,7 +1369,7 @@ void gated_linear_fwd(const GatedLinear &a, Workspace &ws, cudaStream_t s) {
   g.N = a.F;
   g.K = a.K;
   g.dual = true;
-  g.a[0] = a.x_split ? from_split(*a.x_split) : prep.add(a.x, a.M, a.K, FORM_ROWS);
+  g.a[0] = prep.add(a.x, a.M, a.K, FORM_ROWS);
   g.b[0] = a.wg_split.hi ? split_weight(a.wg_split, a.F, a.K) : prep.add(a.wg, a.F, a.K, FORM_BLOCKS);
   g.b[1] = a.wv_split.hi ? split_weight(a.wv_split, a.F, a.K) : prep.add(a.wv, a.F, a.K, FORM_BLOCKS);
   g.e = plain_out(a.h);
@@ -1410,7 +1395,7 @@ void gated_linear_bwd(const GatedLinear &a, Workspace &ws, cudaStream_t s) {
   }
   const bool weights = a.dwg.p || a.dwv.p;
   if (!a.dx.p && !weights && !a.dbg && !a.dbv) return;
-  if (a.M <= kFewRows && !a.x_split) {
+  if (a.M <= kFewRows) {
     FewRows f = few_of(a);
     f.in = a.dh.p;
     f.ldin = a.dh.ld;
@@ -1438,7 +1423,7 @@ void gated_linear_bwd(const GatedLinear &a, Workspace &ws, cudaStream_t s) {
   g.dt = a.dtype;
   g.products = a.products;
   g.err = a.err;
-  g.a[0] = a.x_split ? from_split(*a.x_split) : prep.add(a.x, a.M, a.K, FORM_ROWS);
+  g.a[0] = prep.add(a.x, a.M, a.K, FORM_ROWS);
   if (weights) xb = f32 ? prep.add(a.x, a.M, a.K, FORM_BLOCKS) : g.a[0];
   g.epi = E_GATED_BWD;
   g.M = a.M;

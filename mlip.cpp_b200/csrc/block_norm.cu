@@ -25,7 +25,6 @@
 #include <type_traits>
 
 #include "block.cuh"
-#include "split16.cuh"
 #include "tc_common.cuh"
 
 namespace pet {
@@ -42,7 +41,6 @@ struct NormArgs {
   const void *w, *b, *pw, *pb;
   void *stream, *out;
   int64_t lds, ldo;
-  Split16View split;
   const void *ds, *dout;
   int64_t ldds, lddo;
   void *dr, *dy, *dgate;       // dgate: the gate of each row
@@ -97,14 +95,14 @@ __device__ __forceinline__ uint4 close16(const float2 *x) {
 template <typename T, int TPR, int E, bool VEC, bool FULL = false>
 struct Row {
   static constexpr int V = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
-  static constexpr int NV = E / V, P = E / 2;
+  static constexpr int P = E / 2;
   static __device__ __forceinline__ int col(int i, int t) { return (i * TPR + t) * V; }
   // elements of one row at p + off; zeros past d (VEC: d is a multiple of V)
   static __device__ __forceinline__ void load(const void *p, int64_t off, int t, int d, float2 (&x)[P]) {
     const T *q = static_cast<const T *>(p) + off;
     if constexpr (VEC) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
+      for (int i = 0; i < E / V; ++i) {
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
         if (FULL || col(i, t) < d) v = *reinterpret_cast<const uint4 *>(q + col(i, t));
         open16<T>(v, &x[i * V / 2]);
@@ -121,7 +119,7 @@ struct Row {
     T *q = static_cast<T *>(p) + off;
     if constexpr (VEC) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
+      for (int i = 0; i < E / V; ++i)
         if (FULL || col(i, t) < d) *reinterpret_cast<uint4 *>(q + col(i, t)) = close16<T>(&x[i * V / 2]);
     } else {
 #pragma unroll
@@ -406,23 +404,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_norm_fwd(const NormArgs a, co
       feed.give(row);
     }
     if (a.stream) R::store(a.stream, row * a.lds, t, d, x);
-    if (!a.out && !a.split.hi) continue;
+    if (!a.out) continue;
     if (a.norm != NORM_NONE) normalise<R, TPR>(a.norm, a.eps, d, rd, t, sum, x);
     vec.times_w(t, x);
     vec.plus_b(t, x);
     if (a.out) R::store(a.out, row * a.ldo, t, d, x);
-    if constexpr (sizeof(T) == 4 && MODE != 0) {
-      // a warp's 16-byte chunks are one 128-column block
-      if (a.split.hi) {
-#pragma unroll
-        for (int i = 0; i < R::NV; ++i) {
-          const int blk = R::col(i, t) / 128;
-          if (blk * 128 < d)
-            warp_split_block(a.split, static_cast<int>(row), blk, make_float4(x[2 * i].x, x[2 * i].y, x[2 * i + 1].x, x[2 * i + 1].y),
-                             threadIdx.x & 31);
-        }
-      }
-    }
   }
 }
 
@@ -742,6 +728,8 @@ NormArgs args_of(const ResidualNorm &a) {
 
 using namespace blk;
 
+int blk::norm_error(cudaStream_t s) { return take_error(g_norm_err, s); }
+
 void residual_norm_fwd(const ResidualNorm &a, Workspace &ws, cudaStream_t s) {
   if (a.M == 0 || ws.sizing()) return;
   NormArgs n = args_of(a);
@@ -750,10 +738,6 @@ void residual_norm_fwd(const ResidualNorm &a, Workspace &ws, cudaStream_t s) {
   n.out = a.out.p;
   n.ldo = a.out.ld;
   const bool vec = vectorised(a);
-  if (a.out_split) {
-    if (a.dtype != DT_F32 || !vec || a.d % 128) throw Error(kErrInternal, "residual_norm: split output needs aligned f32 rows");
-    n.split = *a.out_split;
-  }
   by_type<false>(a.dtype, vec, n, layout_of(n, a.dtype, vec, false), s);
 }
 

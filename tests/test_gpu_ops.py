@@ -590,3 +590,25 @@ def test_rows_beyond_the_call_stay(dtype):
             ops._call("linear", args, 0, False)
             assert (y[m:] == 5).all() and (y[:, :pad] == 5).all() and (y[:, pad + 70:] == 5).all()
             assert torch.equal(y[:m, pad:pad + 70], ops.linear(x[:m], w))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("m", [150, 4101])
+def test_expired_wait_is_reported(dtype, m):
+    """With a bound of a nanosecond on every wait the pipelines give up: the
+    call's status says so once, and the next call is whole again."""
+    x, r, p = block_inputs(81, dtype, rows=(m,), f=1100)
+    want = ops.gated_linear(x, p["wg"], p["wv"], p["bg"])
+    ops.check_status()
+    L = mb.lib()
+    assert L.mlipcpp_b200_set_wait_bound_ns(1) == mb.OK
+    try:
+        ops.gated_linear(x, p["wg"], p["wv"], p["bg"])
+        with pytest.raises(mb.MLIPError) as e:
+            ops.check_status()
+        assert e.value.code == mb.COMPUTATION
+    finally:
+        assert L.mlipcpp_b200_set_wait_bound_ns(0) == mb.OK
+    ops.check_status()
+    assert torch.equal(ops.gated_linear(x, p["wg"], p["wv"], p["bg"]), want)
+    ops.check_status()
