@@ -574,7 +574,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 2 : 1) k_norm_bwd(const NormAr
 }
 
 // The vectors' gradients from the CTAs' sums, in a fixed order; block: 32
-// columns x 8 interleaved shares.
+// columns x 32 interleaved shares.
 //   dw = sum do n, db = sum do;  with one gate for all rows (or none)
 //   dpw = gate sum q u, dpb = gate sum q, dgate = pw sum q u + pb sum q.
 struct VectorGrads {
@@ -584,16 +584,16 @@ struct VectorGrads {
   const void *pw, *pb, *gate;  // gate: of one row, or null
   void *dw, *db, *dpw, *dpb, *dgate;
 };
-__global__ void __launch_bounds__(256) k_norm_vectors(const VectorGrads a) {
-  __shared__ float sums[4][8][33];
+__global__ void __launch_bounds__(1024) k_norm_vectors(const VectorGrads a) {
+  __shared__ float sums[4][32][33];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int c = blockIdx.x * 32 + lane, na = a.hb ? 4 : 2;
   for (int v = 0; v < na; ++v) {
     float s = 0.f;
     if (c < a.d) {
       const float *p = a.part + static_cast<size_t>(v) * a.P * a.d + c;
-#pragma unroll 16
-      for (int q = warp; q < a.P; q += 8) s += p[static_cast<size_t>(q) * a.d];
+#pragma unroll 8
+      for (int q = warp; q < a.P; q += 32) s += p[static_cast<size_t>(q) * a.d];
     }
     sums[v][warp][lane] = s;
   }
@@ -602,7 +602,7 @@ __global__ void __launch_bounds__(256) k_norm_vectors(const VectorGrads a) {
   float s[4] = {0.f, 0.f, 0.f, 0.f};
   for (int v = 0; v < na; ++v)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s[v] += sums[v][i][lane];
+    for (int i = 0; i < 32; ++i) s[v] += sums[v][i][lane];
   const float gate = a.gate ? load_dt(a.gate, a.dt, c) : 1.f;
   if (a.dw) store_dt(a.dw, a.dt, c, s[0]);
   if (a.db) store_dt(a.db, a.dt, c, s[2]);
@@ -637,9 +637,12 @@ Layout layout_of(const NormArgs &a, int dt, bool vec, bool bwd) {
   if (vec) {
     Ring &r = l.ring;
     for (const void *p : {a.r, a.y, a.ds, a.dout, a.ldg ? a.gate : nullptr}) r.inputs += p ? 1 : 0;
+    // the kernels' own arrays (slots, barriers, the groups' sums) and what the
+    // system keeps of each CTA's shared memory
+    const int fixed = 2048 + 320 * groups + (bwd && groups > 1 ? 4 * l.tpr * e : 0);
     // at least two stages, fewer CTAs rather than fewer stages
     for (; per_sm >= 1; --per_sm) {
-      const int room = kSmemPerSm / per_sm - 15 * 1024 - r.vector_bytes;
+      const int room = kSmemPerSm / per_sm - fixed - r.vector_bytes;
       r.stages = std::min(kMaxStages, room / (groups * r.inputs * r.row_bytes));
       if (r.stages >= 2) break;
     }
@@ -770,7 +773,7 @@ void residual_norm_bwd(const ResidualNorm &a, Workspace &ws, cudaStream_t s) {
   if (!vectors) return;
   const VectorGrads v{n.part, l.grid, a.d, a.dtype, n.hb, a.pw, a.pb, a.gate.ld == 0 ? a.gate.p : nullptr,
                       a.dw, a.db, a.dpw, a.dpb, dgate};
-  k_norm_vectors<<<ceil_div(a.d, 32), 256, 0, s>>>(v);
+  k_norm_vectors<<<ceil_div(a.d, 32), 1024, 0, s>>>(v);
   CUDA_LAUNCH_CHECK();
 }
 
