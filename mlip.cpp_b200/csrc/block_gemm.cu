@@ -35,6 +35,13 @@
 // over CTAs, partial sums to the workspace and a second kernel that adds them
 // in order and runs the epilogue, for outputs of few tiles).
 //
+// What bounds it: 16-bit, 8192 x 1024 x 8192 bf16 in 99 us (1.39 PFLOP/s, 72% of
+// the tensor pipe): 128 pair tiles in two waves of 74.  With the gated backward's
+// epilogue (two outputs, an input and the activation for every two columns) the
+// same work takes 129 us.  f32: 128 x 128 tiles read 128 bytes of shared memory a
+// cycle for the MMAs and write 85 more by TMA, so 65,202 x 512 x 2048 takes 365 us
+// (59% of the pipe, 375 TFLOP/s of fp32-accurate products).
+//
 // Every wait is bounded; on expiry the CTA records an error, waits for its
 // own loads and MMAs, frees its tensor memory and returns.
 #include <cuda.h>
