@@ -151,9 +151,11 @@ __global__ void __launch_bounds__(256) k_few_rows(const FewRows a, int wpr) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t n = static_cast<int64_t>(blockIdx.x) * (8 / wpr) + warp / wpr;
   const int sub = warp % wpr;
-  float sum[NS];
+  // sums of even and of odd elements (VEC): two to an instruction
+  float2 pair[NS];
 #pragma unroll
-  for (int i = 0; i < NS; ++i) sum[i] = 0.f;
+  for (int i = 0; i < NS; ++i) pair[i] = make_float2(0.f, 0.f);
+  constexpr int D1 = DUAL ? MR : 0;  // the second product's sums
   if (n < a.N) {
     const T *x = static_cast<const T *>(a.x);
     const T *w0 = static_cast<const T *>(a.w0) + n * a.ldw0;
@@ -184,9 +186,10 @@ __global__ void __launch_bounds__(256) k_few_rows(const FewRows a, int wpr) {
             float xv[16 / sizeof(T)];
             unpack<T>(__ldg(reinterpret_cast<const uint4 *>(x + m * a.ldx + k)), xv);
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-              sum[m] = fmaf(xv[j], f0[j], sum[m]);
-              if (DUAL) sum[MR * (DUAL ? 1 : 0) + m] = fmaf(xv[j], f1[j], sum[MR * (DUAL ? 1 : 0) + m]);
+            for (int j = 0; j + 1 < V; j += 2) {
+              const float2 x2 = make_float2(xv[j], xv[j + 1]);
+              pair[m] = __ffma2_rn(x2, make_float2(f0[j], f0[j + 1]), pair[m]);
+              if (DUAL) pair[D1 + m] = __ffma2_rn(x2, make_float2(f1[j], f1[j + 1]), pair[D1 + m]);
             }
           }
         }
@@ -200,15 +203,16 @@ __global__ void __launch_bounds__(256) k_few_rows(const FewRows a, int wpr) {
           for (int m = 0; m < MR; ++m) {
             if (m >= a.M) break;
             const float xv = to_f(x[m * a.ldx + k]);
-            sum[m] = fmaf(xv, f0, sum[m]);
-            if (DUAL) sum[MR * (DUAL ? 1 : 0) + m] = fmaf(xv, f1, sum[MR * (DUAL ? 1 : 0) + m]);
+            pair[m].x = fmaf(xv, f0, pair[m].x);
+            if (DUAL) pair[D1 + m].x = fmaf(xv, f1, pair[D1 + m].x);
           }
         }
       }
     }
   }
+  float sum[NS];
 #pragma unroll
-  for (int i = 0; i < NS; ++i) sum[i] = warp_sum(sum[i]);
+  for (int i = 0; i < NS; ++i) sum[i] = warp_sum(pair[i].x + pair[i].y);
   if (wpr > 1) {
     if (lane == 0) {
 #pragma unroll
@@ -229,7 +233,7 @@ __global__ void __launch_bounds__(256) k_few_rows(const FewRows a, int wpr) {
   for (int m = 0; m < MR; ++m)
     if (lane == m) {
       v = sum[m];
-      if (DUAL) w = sum[MR * (DUAL ? 1 : 0) + m];
+      if (DUAL) w = sum[D1 + m];
     }
   if (n >= a.N) return;
   if (!a.out && lane >= a.M && lane < kRowPad) {
@@ -276,17 +280,21 @@ void rows_of(const FewRows &a, cudaStream_t s) {
   else launch_rows<T, kFewRows, DUAL>(a, s);
 }
 
-__device__ __forceinline__ void load_dz(const float *dz, int64_t n, float (&z)[kRowPad]) {
-  const float4 a = __ldg(reinterpret_cast<const float4 *>(dz + n * kRowPad)),
-               b = __ldg(reinterpret_cast<const float4 *>(dz + n * kRowPad) + 1);
-  z[0] = a.x;
-  z[1] = a.y;
-  z[2] = a.z;
-  z[3] = a.w;
-  z[4] = b.x;
-  z[5] = b.y;
-  z[6] = b.z;
-  z[7] = b.w;
+// dz of feature n: the first MR rows.
+template <int MR>
+__device__ __forceinline__ void load_dz(const float *dz, int64_t n, float (&z)[MR]) {
+  if constexpr (MR == 1) {
+    z[0] = __ldg(dz + n * kRowPad);
+  } else {
+#pragma unroll
+    for (int m = 0; m < MR; m += 4) {
+      const float4 a = __ldg(reinterpret_cast<const float4 *>(dz + n * kRowPad + m));
+      z[m] = a.x;
+      z[m + 1] = a.y;
+      z[m + 2] = a.z;
+      z[m + 3] = a.w;
+    }
+  }
 }
 
 // dz of a linear layer without an activation.
@@ -302,7 +310,7 @@ __global__ void __launch_bounds__(256) k_rows_dz(const FewRows a) {
 // dW[n][k] = sum over m of dz[m][n] x[m][k]; db[n] = sum of dz[m][n].  Block:
 // kStrip features n, 32 V columns k a warp and 8 of those; blockIdx.z: product.
 constexpr int kStrip = 16;
-template <typename T, bool VEC>
+template <typename T, int MR, bool VEC>
 __global__ void __launch_bounds__(256) k_rows_dw(const FewRows a) {
   constexpr int V = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -319,9 +327,9 @@ __global__ void __launch_bounds__(256) k_rows_dw(const FewRows a) {
   const int64_t k = ((static_cast<int64_t>(blockIdx.x) * 8 + warp) * 32 + lane) * V;
   if (!dw || k >= a.K) return;
   constexpr int P = V > 1 ? V / 2 : 1;  // pairs of columns (V = 1: .y unused)
-  float2 x[kRowPad][P];
+  float2 x[MR][P];
 #pragma unroll
-  for (int m = 0; m < kRowPad; ++m) {
+  for (int m = 0; m < MR; ++m) {
 #pragma unroll
     for (int j = 0; j < P; ++j) x[m][j] = make_float2(0.f, 0.f);
     if (m >= a.M) continue;
@@ -339,13 +347,13 @@ __global__ void __launch_bounds__(256) k_rows_dw(const FewRows a) {
     const int64_t s1 = min(a.N, s0 + kStrip);
 #pragma unroll 4
     for (int64_t n = s0; n < s1; ++n) {
-      float z[kRowPad];
-      load_dz(dz, n, z);
+      float z[MR];
+      load_dz<MR>(dz, n, z);
       float2 v[P];
 #pragma unroll
       for (int j = 0; j < P; ++j) v[j] = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int m = 0; m < kRowPad; ++m)
+      for (int m = 0; m < MR; ++m)
 #pragma unroll
         for (int j = 0; j < P; ++j) v[j] = __ffma2_rn(make_float2(z[m], z[m]), x[m][j], v[j]);
       if constexpr (VEC) {
@@ -365,17 +373,17 @@ __global__ void __launch_bounds__(256) k_rows_dw(const FewRows a) {
 
 // part[strip][m][k] = sum over the strip's features n of dz[m][n] W[n][k], over
 // both products; a strip of W's rows in eight interleaved shares, one a warp.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) k_rows_dx(const FewRows a, int64_t strip, float *part) {
+template <typename T, int MR, bool VEC>
+__global__ void __launch_bounds__(256, 2) k_rows_dx(const FewRows a, int64_t strip, float *part) {
   constexpr int V = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
   __shared__ float sums[8][32 * V];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t k0 = static_cast<int64_t>(blockIdx.x) * 32 * V, k = k0 + lane * V;
   const int64_t n0 = blockIdx.y * strip, n1 = min(a.N, n0 + strip);
   constexpr int P = V > 1 ? V / 2 : 1;
-  float2 acc[kRowPad][P];
+  float2 acc[MR][P];
 #pragma unroll
-  for (int m = 0; m < kRowPad; ++m)
+  for (int m = 0; m < MR; ++m)
 #pragma unroll
     for (int j = 0; j < P; ++j) acc[m][j] = make_float2(0.f, 0.f);
   for (int q = 0; q < (a.w1 ? 2 : 1); ++q) {
@@ -394,17 +402,17 @@ __global__ void __launch_bounds__(256) k_rows_dx(const FewRows a, int64_t strip,
         } else {
           f[0] = make_float2(to_f(w[n * ld]), 0.f);
         }
-        float z[kRowPad];
-        load_dz(dz, n, z);
+        float z[MR];
+        load_dz<MR>(dz, n, z);
 #pragma unroll
-        for (int m = 0; m < kRowPad; ++m)
+        for (int m = 0; m < MR; ++m)
 #pragma unroll
           for (int j = 0; j < P; ++j) acc[m][j] = __ffma2_rn(make_float2(z[m], z[m]), f[j], acc[m][j]);
       }
     }
   }
 #pragma unroll
-  for (int m = 0; m < kRowPad; ++m) {
+  for (int m = 0; m < MR; ++m) {
     if (m >= a.M) break;
     __syncthreads();
 #pragma unroll
@@ -419,15 +427,24 @@ __global__ void __launch_bounds__(256) k_rows_dx(const FewRows a, int64_t strip,
     }
   }
 }
+// dx from the strips' sums, in 32 interleaved shares; block: 32 elements.
 template <typename T>
-__global__ void __launch_bounds__(256) k_rows_join(const FewRows a, int strips, const float *part) {
+__global__ void __launch_bounds__(1024) k_rows_join(const FewRows a, int strips, const float *part) {
+  __shared__ float sums[32][33];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t all = a.M * a.K;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * 256) {
+  for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * 32; i0 < all; i0 += static_cast<int64_t>(gridDim.x) * 32) {
+    const int64_t i = i0 + lane;
     float t = 0.f;
-#pragma unroll 8
-    for (int s = 0; s < strips; ++s) t += part[s * all + i];
-    const int64_t m = i / a.K;
-    static_cast<T *>(a.dx)[m * a.lddx + (i - m * a.K)] = from_f<T>(t);
+    if (i < all)
+      for (int s = warp; s < strips; s += 32) t += part[s * all + i];
+    __syncthreads();
+    sums[warp][lane] = t;
+    __syncthreads();
+    // row `warp` of the transpose: the shares of one element
+    t = warp_sum(sums[lane][warp]);
+    const int64_t o = i0 + warp, m = o / a.K;
+    if (lane == 0 && o < all) static_cast<T *>(a.dx)[m * a.lddx + (o - m * a.K)] = from_f<T>(t);
   }
 }
 
@@ -442,7 +459,7 @@ int blocks_for(int64_t threads) {
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((threads + 255) / 256, 8LL * sm_count())));
 }
 
-template <typename T>
+template <typename T, int MR>
 void bwd_of(const FewRows &a, cudaStream_t s) {
   constexpr int V = 16 / static_cast<int>(sizeof(T));
   if (a.w1 || a.act != ACT_IDENTITY) {
@@ -460,8 +477,8 @@ void bwd_of(const FewRows &a, cudaStream_t s) {
     const int64_t strips = (a.N + kStrip - 1) / kStrip;
     const dim3 g(static_cast<unsigned>((a.K + span - 1) / span), static_cast<unsigned>(std::min<int64_t>(strips, 65535)),
                  a.w1 ? 2 : 1);
-    if (vec) k_rows_dw<T, true><<<g, 256, 0, s>>>(a);
-    else k_rows_dw<T, false><<<g, 256, 0, s>>>(a);
+    if (vec) k_rows_dw<T, MR, true><<<g, 256, 0, s>>>(a);
+    else k_rows_dw<T, MR, false><<<g, 256, 0, s>>>(a);
     CUDA_LAUNCH_CHECK();
   }
   if (!a.dx) return;
@@ -470,10 +487,10 @@ void bwd_of(const FewRows &a, cudaStream_t s) {
   const int64_t strip = (a.N + y - 1) / y, span = 32LL * (vec ? V : 1);
   float *part = a.dz + (a.w1 ? 2 : 1) * a.N * kRowPad;
   const dim3 g(static_cast<unsigned>((a.K + span - 1) / span), y);
-  if (vec) k_rows_dx<T, true><<<g, 256, 0, s>>>(a, strip, part);
-  else k_rows_dx<T, false><<<g, 256, 0, s>>>(a, strip, part);
+  if (vec) k_rows_dx<T, MR, true><<<g, 256, 0, s>>>(a, strip, part);
+  else k_rows_dx<T, MR, false><<<g, 256, 0, s>>>(a, strip, part);
   CUDA_LAUNCH_CHECK();
-  k_rows_join<T><<<blocks_for(a.M * a.K), 256, 0, s>>>(a, y, part);
+  k_rows_join<T><<<static_cast<unsigned>(std::min<int64_t>((a.M * a.K + 31) / 32, 16LL * sm_count())), 1024, 0, s>>>(a, y, part);
   CUDA_LAUNCH_CHECK();
 }
 
@@ -593,9 +610,15 @@ size_t few_rows_floats(const FewRows &a) {
 }
 
 void few_rows_bwd(const FewRows &a, cudaStream_t s) {
-  if (a.dt == DT_F32) bwd_of<float>(a, s);
-  else if (a.dt == DT_F16) bwd_of<__half>(a, s);
-  else bwd_of<__nv_bfloat16>(a, s);
+  auto go = [&](auto tag) {
+    using T = decltype(tag);
+    if (a.M == 1) bwd_of<T, 1>(a, s);
+    else if (a.M <= 4) bwd_of<T, 4>(a, s);
+    else bwd_of<T, kRowPad>(a, s);
+  };
+  if (a.dt == DT_F32) go(float{});
+  else if (a.dt == DT_F16) go(__half{});
+  else go(__nv_bfloat16{});
 }
 
 int column_strips(int64_t M) { return static_cast<int>(std::min<int64_t>(128, (M + 63) / 64)); }

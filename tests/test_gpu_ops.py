@@ -612,3 +612,30 @@ def test_expired_wait_is_reported(dtype, m):
     ops.check_status()
     assert torch.equal(ops.gated_linear(x, p["wg"], p["wv"], p["bg"]), want)
     ops.check_status()
+
+
+def test_offsets_past_32_bits():
+    """Rows that start beyond 2^31 elements: the last rows of a long call are
+    those of a short one."""
+    m, d, n = 1_100_000, 2048, 64
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB of free device memory")
+    bf = torch.bfloat16
+    x = torch.empty(m, d, dtype=bf, device="cuda").normal_()
+    w, v = rand(gen(91), n, d, dtype=bf, std=0.02), rand(gen(92), d, dtype=bf, std=0.1, mean=1)
+    tail = slice(m - 300, m)
+    y = ops.linear(x, w)
+    assert (y[tail].double() - x[tail].double() @ w.double().T).abs().max() <= 0.05
+    dx, dw, _ = ops.linear_backward(y, x, w)
+    assert torch.equal(dx[tail], ops.linear_backward(y[tail], x[tail], w, needs=(True, False, False))[0])
+    ref = sum(y[i:i + 100_000].float().T.double() @ x[i:i + 100_000].double() for i in range(0, m, 100_000))
+    # 22 split sums of 50,000 tokens each in 3,125 truncating additions, then
+    # one rounding: 2^-9 of an element, 2^-11 of the largest
+    assert ((dw.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -11 * ref.abs().max()).all()
+    del dx, dw, y
+    s, o = ops.residual_norm(x, x, v, norm="rms", post_norm="rms")
+    s2, o2 = ops.residual_norm(x[tail], x[tail], v, norm="rms", post_norm="rms")
+    assert torch.equal(s[tail], s2) and torch.equal(o[tail], o2)
+    g = ops.residual_norm_backward(None, o, x, x, v, norm="rms", post_norm="rms", needs=(True, False, True) + (False,) * 4)
+    g2 = ops.residual_norm_backward(None, o2, x[tail], x[tail], v, norm="rms", post_norm="rms")
+    assert torch.equal(g.residual[tail], g2.residual)
