@@ -639,3 +639,45 @@ def test_offsets_past_32_bits():
     g = ops.residual_norm_backward(None, o, x, x, v, norm="rms", post_norm="rms", needs=(True, False, True) + (False,) * 4)
     g2 = ops.residual_norm_backward(None, o2, x[tail], x[tail], v, norm="rms", post_norm="rms")
     assert torch.equal(g.residual[tail], g2.residual)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("shape", [(3000, 640, 529), (200, 2500, 72)], ids=str)
+def test_relu_near_zero(dtype, shape):
+    """The derivative's side where z is next to 0 is that of float64: every
+    other weight row is chosen so that z is 0 up to its last bits."""
+    m, k, f = shape
+    g = gen(101)
+    x, w = rand(g, m, k, dtype=dtype), rand(g, f, k, dtype=dtype, std=k ** -0.5)
+    x[:, 1] = x[:, 0]
+    w[::2, 1] = -w[::2, 0]          # two large terms that cancel
+    w[::2, 2:] *= 2.0 ** -7
+    dy = rand(g, m, f, dtype=dtype)
+    z = x.double() @ w.double().T
+    dz = dy.double() * (z > 0)
+    db = ops.linear_backward(dy, x, w, torch.zeros(f, dtype=dtype, device="cuda"), "relu")[2]
+    # no term may be missing or too many: each is a whole dy, the rounding of
+    # the sums far less than the smallest that counts
+    err = (db.double() - dz.sum(0)).abs()
+    assert (err <= unit(dtype) * dz.sum(0).abs() + 2.0 ** -18 * dz.abs().sum(0)).all()
+    v = rand(g, f, k, dtype=dtype, std=k ** -0.5)
+    dbg = ops.gated_linear_backward(dy, x, w, v, torch.zeros(f, dtype=dtype, device="cuda"), None, "relu")[3]
+    t = dz * (x.double() @ v.double().T)
+    assert ((dbg.double() - t.sum(0)).abs() <= unit(dtype) * t.sum(0).abs() + 2.0 ** -15 * t.abs().sum(0)).all()
+
+
+def test_relu_rows_of_zeros_and_of_other_scales():
+    """Blocks of zeros, and blocks next to 0 as a whole, cost and give what
+    others do."""
+    g = gen(102)
+    m, k, f = 2048, 256, 512
+    x, w = rand(g, m, k, dtype=torch.float32), rand(g, f, k, dtype=torch.float32, std=k ** -0.5)
+    x[100:900] = 0
+    x[901:1500] *= 2.0 ** -30
+    dy = rand(g, m, f, dtype=torch.float32)
+    dx, dw, db = ops.linear_backward(dy, x, w, torch.zeros(f, device="cuda"), "relu")
+    z = x.double() @ w.double().T
+    dz = dy.double() * (z > 0)
+    assert (dx.double()[100:900] == 0).all()
+    for a, b in ((db, dz.sum(0)), (dx, dz @ w.double()), (dw, dz.T @ x.double())):
+        assert ((a.double() - b).norm() / b.norm()) <= 2.0 ** -10  # (a flip among 2^18 would be 2^-9)
