@@ -212,10 +212,10 @@ mlipcpp_error_t mlipcpp_b200_domain_stats(mlipcpp_b200_domain_t domain, double s
  *
  * Products accumulate in fp32; activations, norms and sums run in fp32 and
  * each output is rounded once.  f32 products have fp32 accuracy (22-bit
- * split operands, one scale per 128 elements of a row of x or of a gradient,
- * and one per weight matrix).  A backward call recomputes what it needs from
- * the forward's inputs; gradients that enter a product are rounded to the
- * call's type first.  Results do not depend on timing: no sum's order varies.
+ * split operands; one operand has a scale per 128 elements of its sums, the
+ * other one per block of 128 x 128).  A backward call recomputes what it needs
+ * from the forward's inputs; gradients that enter a product are rounded to the
+ * call's type first.  The derivative of relu at 0 is 0.  Results do not depend on timing: no sum's order varies.
  * In f32 an infinite element makes its row or column of a product NaN.
  *
  * `workspace`: device memory of at least the bytes that the matching

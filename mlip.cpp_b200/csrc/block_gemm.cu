@@ -14,12 +14,12 @@
 //    the whole contraction; BN = 256 (one 128 x 256 tile, two accumulators)
 //    or 128 (four accumulators) when 256-wide tiles would leave SMs idle.
 //  * f32: A = 2^-s (hi + lo) with one scale per row and 128 contraction
-//    elements, B = 2^-t (hi + lo) with one scale per 128 x 128 block (or one
-//    for all) in the way of split16.cuh; A_lo B_hi + A_hi B_lo + A_hi B_hi per
-//    step.  The tensor core truncates
-//    when it adds to its accumulator, so every 128 contraction elements the
-//    accumulator warps add the partial sum to fp32 registers with
-//    round-to-nearest.
+//    elements, B = 2^-t (hi + lo) with one scale per 128 x 128 block (one for
+//    all of a model's weight, split when it was loaded) in the way of
+//    split16.cuh; A_lo B_hi + A_hi B_lo + A_hi B_hi per step.  The tensor core
+//    truncates when it adds to its accumulator, so every 128 contraction
+//    elements the accumulator warps add the partial sum to fp32 registers
+//    with round-to-nearest.
 //
 // Pairs (16-bit): where there are enough rows, two SMs take a tile of 256 x 256
 // together (cta_group::2).  Each loads its own 128 rows of A and half of B's
