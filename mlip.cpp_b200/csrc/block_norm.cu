@@ -22,6 +22,9 @@
 // has rows that are not 16-byte aligned, or too long for the ring, is read
 // directly.
 //
+// Outputs leave L2 before anything else (__stcs): the inputs of later rows are
+// still to be read there.  16,383 x 4096 f16 forward: 101 us a call, without 106.
+//
 // Measured: 16,383 x 4096 f16 forward in 93 us (5.8 TB/s), 8192 x 4096 bf16
 // backward in 98 us (4.1 TB/s: four reductions a row and only two CTAs an SM,
 // since a row's values and its column sums take 110 registers a thread).
@@ -124,7 +127,7 @@ struct Row {
     if constexpr (VEC) {
 #pragma unroll
       for (int i = 0; i < E / V; ++i)
-        if (FULL || col(i, t) < d) *reinterpret_cast<uint4 *>(q + col(i, t)) = close16<T>(&x[i * V / 2]);
+        if (FULL || col(i, t) < d) __stcs(reinterpret_cast<uint4 *>(q + col(i, t)), close16<T>(&x[i * V / 2]));
     } else {
 #pragma unroll
       for (int k = 0; k < P; ++k) {
