@@ -296,11 +296,11 @@ mlipcpp_error_t mlipcpp_b200_linear_backward(const mlipcpp_b200_linear_t *args, 
 /* stream = scale residual + gate * post(y), out = norm(stream), on rows of
  * `features` <= 16384 elements: post and norm are none, RMS or layer norms
  * (eps > 0) with an optional weight and bias [features]; y NULL leaves
- * scale * residual; gate NULL is 1, ldgate 0 is one row for all, else a gate
- * for every row.  Forward writes each of stream and out that is not NULL.
- * Backward reads residual, y and the gradients dstream and dout (NULL: zero)
- * and writes each gradient that is not NULL (dgate: [features] where ldgate
- * is 0, else rows of stride lddgate). */
+ * scale * residual; gate NULL is 1 (ldgate is not read then), ldgate 0 is one
+ * row for all, else a gate for every row.  Forward writes each of stream and
+ * out that is not NULL.  Backward reads residual, y and the gradients dstream
+ * and dout (NULL: zero) and writes each gradient that is not NULL (dgate:
+ * [features] where ldgate is 0, else rows of stride lddgate). */
 typedef struct {
   int32_t dtype, norm, post_norm;
   int64_t rows, features;

@@ -273,7 +273,9 @@ mlipcpp_error_t op_args(const mlipcpp_b200_residual_norm_t *a, bool back, pet::R
   if (c.code != MLIPCPP_OK) return c.code;
   c.es = pet::dtype_size(a->dtype);
   const int64_t M = a->rows, d = a->features;
-  const bool each = a->ldgate != 0;  // a gate for every row
+  // a gate for every row (without a gate its stride says nothing of the rows,
+  // but still the form of dgate: empty tensors may have no address)
+  const bool each = a->ldgate != 0;
   c.mat(a->residual, a->ldresidual, M, d, "residual", true);
   c.mat(a->y, a->ldy, M, d, "y", false);
   if (each) c.mat(a->gate, a->ldgate, M, d, "gate", false);
@@ -302,7 +304,7 @@ mlipcpp_error_t op_args(const mlipcpp_b200_residual_norm_t *a, bool back, pet::R
   o.eps = a->eps;
   o.residual = {a->residual, op_ld(a->ldresidual, M, d)};
   o.y = {a->y, op_ld(a->ldy, M, d)};
-  o.gate = {a->gate, each ? op_ld(a->ldgate, M, d) : 0};
+  o.gate = {a->gate, each && a->gate ? op_ld(a->ldgate, M, d) : 0};
   o.w = a->weight;
   o.b = a->bias;
   o.pw = a->post_weight;

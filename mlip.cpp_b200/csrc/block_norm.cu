@@ -725,7 +725,7 @@ NormArgs args_of(const ResidualNorm &a) {
   n.y = a.y.p;
   n.ldy = a.y.ld;
   n.gate = a.gate.p;
-  n.ldg = a.gate.ld;
+  n.ldg = a.gate.p ? a.gate.ld : 0;
   n.w = a.w;
   n.b = a.b;
   n.pw = a.pw;
@@ -752,7 +752,7 @@ void residual_norm_fwd(const ResidualNorm &a, Workspace &ws, cudaStream_t s) {
 }
 
 void residual_norm_bwd(const ResidualNorm &a, Workspace &ws, cudaStream_t s) {
-  void *const dgate = a.gate.ld == 0 ? a.dgate.p : nullptr;  // of one row
+  void *const dgate = a.dgate.ld == 0 ? a.dgate.p : nullptr;  // of one row
   if (a.M == 0) {
     for (void *g : {a.dw, a.db, a.dpw, a.dpb, dgate})
       if (g && !ws.sizing()) CUDA_CHECK(cudaMemsetAsync(g, 0, a.d * dtype_size(a.dtype), s));
@@ -768,7 +768,7 @@ void residual_norm_bwd(const ResidualNorm &a, Workspace &ws, cudaStream_t s) {
   n.lddr = a.dresidual.ld;
   n.dy = a.dy.p;
   n.lddy = a.dy.ld;
-  if (a.gate.ld != 0) {
+  if (n.ldg != 0) {
     n.dgate = a.dgate.p;
     n.lddg = a.dgate.ld;
   }
