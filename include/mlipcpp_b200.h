@@ -332,15 +332,19 @@ int64_t mlipcpp_b200_kernel_launches(void);
 int64_t mlipcpp_b200_device_allocations(void);
 
 /* Failure-detection test hooks (no counterpart in the reference).  Every
- * wait of the tensor-core GEMM pipelines is bounded; on expiry the CTA
- * stops, lets its own copies and MMAs complete, frees its tensor memory and
- * records a device error that the call returns as MLIPCPP_ERROR_COMPUTATION;
- * the model stays usable.  set_wait_bound_ns sets that bound on the current
- * device (0: the default of 1 s).  inject_gemm_stall makes the next GEMM
- * launch with a plain store epilogue withhold the operand loads of its
- * first CTA, so that CTA's waits run out. */
+ * wait of the tensor-core GEMM pipelines and of the norms' rings is bounded;
+ * on expiry the CTA stops (a norm: goes on without waiting), lets its own
+ * copies and MMAs complete, frees its tensor memory and records a device error
+ * that the call returns as MLIPCPP_ERROR_COMPUTATION (an operator: that
+ * mlipcpp_b200_ops_status returns); the model stays usable.  set_wait_bound_ns
+ * sets that bound on the current device (0: the default of 1 s).
+ * inject_gemm_stall makes the next GEMM launch with a plain store epilogue
+ * withhold the operand loads of its first CTA, inject_norm_stall the next norm
+ * whose rows are aligned to 16 bytes those of its first rows, so that their
+ * waits run out. */
 mlipcpp_error_t mlipcpp_b200_set_wait_bound_ns(uint64_t ns);
 mlipcpp_error_t mlipcpp_b200_inject_gemm_stall(void);
+mlipcpp_error_t mlipcpp_b200_inject_norm_stall(void);
 
 /* CUDA device ordinal used by models created afterwards (default: the
  * calling thread's current device). */

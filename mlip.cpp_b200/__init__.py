@@ -108,6 +108,7 @@ def lib() -> ctypes.CDLL:
         "mlipcpp_b200_device_allocations": (i64, []),
         "mlipcpp_b200_set_wait_bound_ns": (ctypes.c_int, [ctypes.c_uint64]),
         "mlipcpp_b200_inject_gemm_stall": (ctypes.c_int, []),
+        "mlipcpp_b200_inject_norm_stall": (ctypes.c_int, []),
         "mlipcpp_b200_set_device": (ctypes.c_int, [i32]),
         "mlipcpp_b200_domain_create": (vp, [vp, vp, vp, i32, f32, vp]),
         "mlipcpp_b200_domain_free": (None, [vp]),

@@ -1201,6 +1201,12 @@ mlipcpp_error_t mlipcpp_b200_inject_gemm_stall(void) {
   return MLIPCPP_OK;
 }
 
+mlipcpp_error_t mlipcpp_b200_inject_norm_stall(void) {
+  pet::inject_norm_stall();
+  clear_error();
+  return MLIPCPP_OK;
+}
+
 mlipcpp_error_t mlipcpp_b200_set_device(int32_t device) {
   int n = 0;
   if (cudaGetDeviceCount(&n) != cudaSuccess || device < 0 || device >= n) {

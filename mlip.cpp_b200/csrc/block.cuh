@@ -31,7 +31,9 @@ inline int take_error(const int &word, cudaStream_t s) {
   }
   return v;
 }
-int norm_error(cudaStream_t s);  // of the norms' rings (block_norm.cu)
+// of the norms' rings (block_norm.cu)
+int norm_error(cudaStream_t s);
+void norm_wait_bound(uint64_t ns);
 
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }

@@ -111,7 +111,11 @@ constexpr int kMaxNormDim = 16384;
 // Error word of the operators' pipelines on the current device: nonzero once a
 // bounded wait ran out.  Synchronises `s`, reads and clears it.
 int block_status(cudaStream_t s);
-// Bound on the waits of the tensor-core pipelines (0: the default).
+// Bound on the waits of the operators' pipelines (0: the default).
 void set_block_wait_bound_ns(uint64_t ns);
+// Test hook: the next norm launch with a ring withholds the copies of its first
+// rows, so that their waits run out.
+void inject_norm_stall();
+bool norm_stall_armed();
 
 }  // namespace pet

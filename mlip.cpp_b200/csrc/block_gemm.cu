@@ -1382,6 +1382,7 @@ int block_status(cudaStream_t s) {
 void set_block_wait_bound_ns(uint64_t ns) {
   const uint64_t v = ns ? ns : tc::kWaitNs;
   CUDA_CHECK(cudaMemcpyToSymbol(tc::g_wait_ns, &v, sizeof(v)));
+  norm_wait_bound(v);
 }
 
 namespace {

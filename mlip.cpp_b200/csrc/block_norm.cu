@@ -29,6 +29,7 @@
 // backward in 98 us (4.1 TB/s: four reductions a row and only two CTAs an SM,
 // since a row's values and its column sums take 110 registers a thread).
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "block.cuh"
@@ -241,10 +242,16 @@ constexpr int kInputs = 5;  // rows of a stage: r, y, dstream, dout, gate
 struct Ring {
   int stages, inputs;  // stages 0: rows are read directly
   int row_bytes, vector_bytes;
+  bool stall;  // test hook: the first group of the first CTA issues no copies
   int bytes(int groups) const { return vector_bytes + row_bytes * groups * stages * inputs; }
 };
 
-// One group's ring: `take` waits for the next row's inputs.
+// One group's ring: `take` waits for the next row's inputs.  A thread whose
+// wait runs out records the error and waits no more: the results are void.  The
+// one that issues the copies then waits, with the default bound, for those on
+// their way, and issues no further ones: no CTA ends while something is written
+// to its shared memory, and no barrier is armed again in an unfinished phase
+// (the others run into their own bounds, once each).
 template <int TPR>
 struct Feed {
   const NormArgs &a;
@@ -270,21 +277,29 @@ struct Feed {
       dst += ring.row_bytes;
     }
   }
+  __device__ __forceinline__ bool stalled() const { return ring.stall && blockIdx.x == 0 && threadIdx.x < TPR; }
   __device__ __forceinline__ void start() {
-    if (t == 0)
+    if (t == 0 && !stalled())
       for (int s = 0; s < ring.stages && row + s * step < a.M; ++s) issue(s, row + s * step);
   }
-  __device__ __forceinline__ const char *take() {
+  // inputs of row `at`
+  __device__ __forceinline__ const char *take(int64_t at) {
     const uint32_t bar = tc::smem_u32(bars + stage);
-    if (ok && !tc::mbar_try_wait(bar, phase) && !tc::wait_bounded(bar, phase)) {
-      ok = false;  // waits no more: the results are void, the copies land by themselves
+    if (ok && !tc::mbar_try_wait(bar, phase) && !tc::wait_within(bar, phase)) {
+      ok = false;
       atomicExch(&g_norm_err, 1);
+      // rows issued and not waited for: this one and the ring's next
+      if (t == 0 && !stalled())
+        for (int i = 0; i < ring.stages && at + i * step < a.M; ++i) {
+          const int s = stage + i < ring.stages ? stage + i : stage + i - ring.stages;
+          tc::wait_bounded(tc::smem_u32(bars + s), phase ^ (s < stage ? 1 : 0));
+        }
     }
     return base + static_cast<size_t>(stage) * ring.inputs * ring.row_bytes;
   }
   // every thread of the group has read the stage (after a group barrier)
   __device__ __forceinline__ void give(int64_t at) {
-    if (t == 0 && at + ring.stages * step < a.M) issue(stage, at + ring.stages * step);
+    if (t == 0 && ok && at + ring.stages * step < a.M) issue(stage, at + ring.stages * step);
     if (++stage == ring.stages) {
       stage = 0;
       phase ^= 1;
@@ -383,7 +398,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_norm_fwd(const NormArgs a, co
   for (; row < a.M; row += step) {
     float2 x[P];
     const char *in = nullptr;
-    if (RING) in = feed.take();
+    if (RING) in = feed.take(row);
     if (RING) R::load(in, 0, t, d, x);
     else R::load(a.r, row * a.ldr, t, d, x);
 #pragma unroll
@@ -439,7 +454,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 2 : 1) k_norm_bwd(const NormAr
     float2 n[P], u[P], g[P], f[P];
     const char *in[kInputs] = {};
     if (RING) {
-      const char *p = feed.take();
+      const char *p = feed.take(row);
       const void *there[kInputs] = {a.r, a.y, a.ds, a.dout, each ? a.gate : nullptr};
 #pragma unroll
       for (int k = 0; k < kInputs; ++k) {
@@ -634,7 +649,7 @@ struct Layout {
 };
 Layout layout_of(const NormArgs &a, int dt, bool vec, bool bwd) {
   const int es = static_cast<int>(dtype_size(dt)), e = dt == DT_F32 ? 8 : 16;
-  Layout l{32, dt == DT_F32 ? 512 : 256, 0, {0, 0, a.d * es, Vectors<Row<float, 32, 8, true>, float, true>::count(a)}};
+  Layout l{32, dt == DT_F32 ? 512 : 256, 0, {0, 0, a.d * es, Vectors<Row<float, 32, 8, true>, float, true>::count(a), false}};
   while (l.tpr * e < a.d && l.tpr < 1024) l.tpr *= 2;
   l.ring.vector_bytes *= 4 * l.tpr * (l.tpr == 1024 ? 16 : e);
   l.nt = std::max(l.nt, l.tpr);
@@ -662,12 +677,16 @@ Layout layout_of(const NormArgs &a, int dt, bool vec, bool bwd) {
   return l;
 }
 
+std::atomic<bool> g_norm_stall{false};
+
 template <typename T, int TPR, int NT, int E, int MODE, bool BWD>
 void launch(const NormArgs &a, const Layout &l, cudaStream_t s) {
   const int smem = MODE >= 2 ? l.ring.bytes(NT / TPR) : 0;
+  Ring ring = l.ring;
+  ring.stall = MODE >= 2 && norm_stall_armed() && g_norm_stall.exchange(false);
   auto go = [&](auto *kernel) {
     if (smem) CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    kernel<<<l.grid, NT, smem, s>>>(a, l.ring);
+    kernel<<<l.grid, NT, smem, s>>>(a, ring);
     CUDA_LAUNCH_CHECK();
   };
   if constexpr (!BWD) go(k_norm_fwd<T, TPR, NT, E, MODE>);
@@ -739,6 +758,10 @@ NormArgs args_of(const ResidualNorm &a) {
 using namespace blk;
 
 int blk::norm_error(cudaStream_t s) { return take_error(g_norm_err, s); }
+void blk::norm_wait_bound(uint64_t ns) { CUDA_CHECK(cudaMemcpyToSymbol(tc::g_wait_ns, &ns, sizeof(ns))); }
+
+void inject_norm_stall() { g_norm_stall.store(true); }
+bool norm_stall_armed() { return g_norm_stall.load(std::memory_order_relaxed); }
 
 void residual_norm_fwd(const ResidualNorm &a, Workspace &ws, cudaStream_t s) {
   if (a.M == 0 || ws.sizing()) return;

@@ -1077,7 +1077,7 @@ void PETModel::record_phase(int i) {
 // always run eagerly.  If the capture fails, graphs are switched off for
 // this model and the step runs eagerly.
 void PETModel::run_forward_backward(bool grad) {
-  if (!use_graph_ || kprof_ || rm_ || gemm_stall_armed()) {
+  if (!use_graph_ || kprof_ || rm_ || gemm_stall_armed() || norm_stall_armed()) {
     forward_backward(grad);
     return;
   }

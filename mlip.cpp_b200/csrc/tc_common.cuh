@@ -121,6 +121,14 @@ __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity) {
   return true;
 }
 
+// Wait of at most g_wait_ns without an abort flag.
+__device__ __forceinline__ bool wait_within(uint32_t bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer(), bound = g_wait_ns;
+  while (!mbar_try_wait(bar, parity))
+    if (globaltimer() - t0 > bound) return false;
+  return true;
+}
+
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }

@@ -50,3 +50,37 @@ def test_no_gate_whatever_its_stride(dtype, shape):
                           *(0,) * 6, guard.data_ptr(), d, d, d)
     ops._call("residual_norm", args, 0, True)
     assert (guard == 7).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("shape", [(1, 256), (40, 64), (4100, 2048), (3000, 520)], ids=str)
+def test_expired_norm_wait_is_reported(dtype, shape):
+    """Rows whose copies never come: their waits run out, the status says so
+    once, and the next call is whole."""
+    m, d = shape
+    g = gen(m)
+    r, y, gate = (rand(g, m, d, dtype=dtype) for _ in range(3))
+    w = rand(g, d, dtype=dtype, mean=1)
+
+    def run():
+        s, o = ops.residual_norm(r, y, w, post_weight=w, gate=gate, post_norm="layer")
+        return [s, o, *[t for t in ops.residual_norm_backward(r, y, r, y, w, post_weight=w, gate=gate, post_norm="layer")
+                        if t is not None]]
+
+    want = run()
+    ops.check_status()
+    L = mb.lib()
+    for call in (lambda: ops.residual_norm(r, y, w), lambda: ops.residual_norm_backward(r, y, r, y, w)):
+        assert L.mlipcpp_b200_set_wait_bound_ns(1_000_000) == mb.OK
+        try:
+            assert L.mlipcpp_b200_inject_norm_stall() == mb.OK
+            call()
+            with pytest.raises(mb.MLIPError) as e:
+                ops.check_status()
+            assert e.value.code == mb.COMPUTATION
+        finally:
+            assert L.mlipcpp_b200_set_wait_bound_ns(0) == mb.OK
+        ops.check_status()
+        for a, b in zip(run(), want):
+            assert torch.equal(a, b)
+    ops.check_status()
