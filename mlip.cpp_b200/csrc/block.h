@@ -103,6 +103,7 @@ struct ResidualNorm {
   Mat dstream, dout;
   MutMat dresidual, dy, dgate;
   void *dw = nullptr, *db = nullptr, *dpw = nullptr, *dpb = nullptr;
+  int *err = nullptr;  // device error word (null: the one of block_status)
 };
 void residual_norm_fwd(const ResidualNorm &a, Workspace &ws, cudaStream_t s);
 void residual_norm_bwd(const ResidualNorm &a, Workspace &ws, cudaStream_t s);

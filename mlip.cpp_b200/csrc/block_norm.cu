@@ -55,6 +55,7 @@ struct NormArgs {
   int64_t lddr, lddy, lddg;
   float *part;                 // [sum][CTA][d] of the vectors' gradients, or null
   bool hb;                     // a bias or its gradient is there
+  int *err;                    // error word, or null for the file's own
 };
 
 // 16 bytes of T <-> pairs of floats
@@ -287,7 +288,7 @@ struct Feed {
     const uint32_t bar = tc::smem_u32(bars + stage);
     if (ok && !tc::mbar_try_wait(bar, phase) && !tc::wait_within(bar, phase)) {
       ok = false;
-      atomicExch(&g_norm_err, 1);
+      atomicExch(a.err ? a.err : &g_norm_err, 1);
       // rows issued and not waited for: this one and the ring's next
       if (t == 0 && !stalled())
         for (int i = 0; i < ring.stages && at + i * step < a.M; ++i) {
@@ -749,6 +750,7 @@ NormArgs args_of(const ResidualNorm &a) {
   n.b = a.b;
   n.pw = a.pw;
   n.pb = a.pb;
+  n.err = a.err;
   return n;
 }
 

@@ -739,6 +739,7 @@ void PETModel::forward_backward(bool grad) {
     n.d = d;
     n.w = g;
     n.b = b;
+    n.err = d_err_.as<int>();
     return n;
   };
   auto block_ws = [&]() {

@@ -84,3 +84,25 @@ def test_expired_norm_wait_is_reported(dtype, shape):
         for a, b in zip(run(), want):
             assert torch.equal(a, b)
     ops.check_status()
+
+
+def test_expired_norm_wait_fails_the_prediction(model_file):
+    """A norm of a pre-norm model that gives up a wait fails that prediction,
+    and no operator call of someone else; the model stays usable."""
+    from mlipcpp_b200 import workloads as wl
+    p, s = mb.Predictor(model_file("pet-mad-s-gated")), wl.si_diamond(2, seed=3)
+    args = (s.positions, s.numbers, s.cell)
+    want = p.predict(*args)
+    ops.check_status()
+    L = mb.lib()
+    assert L.mlipcpp_b200_set_wait_bound_ns(1_000_000) == mb.OK
+    try:
+        assert L.mlipcpp_b200_inject_norm_stall() == mb.OK
+        with pytest.raises(mb.MLIPError) as e:
+            p.predict(*args)
+        assert e.value.code == mb.COMPUTATION
+    finally:
+        assert L.mlipcpp_b200_set_wait_bound_ns(0) == mb.OK
+    ops.check_status()
+    got = p.predict(*args)
+    assert got.energy == want.energy and (got.forces == want.forces).all()
