@@ -68,9 +68,10 @@ __device__ __forceinline__ uint4 pack(const float (&v)[16 / sizeof(T)]) {
 }
 
 // 1 / (1 + e^-z) by the intrinsics: a few ulp of fp32, and 2^-23 |z| of
-// e^-z, which no result sees where |z| is large.  The exponent's argument stops
-// at -80, where the result is below 2e-35, so that e^-z stays finite.
-__device__ __forceinline__ float logistic(float z) { return __fdividef(1.f, 1.f + __expf(-fmaxf(z, -80.f))); }
+// e^-z, which no result sees where |z| is large.  Below z = -87 e^-z passes 2^126
+// or is infinite and the quotient 0, so nothing is clamped (a clamp by fmaxf
+// would turn NaN into a number).
+__device__ __forceinline__ float logistic(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
 
 // a = act(z), da = act'(z)
 template <int ACT>

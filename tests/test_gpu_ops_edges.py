@@ -106,3 +106,65 @@ def test_expired_norm_wait_fails_the_prediction(model_file):
     ops.check_status()
     got = p.predict(*args)
     assert got.energy == want.energy and (got.forces == want.forces).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("shape", PATHS, ids=str)
+def test_nan_reaches_the_results(dtype, act, shape):
+    """A NaN in x, a weight or a bias makes exactly the results and gradients
+    NaN that it makes NaN in float64."""
+    m, k, n = shape
+    g = gen(m + k)
+    clean = [rand(g, m, k, dtype=dtype), rand(g, n, k, dtype=dtype, std=k ** -0.5),
+             rand(g, n, k, dtype=dtype, std=k ** -0.5), rand(g, n, dtype=dtype), rand(g, n, dtype=dtype)]
+    dy = rand(g, m, n, dtype=dtype)
+    for i, at in ((0, (2, 5)), (1, (7, 9)), (3, (11,))):
+        t = [c.clone() for c in clean]
+        t[i][at] = float("nan")
+        x, w, v, b, c = t
+        X, W, V, B, C, D = (s.double() for s in (*t, dy))
+        a, da = act64(act, X @ W.T + B)
+        z = X @ V.T + C
+        # (an activation has no derivative at NaN: relu's is 0, the others' NaN)
+        dz, dg, dv = D * da, D * z * da, D * a
+        for got, ref, what in (
+                (ops.linear(x, w, b, act), a, "y"),
+                (ops.gated_linear(x, w, v, b, c, act), a * z, "h"),
+                *zip(ops.linear_backward(dy, x, w, b, act), (dz @ W, dz.T @ X, dz.sum(0)), ("dx", "dw", "db")),
+                *zip(ops.gated_linear_backward(dy, x, w, v, b, c, act),
+                     (dg @ W + dv @ V, dg.T @ X, dv.T @ X, dg.sum(0), dv.sum(0)),
+                     ("dx", "dw_gate", "dw_value", "db_gate", "db_value"))):
+            assert torch.equal(got.isnan(), ref.isnan()), (i, what, int(got.isnan().sum()), int(ref.isnan().sum()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("shape", PATHS, ids=str)
+def test_activations_far_out(dtype, act, shape):
+    """Where an activation has reached its limits (|z| >= 100): 0, 1 or z, and
+    a derivative of 0 or 1, up to one rounding and, in f32, what the 22 bits of a
+    product's operands leave.  z is one element of x times 1, the value half 1."""
+    m, k, n = shape
+    far = [100.0, 2e3, 5e4] if dtype == torch.float16 else [100.0, 2e3, 1e6, 1e10, 1e12, 1e13, 1e18]
+    far = torch.tensor(far, device="cuda").to(dtype)
+    z = torch.cat([far, -far])
+    w, v = torch.zeros(n, k, dtype=dtype, device="cuda"), torch.zeros(n, k, dtype=dtype, device="cuda")
+    w[0, 0] = 1
+    c = torch.ones(n, dtype=dtype, device="cuda")
+    u = 1.01 * unit(dtype) + (2.0 ** -22 if dtype == torch.float32 else 0)
+    for i in range(0, len(z), m):
+        zi = z[i:i + m]
+        x = torch.zeros(m, k, dtype=dtype, device="cuda")
+        x[:len(zi), 0] = zi
+        a, da = act64(act, zi.double())
+        one = torch.zeros(m, n, dtype=dtype, device="cuda")
+        one[:, 0] = 1
+        rows = slice(0, len(zi))
+        for got, ref, what in (
+                (ops.linear(x, w, None, act)[rows, 0], a, "y"),
+                (ops.linear_backward(one, x, w, None, act)[0][rows, 0], da, "dx"),
+                (ops.gated_linear(x, w, v, None, c, act)[rows, 0], a, "h"),
+                (ops.gated_linear_backward(one, x, w, v, None, c, act)[0][rows, 0], da, "gated dx")):
+            # p = 1 / (1 + e^-z) is 0 or 1 to 2^-126 here
+            assert ((got.double() - ref).abs() <= u * ref.abs() + 1e-30).all(), (what, zi, got, ref)
