@@ -88,9 +88,10 @@ __device__ __forceinline__ void act_pair(float z, float &a, float &da) {
     a = z * c;
     da = c + z * __expf(-0.5f * z * z) * 0.3989422804014327f;
   } else if (ACT == ACT_GELU_TANH) {
-    const float p = logistic(1.5957691216057308f * (z + 0.044715f * z * z * z));
+    const float p = logistic(1.5957691216057308f * (z + 0.044715f * z * z * z)), q = z * p * (1.f - p);
     a = z * p;
-    da = p + z * p * (1.f - p) * 1.5957691216057308f * (1.f + 0.134145f * z * z);
+    // (q is 0 from about |z| = 10 on; z^2 passes fp32's range later)
+    da = q == 0.f ? p : p + q * 1.5957691216057308f * (1.f + 0.134145f * z * z);
   } else if (ACT == ACT_RELU) {
     a = z > 0.f ? z : (z == z ? 0.f : z);
     da = z > 0.f ? 1.f : 0.f;

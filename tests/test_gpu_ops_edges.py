@@ -146,7 +146,7 @@ def test_activations_far_out(dtype, act, shape):
     a derivative of 0 or 1, up to one rounding and, in f32, what the 22 bits of a
     product's operands leave.  z is one element of x times 1, the value half 1."""
     m, k, n = shape
-    far = [100.0, 2e3, 5e4] if dtype == torch.float16 else [100.0, 2e3, 1e6, 1e10, 1e12, 1e13, 1e18]
+    far = [100.0, 2e3, 5e4] if dtype == torch.float16 else [100.0, 2e3, 1e6, 1e10, 1e12, 1e13, 1e18, 1e20, 1e30, 1e36, 3e38]
     far = torch.tensor(far, device="cuda").to(dtype)
     z = torch.cat([far, -far])
     w, v = torch.zeros(n, k, dtype=dtype, device="cuda"), torch.zeros(n, k, dtype=dtype, device="cuda")
