@@ -128,6 +128,74 @@ __device__ __forceinline__ void store_dt(void *p, int dt, int64_t j, float v) {
   else static_cast<__nv_bfloat16 *>(p)[j] = __float2bfloat16_rn(v);
 }
 
+// ReLU's derivative jumps at 0, where fp32 sums of different orders disagree
+// about the sign of z, or cancel to 0 with a remainder below their last bit.
+// Elements within kNear of the largest beside them (5 or more of those sums'
+// largest errors) get z from a dot product in 64 bits, all lanes of the warp on
+// one element at a time: about one in 100,000.  What bounds that work: more than
+// kNearMost of a 32 x 32 block (kNearRow of a warp's 32 elements) that are near 0
+// are rows or features of a smaller scale than the others', whose own sums are as
+// exact; a block's row of zeros is a row of zeros in x (padding), a column of them
+// costs one product if its weights are zeros, and more than kZeroMost others are
+// such rows and columns in number.  All of these are left as they are.  Measured
+// for dz, dWg, dWv, dx of 8192 x 1024 x 4096 in bf16: 340 us, with the smooth silu
+// 324; one column of zero weights in each 32: 510.
+constexpr float kNear = 1.f / 262144.f;
+constexpr unsigned kNearMost = 32, kZeroMost = 64;
+constexpr int kNearRow = 2;
+// z = x w^T + b of the elements in doubt
+struct NearZero {
+  const void *x, *w, *b;
+  int64_t ldx, ldw, k;
+};
+// dead: the columns c0 + bit that have turned out to have no weights.
+template <typename T>
+__device__ __forceinline__ float settled(const NearZero &e, bool flag, int64_t row, int64_t col, float z, int lane,
+                                         unsigned &dead, int64_t c0) {
+  unsigned todo = __ballot_sync(0xffffffffu, flag && !(dead >> (col - c0) & 1));
+  while (todo) {
+    const int src = __ffs(todo) - 1;
+    todo &= todo - 1;
+    const int64_t r = __shfl_sync(0xffffffffu, row, src), c = __shfl_sync(0xffffffffu, col, src);
+    const T *x = static_cast<const T *>(e.x) + r * e.ldx, *w = static_cast<const T *>(e.w) + c * e.ldw;
+    double t = 0.0;
+    bool live = false;
+    int64_t k = lane;
+    for (; k + 7 * 32 < e.k; k += 8 * 32) {  // 16 loads in flight: latency is all it costs
+      T a[8], b[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] = x[k + i * 32], b[i] = w[k + i * 32];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        t = fma(static_cast<double>(to_f(a[i])), static_cast<double>(to_f(b[i])), t);
+        live |= to_f(b[i]) != 0.f;
+      }
+    }
+    for (; k < e.k; k += 32) {
+      t = fma(static_cast<double>(to_f(x[k])), static_cast<double>(to_f(w[k])), t);
+      live |= to_f(w[k]) != 0.f;
+    }
+    if (!__any_sync(0xffffffffu, live)) {
+      dead |= 1u << (c - c0);
+      todo &= ~__ballot_sync(0xffffffffu, col == c);
+    }
+    t = warp_sum_d(t);
+    if (e.b) t += static_cast<double>(to_f(static_cast<const T *>(e.b)[c]));
+    if (lane == src) z = t > 0.0 ? fmaxf(static_cast<float>(t), 1e-37f) : fminf(static_cast<float>(t), 0.f);
+  }
+  return z;
+}
+// The same for one element a lane (there: it has one), of columns from lane 0's on.
+template <typename T>
+__device__ __forceinline__ float settled_row(const NearZero &e, bool there, float near, int64_t row, int64_t col,
+                                             float z, int lane, int most = kNearRow) {
+  const bool flag = there && fabsf(z) <= near, nonzero = flag && z != 0.f;
+  const bool all = __popc(__ballot_sync(0xffffffffu, flag)) <= most;
+  if (!all && __popc(__ballot_sync(0xffffffffu, nonzero)) > most) return z;
+  unsigned dead = 0;
+  return settled<T>(e, all ? flag : nonzero, row, col, z, lane, dead, __shfl_sync(0xffffffffu, col, 0));
+}
+
 // ---- few rows (block_rows.cu) ---------------------------------------------
 // At most kFewRows rows (forward of 16-bit aligned ones: 16): each weight read
 // once with plain loads, every sum and gradient in fp32.

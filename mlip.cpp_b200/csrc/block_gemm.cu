@@ -70,7 +70,9 @@ constexpr int kAccWarps = 8;  // two per quarter of the tensor-memory lanes
 constexpr int kThreads = 64 + 32 * kAccWarps;
 constexpr int kStageFloats = 32 * 32;  // turning block of one accumulator warp
 
-enum Epi : int { E_LINEAR = 0, E_LINEAR_BWD = 1, E_GATED = 2, E_GATED_BWD = 3, E_PARTIAL = 4 };
+// (E_RELU beside E_*_BWD: a variant that settles the sign of z near 0, whose
+// registers cost the other activations' launches 2 to 9%)
+enum Epi : int { E_LINEAR = 0, E_LINEAR_BWD = 1, E_GATED = 2, E_GATED_BWD = 3, E_PARTIAL = 4, E_RELU = 8 };
 
 // MODE: 16-bit operands (one product, planes = 1) or split-fp16 (planes = 2).
 template <bool F32, int BN, bool PAIR>
@@ -100,10 +102,7 @@ struct EpiArgs {
   float scale;
   float *sums0, *sums1;   // E_*_BWD, or null: column sums of each 32 rows of the
                           // results before they are rounded, [row / 32][N]
-  // E_*_BWD of a ReLU: what z (the gate) comes from, to settle its sign where
-  // it is near 0 (nx null: not asked for)
-  const void *nx, *nw;
-  int64_t nldx, nldw, nk;
+  NearZero near;          // E_*_BWD of a ReLU: what z (the gate) comes from (x null: not asked for)
   bool vin, vout;         // rows movable in 16-byte pieces
   float *part;            // E_PARTIAL: [batch][split][M][nacc]
   int64_t nacc;
@@ -279,41 +278,6 @@ __device__ __forceinline__ void block_store(const Turned<T> &b, T *out, int64_t 
   }
 }
 
-// ReLU's derivative jumps at 0, where fp32 sums of different orders disagree
-// about the sign of z.  Elements within kNear of the largest of their block (5 or
-// more of those sums' largest errors) get z from a dot product in 64 bits, all
-// lanes of the warp on one element at a time: about one in 100,000.
-// More than kNearMost of a block's 1024 are rows or features of a smaller scale
-// than the others', whose own sums are as exact; they are left, which bounds the
-// work.  Measured for dz, dWg, dWv, dx of 8192 x 1024 x 4096 in bf16: 336 us, with
-// the smooth silu 328.
-constexpr float kNear = 1.f / 262144.f;
-constexpr unsigned kNearMost = 32;
-template <typename T>
-__device__ __forceinline__ float settled(const EpiArgs &e, bool flag, int64_t row, int64_t col, float z, int lane) {
-  unsigned todo = __ballot_sync(0xffffffffu, flag);
-  while (todo) {
-    const int src = __ffs(todo) - 1;
-    todo &= todo - 1;
-    const int64_t r = __shfl_sync(0xffffffffu, row, src), c = __shfl_sync(0xffffffffu, col, src);
-    const T *x = static_cast<const T *>(e.nx) + r * e.nldx, *w = static_cast<const T *>(e.nw) + c * e.nldw;
-    double t = 0.0;
-    int64_t k = lane;
-    for (; k + 7 * 32 < e.nk; k += 8 * 32) {  // 16 loads in flight: latency is all it costs
-      T a[8], b[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) a[i] = x[k + i * 32], b[i] = w[k + i * 32];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) t = fma(static_cast<double>(to_f(a[i])), static_cast<double>(to_f(b[i])), t);
-    }
-    for (; k < e.nk; k += 32) t = fma(static_cast<double>(to_f(x[k])), static_cast<double>(to_f(w[k])), t);
-    t = warp_sum_d(t);
-    if (e.b0) t += static_cast<double>(to_f(static_cast<const T *>(e.b0)[c]));
-    if (lane == src) z = t > 0.0 ? fmaxf(static_cast<float>(t), 1e-37f) : fminf(static_cast<float>(t), 0.f);
-  }
-  return z;
-}
-
 // Sums of the block's columns (bias gradients), in a fixed order: rows past M
 // are zeros.
 template <typename T>
@@ -337,7 +301,7 @@ __device__ __forceinline__ void block_sums(const Turned<T> &b, float *sums, int 
 
 // The epilogue of one block: v (and w, the value half of the gated forms) as
 // they come from the accumulator, `in` from the rows' input.
-template <int EPI, typename T>
+template <int EPI, bool RELU, typename T>
 __device__ __forceinline__ void epilogue(const Params &p, int batch, float *st, int lane, int row0, int col0,
                                          const float (&v)[32], const float (&w)[32], const Input<T> &in) {
   using U = Turned<T>;
@@ -355,7 +319,7 @@ __device__ __forceinline__ void epilogue(const Params &p, int batch, float *st, 
 #pragma unroll
       for (int j = 0; j < U::V; ++j) a.x[i][j] += f[j];
   }
-  if ((EPI == E_LINEAR_BWD || EPI == E_GATED_BWD) && e.nx) {
+  if (RELU) {
     float top = 0.f;
 #pragma unroll
     for (int i = 0; i < U::L; ++i)
@@ -363,19 +327,43 @@ __device__ __forceinline__ void epilogue(const Params &p, int batch, float *st, 
       for (int j = 0; j < U::V; ++j)
         if (row0 + U::row(i, lane) < p.M && c + j < p.N) top = fmaxf(top, fabsf(a.x[i][j]));
     const float near = warp_max(top) * kNear;
-    unsigned flags = 0;
+    unsigned flags = 0, zeros = 0;
 #pragma unroll
     for (int i = 0; i < U::L; ++i)
 #pragma unroll
       for (int j = 0; j < U::V; ++j)
-        if (a.x[i][j] != 0.f && fabsf(a.x[i][j]) <= near && row0 + U::row(i, lane) < p.M && c + j < p.N) flags |= 1u << (i * U::V + j);
-    const unsigned count = __reduce_add_sync(0xffffffffu, __popc(flags));
-    if (count && count <= kNearMost) {
+        if (fabsf(a.x[i][j]) <= near && row0 + U::row(i, lane) < p.M && c + j < p.N)
+          (a.x[i][j] == 0.f ? zeros : flags) |= 1u << (i * U::V + j);
+    // (one vote of the warp where nothing is in doubt)
+    const unsigned count = __reduce_add_sync(0xffffffffu, __popc(flags) | __popc(zeros) << 16);
+    if (count) {
+      if ((count & 0xffffu) > kNearMost) flags = 0;
+      if ((count >> 16) && p.N - col0 >= 8) {  // (fewer columns say nothing about a row)
+        const unsigned mine = ((1u << U::L) - 1) << (lane / U::L * U::L);  // lanes of this row
 #pragma unroll
-      for (int i = 0; i < U::L; ++i)
+        for (int i = 0; i < U::L; ++i) {
+          bool all = true;
 #pragma unroll
-        for (int j = 0; j < U::V; ++j)
-          a.x[i][j] = settled<T>(e, flags >> (i * U::V + j) & 1, row0 + U::row(i, lane), c + j, a.x[i][j], lane);
+          for (int j = 0; j < U::V; ++j) all &= (zeros >> (i * U::V + j) & 1) || c + j >= p.N;
+          if ((__ballot_sync(0xffffffffu, all) & mine) == mine) zeros &= ~(((1u << U::V) - 1) << (i * U::V));
+        }
+      }
+      if (__reduce_add_sync(0xffffffffu, __popc(zeros)) <= kZeroMost) flags |= zeros;
+      // through `st`, so that the product's code is there once
+      unsigned any = __reduce_or_sync(0xffffffffu, flags), dead = 0;
+      if (any) {
+        __syncwarp();
+#pragma unroll 1
+        for (; any; any &= any - 1) {
+          const int k = __ffs(any) - 1, i = k / U::V, j = k % U::V;
+          st[k * 32 + lane] = settled<T>(e.near, flags >> k & 1, row0 + U::row(i, lane), c + j, 0.f, lane, dead, col0);
+        }
+#pragma unroll
+        for (int i = 0; i < U::L; ++i)
+#pragma unroll
+          for (int j = 0; j < U::V; ++j)
+            if (flags >> (i * U::V + j) & 1) a.x[i][j] = st[(i * U::V + j) * 32 + lane];
+      }
     }
   }
   if (kDual && e.b1) {
@@ -417,9 +405,10 @@ __device__ __forceinline__ void epilogue(const Params &p, int batch, float *st, 
   if (EPI == E_GATED_BWD) block_store<T>(b, static_cast<T *>(e.out1), e.ldo, e.vout, st, lane, row0, col0, p.M, p.N);
 }
 
-template <bool F32, int BN, bool PAIR, int EPI, typename T>
+template <bool F32, int BN, bool PAIR, int FORM, typename T>
 __global__ void __launch_bounds__(kThreads, 1) k_block_gemm(const __grid_constant__ Maps maps, const Params p) {
   using C = Cfg<F32, BN, PAIR>;
+  constexpr int EPI = FORM & ~E_RELU;
   constexpr bool kDual = EPI == E_GATED || EPI == E_GATED_BWD;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
@@ -737,7 +726,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block_gemm(const __grid_constan
           const Input<T> cur = next;
           if (kIn && p.e.in && i + 32 < kCols) next.fetch(p, lane, row0, col_of(i + 32));
           if (col >= p.N || row0 >= p.M) return;
-          epilogue<EPI, T>(p, t.batch, st, lane, row0, col, v, w, cur);
+          epilogue<EPI, (FORM & E_RELU) != 0, T>(p, t.batch, st, lane, row0, col, v, w, cur);
         }
       };
       if (F32) {  // register arrays: constant indices
@@ -811,10 +800,9 @@ __global__ void __launch_bounds__(256) k_join(const Params p) {
         if (p.dual && e.b1) w += to_f(static_cast<const T *>(e.b1)[col]);
         if (e.in) in = to_f(static_cast<const T *>(e.in)[row * e.ldin + col]);
       }
-      if ((EPI == E_LINEAR_BWD || EPI == E_GATED_BWD) && e.nx) {
+      if ((EPI == E_LINEAR_BWD || EPI == E_GATED_BWD) && e.near.x) {
         const float near = warp_max(top) * kNear;  // (of the whole warp: lanes past the edges bring 0)
-        const bool flag = there && v != 0.f && fabsf(v) <= near;
-        if (__popc(__ballot_sync(0xffffffffu, flag)) <= 2) v = settled<T>(e, flag, row, col, v, lane);
+        v = settled_row<T>(e.near, there, near, row, col, v, lane);
       }
       if (!there) continue;
       T *o = static_cast<T *>(batch ? e.out1 : e.out0) + row * e.ldo + col;
@@ -1321,23 +1309,21 @@ void run(const Product &g, Workspace &ws, cudaStream_t s) {
   }
   switch (g.epi) {
     case E_LINEAR: launch_epi<E_LINEAR>(g.dt, tile, maps, q, s); break;
-    case E_LINEAR_BWD: launch_epi<E_LINEAR_BWD>(g.dt, tile, maps, q, s); break;
+    case E_LINEAR_BWD:
+      if (g.e.near.x) launch_epi<E_LINEAR_BWD | E_RELU>(g.dt, tile, maps, q, s);
+      else launch_epi<E_LINEAR_BWD>(g.dt, tile, maps, q, s);
+      break;
     case E_GATED: launch_epi<E_GATED>(g.dt, tile, maps, q, s); break;
-    default: launch_epi<E_GATED_BWD>(g.dt, tile, maps, q, s); break;
+    default:
+      if (g.e.near.x) launch_epi<E_GATED_BWD | E_RELU>(g.dt, tile, maps, q, s);
+      else launch_epi<E_GATED_BWD>(g.dt, tile, maps, q, s);
+      break;
   }
 }
 
 void zero_rows(void *p, int64_t ld, int64_t rows, int64_t cols, int dt, cudaStream_t s) {
   if (p && rows > 0)
     CUDA_CHECK(cudaMemset2DAsync(p, ld * dtype_size(dt), 0, cols * dtype_size(dt), rows, s));
-}
-
-void settle_from(EpiArgs &e, const Mat &x, const Mat &w, int64_t K) {
-  e.nx = x.p;
-  e.nldx = x.ld;
-  e.nw = w.p;
-  e.nldw = w.ld;
-  e.nk = K;
 }
 
 EpiArgs plain_out(const MutMat &m) {
@@ -1528,7 +1514,7 @@ void gated_linear_bwd(const GatedLinear &a, Workspace &ws, cudaStream_t s) {
   g.e.b1 = a.bv;
   g.e.in = a.dh.p;
   g.e.ldin = a.dh.ld;
-  if (a.act == ACT_RELU) settle_from(g.e, a.x, a.wg, a.K);
+  if (a.act == ACT_RELU) g.e.near = {a.x.p, a.wg.p, a.bg, a.x.ld, a.wg.ld, a.K};
   // bias gradients from the unrounded dz: 16-bit in the epilogue (each 32
   // rows), f32 where dz is split (each 128)
   void *const db[2] = {a.dbg, a.dbv};
@@ -1679,7 +1665,7 @@ void linear_bwd(const Linear &a, Workspace &ws, cudaStream_t s) {
     g.e.b0 = a.b;
     g.e.in = a.dy.p;
     g.e.ldin = a.dy.ld;
-    if (a.act == ACT_RELU) settle_from(g.e, a.x, a.w, a.K);
+    if (a.act == ACT_RELU) g.e.near = {a.x.p, a.w.p, a.b, a.x.ld, a.w.ld, a.K};
     if (!f32) g.e.sums0 = part;
     prep.go();
     run(g, ws, s);

@@ -31,12 +31,12 @@ namespace {
 
 constexpr int kDepth = 4;  // loads in flight per lane and weight (8 cost more in resident warps)
 
-// The epilogue of one result: row m, feature n, both products.  dz of a backward
-// goes out as [product][feature][8 rows], the rows past M zeros.
+// The epilogue of one result: row m, feature n, both products, the first with its
+// bias.  dz of a backward goes out as [product][feature][8 rows], the rows past M
+// zeros.
 constexpr int kRowPad = 8;
 template <typename T, bool DUAL>
 __device__ __forceinline__ void finish(const FewRows &a, int m, int64_t n, float v, float w) {
-  if (a.b0) v += to_f(static_cast<const T *>(a.b0)[n]);
   if (DUAL && a.b1) w += to_f(static_cast<const T *>(a.b1)[n]);
   const float in = a.in ? to_f(static_cast<const T *>(a.in)[m * a.ldin + n]) : 0.f;
   float da;
@@ -50,6 +50,8 @@ __device__ __forceinline__ void finish(const FewRows &a, int m, int64_t n, float
     if (DUAL) a.dz[(a.N + n) * kRowPad + m] = v * in;
   }
 }
+
+__device__ __forceinline__ NearZero near_of(const FewRows &a) { return {a.x, a.w0, a.b0, a.ldx, a.ldw0, a.K}; }
 
 // D += A B with A 16 x 16 (four registers a lane), B 16 x 8 (two).
 template <typename T>
@@ -123,23 +125,27 @@ __global__ void __launch_bounds__(256) k_few_mma(const FewRows a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) part[warp][q][i][(2 * t + j % 2) * 16 + g + 8 * (j / 2)] = d[q][i][j];
   __syncthreads();
-  for (int i = threadIdx.x; i < NT * 128; i += 256) {
+  for (int i = threadIdx.x; i < NT * 128; i += 256) {  // (whole warps)
     const int m = i / 16;
     const int64_t n = n0 + i % 16;
-    if (n >= a.N) continue;
-    if (m >= a.M) {
-      if (!a.out && m < kRowPad) {
-        a.dz[n * kRowPad + m] = 0.f;
-        if (DUAL) a.dz[(a.N + n) * kRowPad + m] = 0.f;
-      }
-      continue;
+    const bool there = n < a.N && m < a.M;
+    if (n < a.N && m >= a.M && !a.out && m < kRowPad) {
+      a.dz[n * kRowPad + m] = 0.f;
+      if (DUAL) a.dz[(a.N + n) * kRowPad + m] = 0.f;
     }
-    float v[2] = {0.f, 0.f};
+    float v[2] = {0.f, 0.f}, top = 0.f;
 #pragma unroll
     for (int q = 0; q < NP; ++q)
 #pragma unroll
-      for (int s = 0; s < 8; ++s) v[q] += part[s][q][m / 8][(m % 8) * 16 + i % 16];
-    finish<T, DUAL>(a, m, n, v[0], v[1]);
+      for (int s = 0; s < 8; ++s) {
+        const float t = part[s][q][m / 8][(m % 8) * 16 + i % 16];
+        v[q] += t;
+        if (q == 0) top = fmaxf(top, fabsf(t));
+      }
+    if (there && a.b0) v[0] += to_f(static_cast<const T *>(a.b0)[n]);
+    if (!a.out && a.act == ACT_RELU)
+      v[0] = settled_row<T>(near_of(a), there, warp_max(there ? top : 0.f) * kNear, m, n, v[0], lane);
+    if (there) finish<T, DUAL>(a, m, n, v[0], v[1]);
   }
 }
 
@@ -239,6 +245,14 @@ __global__ void __launch_bounds__(256) k_few_rows(const FewRows a, int wpr) {
   if (!a.out && lane >= a.M && lane < kRowPad) {
     a.dz[n * kRowPad + lane] = 0.f;
     if (DUAL) a.dz[(a.N + n) * kRowPad + lane] = 0.f;
+  }
+  if (a.b0) v += to_f(static_cast<const T *>(a.b0)[n]);
+  if (!a.out && a.act == ACT_RELU) {
+    // the partial sums of this warp's lanes stand for those of all
+    float top = 0.f;
+#pragma unroll
+    for (int m = 0; m < MR; ++m) top = fmaxf(top, fmaxf(fabsf(pair[m].x), fabsf(pair[m].y)));
+    v = settled_row<T>(near_of(a), lane < a.M, warp_max(top) * kNear, lane, n, v, lane, kFewRows);
   }
   if (lane >= a.M) return;
   finish<T, DUAL>(a, lane, n, v, w);

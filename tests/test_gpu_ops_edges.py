@@ -168,3 +168,30 @@ def test_activations_far_out(dtype, act, shape):
                 (ops.gated_linear_backward(one, x, w, v, None, c, act)[0][rows, 0], da, "gated dx")):
             # p = 1 / (1 + e^-z) is 0 or 1 to 2^-126 here
             assert ((got.double() - ref).abs() <= u * ref.abs() + 1e-30).all(), (what, zi, got, ref)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("shape", [(5, 640, 529), (3000, 640, 529), (200, 2500, 72)], ids=str)
+def test_relu_of_sums_that_cancel(dtype, shape):
+    """Two terms of 2^12 that cancel leave a third one of 2^-24 or -2^-24,
+    which is below the last bit of a 32-bit sum: the derivative is the third
+    term's."""
+    m, k, f = shape
+    g = gen(7 * m + k)
+    x, w = rand(g, m, k, dtype=dtype), rand(g, f, k, dtype=dtype, std=k ** -0.5)
+    x[:, 0] = x[:, 1] = 1
+    x[:, 2] = 2.0 ** -10
+    x[::2, 2] = -2.0 ** -10
+    w[5::40] = 0
+    w[5::40, 0], w[5::40, 1], w[5::40, 2] = 2.0 ** 12, -2.0 ** 12, 2.0 ** -14
+    dy = rand(g, m, f, dtype=dtype)
+    zero, v = torch.zeros(f, dtype=dtype, device="cuda"), rand(g, f, k, dtype=dtype, std=k ** -0.5)
+    dz = dy.double() * (x.double() @ w.double().T > 0)
+    # each term counts whole or not at all
+    db = ops.linear_backward(dy, x, w, zero, "relu")[2]
+    assert ((db.double() - dz.sum(0)).abs() <= unit(dtype) * dz.sum(0).abs() + 2.0 ** -18 * dz.abs().sum(0))[5::40].all()
+    dbg = ops.gated_linear_backward(dy, x, w, v, zero, None, "relu")[3]
+    t = dz * (x.double() @ v.double().T)
+    # (the value's own sum is good to c_of of its terms)
+    e = (dz.abs() * (x.double().abs() @ v.double().abs().T)).sum(0) * c_of(k, dtype)
+    assert ((dbg.double() - t.sum(0)).abs() <= unit(dtype) * t.sum(0).abs() + e + 2.0 ** -15 * t.abs().sum(0))[5::40].all()
