@@ -211,12 +211,17 @@ mlipcpp_error_t mlipcpp_b200_domain_stats(mlipcpp_b200_domain_t domain, double s
  * inputs, but for a residual that is also the output with the same stride.
  *
  * Products accumulate in fp32; activations, norms and sums run in fp32 and
- * each output is rounded once.  f32 products have fp32 accuracy (22-bit
- * split operands; one operand has a scale per 128 elements of its sums, the
- * other one per block of 128 x 128).  A backward call recomputes what it needs
- * from the forward's inputs; gradients that enter a product are rounded to the
- * call's type first.  The derivative of relu at 0 is 0.  Results do not depend on timing: no sum's order varies.
- * In f32 an infinite element makes its row or column of a product NaN.
+ * each output is rounded once.  f32 products from 9 rows on take their
+ * operands in two halves of 22 bits together, with a scale for each row of
+ * either operand (each row and column of the result) and 128 elements of the
+ * sum: an element is good to 2^-22 of itself and to 2^-32 of the largest of
+ * those 128, and rows and features may differ in size by any factor.  An
+ * infinite element then makes its row or column of a product NaN.
+ *
+ * A backward call recomputes what it needs from the forward's inputs;
+ * gradients that enter a product are rounded to the call's type first.  The
+ * derivative of relu at 0 is 0.  Results do not depend on timing: no sum's
+ * order varies.
  *
  * `workspace`: device memory of at least the bytes that the matching
  * *_workspace call gives for the same arguments, 256-byte aligned (NULL where

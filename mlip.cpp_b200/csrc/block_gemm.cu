@@ -13,13 +13,15 @@
 //  * 16-bit: one kind::f16 product, fp32 accumulation in tensor memory over
 //    the whole contraction; BN = 256 (one 128 x 256 tile, two accumulators)
 //    or 128 (four accumulators) when 256-wide tiles would leave SMs idle.
-//  * f32: A = 2^-s (hi + lo) with one scale per row and 128 contraction
-//    elements, B = 2^-t (hi + lo) with one scale per 128 x 128 block (one for
-//    all of a model's weight, split when it was loaded) in the way of
-//    split16.cuh; A_lo B_hi + A_hi B_lo + A_hi B_hi per step.  The tensor core
-//    truncates when it adds to its accumulator, so every 128 contraction
-//    elements the accumulator warps add the partial sum to fp32 registers
-//    with round-to-nearest.
+//  * f32: A = 2^-s (hi + lo) and B = 2^-t (hi + lo) with one scale per row (the
+//    output's row or column) and 128 contraction elements (one for all of a
+//    model's weight, split when it was loaded) in the way of split16.cuh;
+//    A_lo B_hi + A_hi B_lo + A_hi B_hi per step.  With one scale per 128 x
+//    128 block of B, features 2^-36 below their block's largest were a quarter
+//    off; the scales per column cost 0.5 to 3% of a call of 65,202 rows.  The
+//    tensor core truncates when it adds to its accumulator, so every 128
+//    contraction elements the accumulator warps add the partial sum to fp32
+//    registers with round-to-nearest.
 //
 // Pairs (16-bit): where there are enough rows, two SMs take a tile of 256 x 256
 // together (cta_group::2).  Each loads its own 128 rows of A and half of B's
@@ -114,11 +116,11 @@ struct Params {
   int tiles_m, tiles_n, splits, kt_split, batch;
   int a_mn, b_mn, dual, bf16, products;
   int *err;                        // error word, or null for the file's own
-  const int8_t *sc[2];             // f32: scale exponents of A, [block][row]
-  int64_t scld[2];
-  const int8_t *bs[2];             // f32: scale exponents of B's blocks, or null
-  int64_t bsn[2], bsk[2];          // ... their strides by 128 rows and 128 k
-  float bsc[2];                    // ... else this factor
+  // f32: scales 2^-s, the upper halves of the floats, of A [block][row] and of
+  // B [block][column] (or null: one pair of them)
+  const uint16_t *sc[2], *bs[2];
+  int64_t scld[2], bsld[2];
+  uint16_t bsc[2];
   EpiArgs e;
 };
 
@@ -652,28 +654,36 @@ __global__ void __launch_bounds__(kThreads, 1) k_block_gemm(const __grid_constan
         for (int gi = 0; gi < 2; ++gi)
 #pragma unroll
           for (int j = 0; j < GA; ++j) acc[gi][j] = 0.f;
-        // scale exponents of this thread's row and of each group's columns in
-        // one pass, requested a pass ahead and not touched before it
-        int sa = 0, sb[2] = {0, 0};
+        // scales of this thread's row and of column `lane` of each group in one
+        // pass, requested a pass ahead and not touched before it
+        uint32_t sa = 0, sb[2] = {p.bsc[0], p.bsc[p.dual ? 1 : 0]};
         auto scales = [&](int kt) {
           const int seg = kt >= p.kt0 ? 1 : 0, o = t.batch | seg;
           const int blk = (kt - (seg ? p.kt0 : 0)) / C::Chunk;
           if (row < p.M) sa = p.sc[o][static_cast<size_t>(blk) * p.scld[o] + row];
 #pragma unroll
           for (int gi = 0; gi < 2; ++gi) {
-            const int bi = p.dual ? (cb[gi] >= BN / 2 ? 1 : 0) : seg;
-            if (p.bs[bi]) sb[gi] = p.bs[bi][((n0 + (p.dual ? 0 : cb[gi])) / 128) * p.bsn[bi] + blk * p.bsk[bi]];
+            const int half = p.dual && cb[gi] >= BN / 2 ? 1 : 0, bi = p.dual ? half : seg;
+            const int col = min(n0 + cb[gi] - half * (BN / 2) + lane, p.N - 1);
+            sb[gi] = p.bs[bi] ? p.bs[bi][static_cast<size_t>(blk) * p.bsld[bi] + col] : p.bsc[bi];
           }
         };
         scales(k0);
         for (int kt = k0; kt < k_end; kt += C::Chunk, ++pass) {
-          const float fa = pow2f(-sa);
+          const float fa = __uint_as_float(sa << 16);
+          // columns of one scale (of ordinary sizes, by k_split's choice) need
+          // one factor; others theirs, by way of `st`
           float f[2];
+          bool even[2];
+          __syncwarp();  // the pass before has been read
 #pragma unroll
           for (int gi = 0; gi < 2; ++gi) {
-            const int bi = p.dual ? (cb[gi] >= BN / 2 ? 1 : 0) : (kt >= p.kt0 ? 1 : 0);
-            f[gi] = fa * (p.bs[bi] ? pow2f(-sb[gi]) : p.bsc[bi]);
+            const float fb = __uint_as_float(sb[gi] << 16);
+            f[gi] = fa * __shfl_sync(0xffffffffu, fb, 0);
+            even[gi] = __all_sync(0xffffffffu, sb[gi] == __shfl_sync(0xffffffffu, sb[gi], 0));
+            if (!even[gi]) st[gi * 32 + lane] = fb;
           }
+          __syncwarp();
           if (kt + C::Chunk < k_end) scales(kt + C::Chunk);
           b = pass % C::Bufs;
           if (!__all_sync(0xffffffffu, wait_or_abort(accf0 + 8 * b, (pass / C::Bufs) & 1, abort_flag))) {
@@ -687,8 +697,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_block_gemm(const __grid_constan
             float v[32];
             tmem_ld32(tq + static_cast<uint32_t>(b * BN + cb[gi]), v);
             if (gi) release(b);
+            if (even[gi]) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) acc[gi][F32 ? j : 0] = __fmaf_rn(v[j], f[gi], acc[gi][F32 ? j : 0]);
+              for (int j = 0; j < 32; ++j) acc[gi][F32 ? j : 0] = __fmaf_rn(v[j], f[gi], acc[gi][F32 ? j : 0]);
+            } else {  // (the two scales first: either may be far from 1)
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                acc[gi][F32 ? j : 0] = __fmaf_rn(v[j], fa * st[gi * 32 + j], acc[gi][F32 ? j : 0]);
+            }
           }
         }
         if (!ok) break;
@@ -858,27 +874,34 @@ __device__ __forceinline__ float finite_abs(float x) {
 // writes each form that a product needs of it:
 //   rows    one scale per row and 128 columns, [column block][row]
 //   cols    one scale per column and 128 rows, [row block][column]
-//   blocks  one scale per block, [row block][column block]
+// (2^-s: the upper half of the float).  Of a B operand, whose scales the product
+// applies to columns, the rows (columns) within 2^-kEven of their block's largest
+// take its scale: an element keeps 2^-40 of what its scale is for, 2^-32 of its
+// own row's (column's) largest, far below the 2^-22 that it is good to.
 // and, for bias gradients, the sums of its columns, [row block][column].
 // All forms are [R][lp] hi, then lo.
 struct SplitForm {
-  uint16_t *hi;
-  int8_t *sc;
+  uint16_t *hi, *sc;
+  int64_t scld;
+  bool even;
 };
 struct SplitJob {
   const float *src;
   int64_t ld;
   int R, C, lp, first;  // first: number of the job's first block
   bool vec;
-  SplitForm rows, cols, blocks;
+  SplitForm rows, cols;
   float *sums;
 };
+// 2^-s as the upper half of a float
+__host__ __device__ __forceinline__ uint16_t scale_bits(int s) { return static_cast<uint16_t>((127 - s) << 7); }
+constexpr int kEven = 8;
 constexpr int kMaxJobs = 4;
 struct SplitJobs {
   SplitJob job[kMaxJobs];
   int n, total;
 };
-__global__ void __launch_bounds__(256) k_split(const SplitJobs all) {
+__global__ void __launch_bounds__(256, 2) k_split(const SplitJobs all) {
   __shared__ float part[8][128];
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int id = blockIdx.x; id < all.total; id += gridDim.x) {
@@ -931,46 +954,64 @@ __global__ void __launch_bounds__(256) k_split(const SplitJobs all) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) out[j] = add ? out[j] + part[k][4 * lane + j] : fmaxf(out[j], part[k][4 * lane + j]);
     };
+    // exponent of one row (column) by its largest element, given the block's
+    // least (kNone: nothing but zeros)
+    constexpr int kNone = 1 << 20;
+    auto exponent = [](float m) { return m > 0.f ? split_scale_exponent(m) : kNone; };
+    auto choose = [](int s, int least, bool even) {
+      if (s == kNone) return least == kNone ? 0 : least;
+      return even && s - least <= kEven ? least : s;
+    };
     if (q.rows.hi) {
+      int s[16], least = kNone;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         float m = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) m = fmaxf(m, finite_abs(v[i][j]));
-        const int s = split_scale_exponent(warp_max(m));
-        const float e = pow2f(s), f[4] = {e, e, e, e};
+        s[i] = exponent(warp_max(m));
+        least = min(least, s[i]);
+      }
+      if (q.rows.even) {
+        __syncthreads();
+        if (lane == 0) part[w][0] = __int_as_float(least);
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) least = min(least, __float_as_int(part[k][0]));
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int si = choose(s[i], least, q.rows.even);
+        const float e = pow2f(si), f[4] = {e, e, e, e};
         put(q.rows.hi, i, f);
-        if (lane == 0 && r0 + i < q.R) q.rows.sc[static_cast<size_t>(cb) * q.R + r0 + i] = static_cast<int8_t>(s);
+        if (lane == 0 && r0 + i < q.R) q.rows.sc[static_cast<size_t>(cb) * q.rows.scld + r0 + i] = scale_bits(si);
       }
     }
-    if (q.cols.hi || q.blocks.hi) {
+    if (q.cols.hi) {
       float m[4] = {0.f, 0.f, 0.f, 0.f}, top[4];
 #pragma unroll
       for (int i = 0; i < 16; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) m[j] = fmaxf(m[j], finite_abs(v[i][j]));
       over_rows(m, false, top);
-      if (q.cols.hi) {
-        int s[4];
-        float f[4];
+      int s[4], least = kNone;
+      float f[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s[j] = split_scale_exponent(top[j]);
-          f[j] = pow2f(s[j]);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) put(q.cols.hi, i, f);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (w == 0 && c + j < q.lp) q.cols.sc[static_cast<size_t>(rb) * q.lp + c + j] = static_cast<int8_t>(s[j]);
+      for (int j = 0; j < 4; ++j) {
+        s[j] = exponent(top[j]);
+        least = min(least, s[j]);
       }
-      if (q.blocks.hi) {
-        const int s = split_scale_exponent(warp_max(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))));
-        const float e = pow2f(s), f[4] = {e, e, e, e};
+      least = __reduce_min_sync(0xffffffffu, least);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) put(q.blocks.hi, i, f);
-        if (threadIdx.x == 0) q.blocks.sc[static_cast<size_t>(rb) * nb + cb] = static_cast<int8_t>(s);
+      for (int j = 0; j < 4; ++j) {
+        s[j] = choose(s[j], least, q.cols.even);
+        f[j] = pow2f(s[j]);
       }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) put(q.cols.hi, i, f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (w == 0 && c + j < q.lp) q.cols.sc[static_cast<size_t>(rb) * q.cols.scld + c + j] = scale_bits(s[j]);
     }
     if (q.sums) {
       float m[4] = {0.f, 0.f, 0.f, 0.f}, sum[4];
@@ -1026,21 +1067,21 @@ struct Operand {
   int64_t rows = 0, cols = 0, ld = 0;
   int planes = 1;
   int64_t plane = 0;           // elements between hi and lo
-  const int8_t *sc = nullptr;  // f32: scale exponents
-  int64_t scld = 0;            // ... between the blocks of 128 (A: of the contraction; B: of rows)
-  float bsc = 1.f;             // f32 B without sc: one factor
+  const uint16_t *sc = nullptr;  // f32: scales
+  int64_t scld = 0;              // ... between the contraction's blocks of 128
+  int scale = 0;                 // f32 B without sc: one exponent
 };
 
 // Prepares operands: 16-bit ones where they lie (or packed), f32 ones in split
 // form, by one launch each, issued by go().
-enum Form { FORM_NONE, FORM_ROWS, FORM_COLS, FORM_BLOCKS };
+enum Form { FORM_NONE, FORM_ROWS, FORM_COLS };
 class Operands {
  public:
   Operands(int dt, Workspace &ws, cudaStream_t s) : dt_(dt), ws_(ws), s_(s) {}
 
-  // `m` for a product: FORM_ROWS / FORM_COLS as its A operand, contracted over
-  // columns / rows, FORM_BLOCKS as its B operand
-  Operand add(const Mat &m, int64_t rows, int64_t cols, Form form) {
+  // `m` for a product that contracts its columns (FORM_ROWS) or rows (FORM_COLS);
+  // even: as the B operand
+  Operand add(const Mat &m, int64_t rows, int64_t cols, Form form, bool even = false) {
     if (dt_ != DT_F32) return packed(m, rows, cols);
     Operand o;
     o.rows = rows;
@@ -1050,12 +1091,12 @@ class Operands {
     o.plane = rows * o.ld;
     uint16_t *d = static_cast<uint16_t *>(ws_.take(4 * rows * o.ld));
     const int64_t rb = (rows + 127) / 128, cb = (cols + 127) / 128;
-    o.scld = form == FORM_ROWS ? rows : form == FORM_COLS ? o.ld : cb;
-    int8_t *sc = static_cast<int8_t *>(ws_.take(form == FORM_ROWS ? cb * rows : rb * o.scld));
+    o.scld = form == FORM_ROWS ? rows : o.ld;
+    uint16_t *sc = static_cast<uint16_t *>(ws_.take(2 * (form == FORM_ROWS ? cb : rb) * o.scld));
     o.p = d;
     o.sc = sc;
     if (ws_.sizing()) return o;
-    of(job(m, rows, cols, form), form) = SplitForm{d, sc};
+    of(job(m, rows, cols, form), form) = SplitForm{d, sc, o.scld, even};
     return o;
   }
   // f32: sums of the columns of each 128 rows of `m` into part [rows / 128][cols]
@@ -1083,7 +1124,7 @@ class Operands {
   }
 
  private:
-  static SplitForm &of(SplitJob &j, Form f) { return f == FORM_ROWS ? j.rows : f == FORM_COLS ? j.cols : j.blocks; }
+  static SplitForm &of(SplitJob &j, Form f) { return f == FORM_ROWS ? j.rows : j.cols; }
   // the job that reads `m`: one for all forms of one matrix (a second one if
   // it has this form already, as when both weights are the same tensor)
   SplitJob &job(const Mat &m, int64_t rows, int64_t cols, Form form) {
@@ -1293,9 +1334,8 @@ void run(const Product &g, Workspace &ws, cudaStream_t s) {
     q.sc[i] = a.sc;
     q.scld[i] = a.scld;
     q.bs[i] = b.sc;
-    q.bsn[i] = g.b_mn ? 1 : b.scld;
-    q.bsk[i] = g.b_mn ? b.scld : 1;
-    q.bsc[i] = b.bsc;
+    q.bsld[i] = b.scld;
+    q.bsc[i] = scale_bits(b.scale);
   }
   if (splits > 1) {
     launch_epi<E_PARTIAL>(g.dt, tile, maps, q, s);
@@ -1379,7 +1419,7 @@ Operand split_weight(const GatedLinear::SplitWeight &w, int64_t rows, int64_t co
   o.cols = o.ld = cols;
   o.planes = w.lo ? 2 : 1;
   o.plane = w.lo ? w.lo - w.hi : 0;
-  o.bsc = std::ldexp(1.f, -w.scale);
+  o.scale = w.scale;
   return o;
 }
 
@@ -1445,8 +1485,8 @@ void gated_linear_fwd(const GatedLinear &a, Workspace &ws, cudaStream_t s) {
   g.K = a.K;
   g.dual = true;
   g.a[0] = prep.add(a.x, a.M, a.K, FORM_ROWS);
-  g.b[0] = a.wg_split.hi ? split_weight(a.wg_split, a.F, a.K) : prep.add(a.wg, a.F, a.K, FORM_BLOCKS);
-  g.b[1] = a.wv_split.hi ? split_weight(a.wv_split, a.F, a.K) : prep.add(a.wv, a.F, a.K, FORM_BLOCKS);
+  g.b[0] = a.wg_split.hi ? split_weight(a.wg_split, a.F, a.K) : prep.add(a.wg, a.F, a.K, FORM_ROWS, true);
+  g.b[1] = a.wv_split.hi ? split_weight(a.wv_split, a.F, a.K) : prep.add(a.wv, a.F, a.K, FORM_ROWS, true);
   g.e = plain_out(a.h);
   g.e.act = a.act;
   g.e.b0 = a.bg;
@@ -1491,15 +1531,21 @@ void gated_linear_bwd(const GatedLinear &a, Workspace &ws, cudaStream_t s) {
   char *buf = static_cast<char *>(ws.take(2 * a.M * fp * es));
   const MutMat dz[2] = {{buf, fp}, {ws.sizing() ? nullptr : buf + a.M * fp * es, fp}};
   Operands prep(a.dtype, ws, s);
-  Operand w[2], xb;
-  w[0] = a.wg_split.hi ? split_weight(a.wg_split, a.F, a.K) : prep.add(a.wg, a.F, a.K, FORM_BLOCKS);
-  w[1] = a.wv_split.hi ? split_weight(a.wv_split, a.F, a.K) : prep.add(a.wv, a.F, a.K, FORM_BLOCKS);
+  // the weights contract their inputs for the projections, their features for
+  // dx; only f32 tells the two apart
+  Operand w[2], wc[2], xb;
+  const Mat wm[2] = {a.wg, a.wv};
+  const GatedLinear::SplitWeight *const split[2] = {&a.wg_split, &a.wv_split};
+  for (int i = 0; i < 2; ++i) {
+    w[i] = split[i]->hi ? split_weight(*split[i], a.F, a.K) : prep.add(wm[i], a.F, a.K, FORM_ROWS, true);
+    wc[i] = f32 && a.dx.p && !split[i]->hi ? prep.add(wm[i], a.F, a.K, FORM_COLS, true) : w[i];
+  }
   Product g;
   g.dt = a.dtype;
   g.products = a.products;
   g.err = a.err;
   g.a[0] = prep.add(a.x, a.M, a.K, FORM_ROWS);
-  if (weights) xb = f32 ? prep.add(a.x, a.M, a.K, FORM_BLOCKS) : g.a[0];
+  if (weights) xb = f32 ? prep.add(a.x, a.M, a.K, FORM_COLS, true) : g.a[0];
   g.epi = E_GATED_BWD;
   g.M = a.M;
   g.N = a.F;
@@ -1551,7 +1597,7 @@ void gated_linear_bwd(const GatedLinear &a, Workspace &ws, cudaStream_t s) {
     q.b_mn = true;
     for (int i = 0; i < 2; ++i) {
       q.a[i] = rows[i];
-      q.b[i] = w[i];
+      q.b[i] = wc[i];
     }
     q.e = plain_out(a.dx);
     run(q, ws, s);
@@ -1604,7 +1650,7 @@ void linear_fwd(const Linear &a, Workspace &ws, cudaStream_t s) {
   g.N = a.N;
   g.K = a.K;
   g.a[0] = prep.add(a.x, a.M, a.K, FORM_ROWS);
-  g.b[0] = prep.add(a.w, a.N, a.K, FORM_BLOCKS);
+  g.b[0] = prep.add(a.w, a.N, a.K, FORM_ROWS, true);
   g.e = plain_out(a.y);
   g.e.act = a.act;
   g.e.scale = a.scale;
@@ -1639,10 +1685,11 @@ void linear_bwd(const Linear &a, Workspace &ws, cudaStream_t s) {
   }
   const bool id = a.act == ACT_IDENTITY, f32 = a.dtype == DT_F32;
   Operands prep(a.dtype, ws, s);
-  Operand w, xr, xb;
-  if (!id || a.dx.p) w = prep.add(a.w, a.N, a.K, FORM_BLOCKS);
+  Operand wr, wc, xr, xb;  // as in gated_linear_bwd
+  if (!id) wr = prep.add(a.w, a.N, a.K, FORM_ROWS, true);
+  if (a.dx.p) wc = f32 || id ? prep.add(a.w, a.N, a.K, FORM_COLS, true) : wr;
   if (!id) xr = prep.add(a.x, a.M, a.K, FORM_ROWS);
-  if (a.dw.p) xb = f32 || id ? prep.add(a.x, a.M, a.K, FORM_BLOCKS) : xr;
+  if (a.dw.p) xb = f32 || id ? prep.add(a.x, a.M, a.K, FORM_COLS, true) : xr;
   Mat dz = a.dy;
   // bias gradient: without an activation the sums of dy itself, else as in
   // gated_linear_bwd
@@ -1658,7 +1705,7 @@ void linear_bwd(const Linear &a, Workspace &ws, cudaStream_t s) {
     g.N = a.N;
     g.K = a.K;
     g.a[0] = xr;
-    g.b[0] = w;
+    g.b[0] = wr;
     g.e = plain_out(out);
     g.e.act = a.act;
     g.e.scale = a.scale;
@@ -1685,7 +1732,7 @@ void linear_bwd(const Linear &a, Workspace &ws, cudaStream_t s) {
     g.K = a.N;
     g.b_mn = true;
     g.a[0] = rows;
-    g.b[0] = w;
+    g.b[0] = wc;
     g.e = plain_out(a.dx);
     g.e.scale = scale;
     run(g, ws, s);

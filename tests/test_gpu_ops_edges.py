@@ -195,3 +195,55 @@ def test_relu_of_sums_that_cancel(dtype, shape):
     # (the value's own sum is good to c_of of its terms)
     e = (dz.abs() * (x.double().abs() @ v.double().abs().T)).sum(0) * c_of(k, dtype)
     assert ((dbg.double() - t.sum(0)).abs() <= unit(dtype) * t.sum(0).abs() + e + 2.0 ** -15 * t.abs().sum(0))[5::40].all()
+
+
+@pytest.mark.parametrize("m", [150, 700])
+def test_f32_features_of_different_sizes(m):
+    """f32 products keep their accuracy in every row and column on its own:
+    weights whose output features, and weights and inputs whose input
+    features, lie up to 2^-36 below the largest of their matrix.
+
+    The bound is c_of of the terms' magnitude, per element of each result: a
+    feature's scale multiplies all terms of its row or column alike, and along
+    a contraction the sizes of both factors fall together, so that a block's
+    largest elements meet."""
+    k, n = 200, 300
+    g = gen(m)
+    f32 = torch.float32
+    fall = 2.0 ** torch.linspace(0, -36, n, device="cuda").round()
+    wide = 2.0 ** torch.linspace(0, -36, k, device="cuda").round()
+
+    def mixed(t, perm_seed):
+        return t[torch.randperm(len(t), generator=gen(perm_seed)).cuda()]
+
+    rows, cols = mixed(fall, 1), mixed(wide, 2)
+    x = rand(g, m, k, dtype=f32) * cols
+    w = rand(g, n, k, dtype=f32) * rows[:, None] * cols
+    v = rand(g, n, k, dtype=f32) * rows[:, None] * cols
+    dy = rand(g, m, n, dtype=f32)
+    c = c_of(max(m, 2 * n), f32) + 2.0 ** -22
+    X, W, V, D = (t.double() for t in (x, w, v, dy))
+
+    def check(got, a, b, what):
+        ref, s = a @ b, a.abs() @ b.abs()
+        bad = (got.double() - ref).abs() / s
+        assert (bad <= c).all(), (what, bad.max().item(), c)
+
+    check(ops.linear(x, w), X, W.T, "y")
+    dx, dw, _ = ops.linear_backward(dy, x, w)
+    check(dx, D, W, "dx")
+    check(dw, D.T, X, "dw")
+    # with one projection the identity of the other: h = (x Wg^T) (x Wv^T)
+    h = ops.gated_linear(x, w, v, None, None, "identity")
+    gate, value = X @ W.T, X @ V.T
+    sg, sv = X.abs() @ W.abs().T, X.abs() @ V.abs().T
+    assert ((h.double() - gate * value).abs() <= c * (sg * value.abs() + gate.abs() * sv + c * sg * sv)
+            + 2.0 ** -22 * (gate * value).abs()).all()
+    gdx, dwg, dwv, _, _ = ops.gated_linear_backward(dy, x, w, v, None, None, "identity")
+    dg, dv = D * value, D * gate
+    eg, ev = D.abs() * sv * c + 2.0 ** -22 * dg.abs(), D.abs() * sg * c + 2.0 ** -22 * dv.abs()
+    for got, ref, tol, what in (
+            (gdx, dg @ W + dv @ V, (c * dg.abs() + eg) @ W.abs() + (c * dv.abs() + ev) @ V.abs(), "gated dx"),
+            (dwg, dg.T @ X, (c * dg.abs() + eg).T @ X.abs(), "dw_gate"),
+            (dwv, dv.T @ X, (c * dv.abs() + ev).T @ X.abs(), "dw_value")):
+        assert ((got.double() - ref).abs() <= tol).all(), (what, ((got.double() - ref).abs() / tol).max().item())
