@@ -11,7 +11,7 @@
 // backward pass needs a transposed copy.
 //
 //  * 16-bit: one kind::f16 product, fp32 accumulation in tensor memory over
-//    the whole contraction; BN = 256 (one 128 x 256 tile, two accumulators)
+//    the whole contraction (divided where its truncations could show, see run); BN = 256 (one 128 x 256 tile, two accumulators)
 //    or 128 (four accumulators) when 256-wide tiles would leave SMs idle.
 //  * f32: A = 2^-s (hi + lo) and B = 2^-t (hi + lo) with one scale per row (the
 //    output's row or column) and 128 contraction elements (one for all of a
@@ -1310,6 +1310,13 @@ void run(const Product &g, Workspace &ws, cudaStream_t s) {
   if (tiles * 2 <= at_once && p.kt >= 16) {
     splits = static_cast<int>(std::min<int64_t>(at_once / tiles, p.kt / 4));
     if (p.kt - (p.kt + splits - 1) / splits < 20) splits = 1;
+  }
+  // 16-bit: an accumulator takes each 16 terms with one truncation of at most
+  // 2^-23 of the sum (f32 joins in registers instead).  Beyond this many all of
+  // them together could pass half a rounding of the result: divided further.
+  if (!f32) {
+    const int most = (g.dt == DT_F16 ? 32768 : 262144) / BK;  // 2^11 steps of 2^-23 against 2^-11 / 2, 2^14 against 2^-8 / 2
+    splits = std::max(splits, (p.kt + most - 1) / most);
   }
   p.kt_split = (p.kt + splits - 1) / splits;
   p.kt_split = (p.kt_split + unit - 1) / unit * unit;

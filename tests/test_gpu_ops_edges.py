@@ -8,7 +8,7 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 import mlipcpp_b200 as mb  # noqa: E402
-from test_gpu_ops import DTYPES, IDS, act64, c_of, gen, rand, unit  # noqa: E402
+from test_gpu_ops import DTYPES, IDS, act64, c_of, check_gated, gen, rand, unit  # noqa: E402
 
 if torch.cuda.is_available():
     from mlipcpp_b200 import ops
@@ -247,3 +247,29 @@ def test_f32_features_of_different_sizes(m):
             (dwg, dg.T @ X, (c * dg.abs() + eg).T @ X.abs(), "dw_gate"),
             (dwv, dv.T @ X, (c * dv.abs() + ev).T @ X.abs(), "dw_value")):
         assert ((got.double() - ref).abs() <= tol).all(), (what, ((got.double() - ref).abs() / tol).max().item())
+
+
+def test_long_f16_contraction():
+    """A weight's gradient over 2^20 tokens: the additions of one accumulator
+    lose at most half a rounding of the result in all, however long the
+    contraction is.  All elements of dy^T x are the same sum of equal terms."""
+    m, n = 1 << 20, 2304
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB of free device memory")
+    f16 = torch.float16
+    a, b, scale = 1 + 37 / 1024, 1 + 101 / 1024, 2.0 ** -14
+    x, dy = torch.full((m, n), a, dtype=f16, device="cuda"), torch.full((m, n), b, dtype=f16, device="cuda")
+    dw = ops.linear_backward(dy, x, x[:n], scale=scale, needs=(False, True, False))[1]
+    ref = m * a * b * scale
+    u = unit(f16)
+    assert (dw.double() - ref).abs().max().item() <= 1.5 * u * (1 + u) * ref
+
+
+def test_long_f16_projection():
+    """Both projections with more inputs than one accumulator takes, over more
+    tiles than there are SMs."""
+    g, f16 = gen(33), torch.float16
+    m, k, f = 2000, 33000, 2700
+    x, dh = rand(g, m, k, dtype=f16), rand(g, m, f, dtype=f16)
+    wg, wv = rand(g, f, k, dtype=f16, std=k ** -0.5), rand(g, f, k, dtype=f16, std=k ** -0.5)
+    check_gated(x, wg, wv, None, dh[0], "silu", dh)
