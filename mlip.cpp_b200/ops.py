@@ -15,7 +15,7 @@ flattened to rows (there may be none); a tensor whose rows are not contiguous
 is copied first.  Everything runs on the tensors' device and its current
 stream, without waiting; the working memory comes from torch's allocator.
 Where an input requires grad, the forwards record themselves for autograd
-(first derivatives); the ``*_backward`` functions are the same gradients
+(first derivatives, reverse mode; forward-mode duals are refused); the ``*_backward`` functions are the same gradients
 called directly.  An autograd backward is captured into a CUDA graph only
 when nothing recorded earlier with the same parameters is still held (torch
 ties a parameter's accumulation to the stream of its first use); the
@@ -30,6 +30,7 @@ import struct
 from collections import namedtuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import INVALID_PARAMETER, MLIPError, _check, lib
 
@@ -74,6 +75,8 @@ def _take(t, first, shape, cols: int, keep: list, name: str):
     had to be copied is appended to `keep`."""
     if t is None:
         return 0, cols
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        _refuse(f"{name} carries a forward-mode tangent, which the operators do not propagate")
     if t.dtype is not first.dtype or t.get_device() != first.get_device():
         _refuse(f"{name} is {t.dtype} on {t.device}, expected {first.dtype} on {first.device}")
     if t.shape != shape:

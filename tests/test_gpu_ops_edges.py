@@ -273,3 +273,21 @@ def test_long_f16_projection():
     x, dh = rand(g, m, k, dtype=f16), rand(g, m, f, dtype=f16)
     wg, wv = rand(g, f, k, dtype=f16, std=k ** -0.5), rand(g, f, k, dtype=f16, std=k ** -0.5)
     check_gated(x, wg, wv, None, dh[0], "silu", dh)
+
+
+def test_forward_mode_is_refused():
+    """The operators have no forward-mode derivatives: a dual tensor is turned
+    down instead of losing its tangent."""
+    from torch.autograd import forward_ad
+    x, w = torch.randn(20, 32, device="cuda"), torch.randn(32, 32, device="cuda")
+    calls = [lambda a, b: ops.linear(a, b), lambda a, b: ops.gated_linear(a, b, w), lambda a, b: ops.residual_norm(a, b[:20]),
+             lambda a, b: ops.linear_backward(x, a, b), lambda a, b: ops.linear(x, w, residual=a, bias=b[0])]
+    with forward_ad.dual_level():
+        dx, dw = forward_ad.make_dual(x, torch.ones_like(x)), forward_ad.make_dual(w, torch.ones_like(w))
+        for call in calls:
+            for a, b in ((dx, w), (x, dw)):
+                with pytest.raises(mb.MLIPError):
+                    call(a, b)
+            call(x, w)
+    for call in calls:
+        call(x, w)

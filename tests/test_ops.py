@@ -192,3 +192,33 @@ class _FakeCuda:
 def test_python_shape_refusals(call):
     with _FakeCuda(), pytest.raises(mb.MLIPError):
         call(torch.zeros(4, 8), torch.zeros(16, 8))
+
+
+def test_forward_mode_is_refused(monkeypatch):
+    """A dual tensor is turned down instead of losing its tangent, whichever
+    argument it is; tensors without one are not."""
+    from torch.autograd import forward_ad
+    x, w = torch.zeros(4, 8), torch.zeros(8, 8)
+    v = torch.zeros(8)
+
+    def calls(x, w, v):
+        return [lambda: ops.gated_linear(x, w, w, v), lambda: ops.linear(x, w, v, residual=x),
+                lambda: ops.residual_norm(x, x, v, v, v, v, v, post_norm="rms"),
+                lambda: ops.gated_linear_backward(x, x, w, w), lambda: ops.linear_backward(x, x, w, v),
+                lambda: ops.residual_norm_backward(x, x, x, x, v, gate=v)]
+
+    reached = []
+    monkeypatch.setattr(ops, "_call", lambda name, *_: reached.append(name))
+    with _FakeCuda(), forward_ad.dual_level():
+        for call in calls(x, w, v):
+            call()
+        assert len(reached) == 6
+        for i in range(3):
+            t = [x, w, v]
+            t[i] = forward_ad.make_dual(t[i], torch.ones_like(t[i]))
+            for n, call in enumerate(calls(*t)):
+                if (i == 1 and n in (2, 5)) or (i == 2 and n == 3):
+                    continue  # (does not take it)
+                with pytest.raises(mb.MLIPError, match="tangent"):
+                    call()
+    assert len(reached) == 6
