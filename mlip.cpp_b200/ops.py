@@ -26,6 +26,7 @@ precision and limits; a refused call raises MLIPError.
 """
 from __future__ import annotations
 
+import numbers
 import struct
 from collections import namedtuple
 
@@ -57,6 +58,14 @@ def _index(name, names, what: str) -> int:
     if name not in names:
         _refuse(f"{what} must be one of {', '.join(names)} (got {name!r})")
     return names.index(name)
+
+
+def _number(v, what: str) -> float:
+    """A number that float32 holds (a tensor would be read on the host, and
+    its gradient lost)."""
+    if (type(v) is float or isinstance(v, numbers.Real)) and abs(v) <= 3.4028234663852886e38:
+        return float(v)
+    _refuse(f"{what} must be a finite float32 number (got {v!r})")
 
 
 def _dtype(t: torch.Tensor) -> int:
@@ -207,7 +216,7 @@ def _linear_inputs(x, w, bias, activation, residual, scale, keep):
     pb = 0 if bias is None else _take(bias, x, (n,), n, keep, "bias")[0]
     pr, lr = (0, n) if residual is None else _take(residual, x, x.shape[:-1] + (n,), n, keep, "residual")
     m = x.numel() // k
-    return m, k, n, (dt, act, m, k, n, scale, px, pw, pb, pr, lx, lw, lr)
+    return m, k, n, (dt, act, m, k, n, _number(scale, "scale"), px, pw, pb, pr, lx, lw, lr)
 
 
 class _Linear(torch.autograd.Function):
@@ -274,7 +283,7 @@ def _norm_inputs(residual, y, weight, bias, post_weight, post_bias, gate, scale,
         pg, lg = _take(gate, residual, (d,) if channel else shape, d, keep, "gate")
         if channel:
             lg = 0
-    return d, (dt, *kinds, residual.numel() // d, d, scale, eps, pr, py, pw, pb, ppw, ppb, pg, lr, ly, lg)
+    return d, (dt, *kinds, residual.numel() // d, d, _number(scale, "scale"), _number(eps, "eps"), pr, py, pw, pb, ppw, ppb, pg, lr, ly, lg)
 
 
 class _ResidualNorm(torch.autograd.Function):

@@ -222,3 +222,29 @@ def test_forward_mode_is_refused(monkeypatch):
                 with pytest.raises(mb.MLIPError, match="tangent"):
                     call()
     assert len(reached) == 6
+
+
+@pytest.mark.parametrize("bad", [torch.tensor(2.0), torch.tensor(2.0, requires_grad=True), 1e39, -1e39, float("nan"),
+                                 float("inf"), None, "1"], ids=str)
+def test_scale_and_eps_are_numbers(bad, monkeypatch):
+    """A tensor as a scale would be read on the host and lose its gradient;
+    numbers that float32 does not hold have no place in a call either."""
+    reached = []
+    monkeypatch.setattr(ops, "_call", lambda name, *_: reached.append(name))
+    x, w = torch.zeros(4, 8), torch.zeros(8, 8)
+
+    def calls(scale, eps):
+        return [lambda: ops.linear(x, w, scale=scale), lambda: ops.linear_backward(x, x, w, scale=scale),
+                lambda: ops.residual_norm(x, scale=scale), lambda: ops.residual_norm_backward(x, x, x, scale=scale),
+                lambda: ops.residual_norm(x, eps=eps), lambda: ops.residual_norm_backward(x, x, x, eps=eps)]
+
+    with _FakeCuda():
+        for call in calls(bad, bad):
+            with pytest.raises(mb.MLIPError) as e:
+                call()
+            assert e.value.code == INVALID
+        assert not reached
+        for good in (2, 2.0, np.float32(2), np.float64(2)):
+            for call in calls(good, good):
+                call()
+    assert len(reached) == 24
