@@ -90,9 +90,12 @@ def _take(t, first, shape, cols: int, keep: list, name: str):
         _refuse(f"{name} is {t.dtype} on {t.device}, expected {first.dtype} on {first.device}")
     if t.shape != shape:
         _refuse(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.is_contiguous():
+    negated = t.is_neg()  # a view whose memory holds the values' opposites
+    if t.is_contiguous() and not negated:
         return t.data_ptr(), cols
     t = t.detach()
+    if negated:
+        t = t.resolve_neg()
     if t.dim() != 2:
         t = t.reshape(-1, cols)
     if t.shape[0] > 1 and t.stride(0) < cols or cols > 1 and t.stride(1) != 1:

@@ -248,3 +248,16 @@ def test_scale_and_eps_are_numbers(bad, monkeypatch):
             for call in calls(good, good):
                 call()
     assert len(reached) == 24
+
+
+def test_lazily_negated_tensors():
+    """The imaginary part of a conjugate is a view whose values torch negates
+    on reading: what the library is given holds them."""
+    import ctypes
+    for z in (torch.complex(torch.zeros(6, 1), torch.arange(6.0)[:, None]), torch.complex(torch.zeros(3, 4), torch.ones(3, 4))):
+        x, keep = z.conj().imag, []
+        assert x.is_neg()
+        at, ld = ops._take(x, x, x.shape, x.shape[1], keep, "x")
+        got = [[ctypes.c_float.from_address(at + 4 * (i * ld + j)).value for j in range(x.shape[1])]
+               for i in range(x.shape[0])]
+        assert got == x.tolist()
