@@ -139,6 +139,8 @@ def _result(x, m: int, n: int):
 def _grads(inputs, needs):
     """Uninitialised gradients of the inputs that are there and needed, and
     their addresses."""
+    if len(needs) != len(inputs):
+        _refuse(f"needs must have {len(inputs)} entries (got {len(needs)})")
     out = tuple([t.new_empty(t.shape) if t is not None and need else None for t, need in zip(inputs, needs)])
     return out, [0 if t is None else t.data_ptr() for t in out]
 

@@ -261,3 +261,16 @@ def test_lazily_negated_tensors():
         got = [[ctypes.c_float.from_address(at + 4 * (i * ld + j)).value for j in range(x.shape[1])]
                for i in range(x.shape[0])]
         assert got == x.tolist()
+
+
+@pytest.mark.parametrize("needs", [(), (True,) * 2, (True,) * 8], ids=len)
+def test_needs_has_an_entry_for_each_input(needs, monkeypatch):
+    monkeypatch.setattr(ops, "_call", lambda *_: None)
+    x, w = torch.zeros(4, 8), torch.zeros(8, 8)
+    with _FakeCuda():
+        for call in (lambda: ops.gated_linear_backward(x, x, w, w, needs=needs),
+                     lambda: ops.linear_backward(x, x, w, needs=needs),
+                     lambda: ops.residual_norm_backward(x, x, x, needs=needs)):
+            with pytest.raises(mb.MLIPError) as e:
+                call()
+            assert e.value.code == INVALID
