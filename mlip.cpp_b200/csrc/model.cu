@@ -17,6 +17,7 @@
 #include "model.h"
 
 #include <algorithm>
+#include <cctype>
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
@@ -239,7 +240,9 @@ void PETModel::load(const std::string &path, float cutoff_override) {
   // gated feed-forward part: mlp.0 holds the gate's rows, then the value's,
   // and mlp(v) = mlp.3 (silu(gate v) * (value v)); their norms divide by
   // sqrt(var + eps) or, RMS norms, sqrt(mean square + eps).  The reference's
-  // files carry none of these keys.
+  // files carry none of these keys.  The plain form's names count in any
+  // spelling (a file of it may say PostLN, SiLU, LayerNorm); the gated form's
+  // only in this one, which stands for the order of mlp.0 too.
   {
     const std::string type = f.get_string("pet.transformer_type", "postln"),
                       act = f.get_string("pet.activation", "silu"),
@@ -247,13 +250,19 @@ void PETModel::load(const std::string &path, float cutoff_override) {
     h.prenorm = type == "preln";
     h.norm = norm == "rmsnorm" ? NORM_RMS : NORM_LAYER;
     h.norm_eps = f.get_f32("pet.norm_eps", 1e-5f);
-    const bool plain = type == "postln" && act == "silu" && norm == "layernorm";
+    auto letters = [](const std::string &name) {
+      std::string o;
+      for (const char c : name)
+        if (c != '-' && c != '_' && c != ' ') o += static_cast<char>(std::tolower(static_cast<unsigned char>(c)));
+      return o;
+    };
+    const bool plain = letters(type) == "postln" && letters(act) == "silu" && letters(norm) == "layernorm";
     const bool gated = h.prenorm && act == "swiglu" && (norm == "rmsnorm" || norm == "layernorm");
     if (!plain && !gated)
       throw Error(kErrUnsupported, "transformer type '" + type + "' with activation '" + act + "' and normalization '" +
                                        norm + "' is not supported (postln with silu and layernorm, or preln with "
                                        "swiglu and layernorm or rmsnorm)");
-    if (!std::isfinite(h.norm_eps) || h.norm_eps <= 0.0f) throw Error(kErrIO, "pet.norm_eps must be finite and positive");
+    if (gated && (!std::isfinite(h.norm_eps) || h.norm_eps <= 0.0f)) throw Error(kErrIO, "pet.norm_eps must be finite and positive");
   }
   const auto *w0 = f.tensor("model.gnn.0.tl.0.mlp.0.weight");
   if (w0) h.ff = static_cast<int>(w0->ne[1]) / (h.prenorm ? 2 : 1);

@@ -80,3 +80,18 @@ def test_reduced_precision(model_file):
     half = mb.Predictor(path, mb.ModelOptions(precision=1)).predict(s.positions, s.numbers, s.cell, compute_stress=True)
     assert abs(full.energy - half.energy) / s.n_atoms <= 2e-3
     assert np.abs(full.forces - half.forces).max() <= 1e-2
+
+
+def test_spellings_of_the_plain_form(model_file):
+    """Files of the plain form that name it are read as they were before the
+    names meant anything, whatever their spelling; other forms are refused."""
+    s = wl.si_diamond(1, seed=2)
+    want = mb.Predictor(model_file("tiny")).predict(s.positions, s.numbers, s.cell)
+    for names in (("PostLN", "SiLU", "LayerNorm"), ("post-ln", "SILU", "layer_norm")):
+        path = model_file("tiny", transformer_type=names[0], activation=names[1], normalization=names[2], norm_eps=0.0)
+        got = mb.Predictor(path).predict(s.positions, s.numbers, s.cell)
+        assert got.energy == want.energy and (got.forces == want.forces).all()
+    for names in (("PreLN", "SwiGLU", "RMSNorm"), ("preln", "silu", "layernorm"), ("PostLN", "SiLU", "RMSNorm")):
+        path = model_file("tiny", transformer_type=names[0], activation=names[1], normalization=names[2])
+        with pytest.raises(mb.MLIPError, match="not supported"):
+            mb.Predictor(path)
