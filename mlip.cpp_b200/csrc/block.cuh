@@ -19,20 +19,17 @@ inline bool rows16(const void *p, int64_t ld, int dt) {
 }
 // SMs of the current device.
 int sm_count();
-// Reads and clears a device error word after the work on s.
-inline int take_error(const int &word, cudaStream_t s) {
-  int v = 0;
-  CUDA_CHECK(cudaMemcpyFromSymbolAsync(&v, word, sizeof(v), 0, cudaMemcpyDeviceToHost, s));
-  CUDA_CHECK(cudaStreamSynchronize(s));
-  if (v) {
-    const int zero = 0;
-    CUDA_CHECK(cudaMemcpyToSymbolAsync(word, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s));
-    CUDA_CHECK(cudaStreamSynchronize(s));
-  }
-  return v;
+// Device error words count the waits given up and are never cleared, so that
+// none is lost beside a check: whether there are new ones, after the work on s,
+// since the last time this was asked of `word` on the current device.
+bool new_errors(const int &word, cudaStream_t s);
+// A wait given up: into the caller's error word, which is 1 then, or the file's.
+__device__ __forceinline__ void raise_error(int *callers, int &files) {
+  if (callers) atomicExch(callers, 1);
+  else atomicAdd(&files, 1);
 }
 // of the norms' rings (block_norm.cu)
-int norm_error(cudaStream_t s);
+bool norm_error(cudaStream_t s);
 void norm_wait_bound(uint64_t ns);
 
 __device__ __forceinline__ float to_f(float x) { return x; }

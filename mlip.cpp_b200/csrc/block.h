@@ -109,9 +109,9 @@ void residual_norm_fwd(const ResidualNorm &a, Workspace &ws, cudaStream_t s);
 void residual_norm_bwd(const ResidualNorm &a, Workspace &ws, cudaStream_t s);
 constexpr int kMaxNormDim = 16384;
 
-// Error word of the operators' pipelines on the current device: nonzero once a
-// bounded wait ran out.  Synchronises `s`, reads and clears it.
-int block_status(cudaStream_t s);
+// Whether a bounded wait of the operators' pipelines on the current device has
+// run out since the last call.  Synchronises `s`.
+bool block_status(cudaStream_t s);
 // Bound on the waits of the operators' pipelines (0: the default).
 void set_block_wait_bound_ns(uint64_t ns);
 // Test hook: the next norm launch with a ring withholds the copies of its first

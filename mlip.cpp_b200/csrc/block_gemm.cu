@@ -50,8 +50,10 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
-#include <cmath>
 #include <cstring>
+#include <map>
+#include <mutex>
+#include <utility>
 
 #include "block.cuh"
 #include "split16.cuh"
@@ -775,7 +777,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block_gemm(const __grid_constan
       wait_bounded(drain, 0);
     }
     __syncthreads();
-    if (tid == 0) atomicExch(p.err ? p.err : &g_block_err, 1);
+    if (tid == 0) raise_error(p.err, g_block_err);
   }
   if (PAIR) {
     cluster_sync();  // neither CTA leaves while the other may still signal it
@@ -1395,6 +1397,21 @@ int sm_count() {
   return n;
 }
 
+bool new_errors(const int &word, cudaStream_t s) {
+  static std::mutex mutex;
+  static std::map<std::pair<const int *, int>, int> seen;
+  int dev = 0, v = 0;
+  CUDA_CHECK(cudaGetDevice(&dev));
+  CUDA_CHECK(cudaStreamSynchronize(s));  // (not while others wait for the lock)
+  std::lock_guard<std::mutex> lock(mutex);
+  CUDA_CHECK(cudaMemcpyFromSymbolAsync(&v, word, sizeof(v), 0, cudaMemcpyDeviceToHost, s));
+  CUDA_CHECK(cudaStreamSynchronize(s));
+  int &last = seen[{&word, dev}];
+  const bool fresh = v != last;
+  last = v;
+  return fresh;
+}
+
 }  // namespace blk
 
 using namespace blk;
@@ -1407,9 +1424,9 @@ void *Workspace::take(size_t bytes) {
   return p;
 }
 
-int block_status(cudaStream_t s) {
-  const int a = take_error(g_block_err, s), b = norm_error(s);
-  return a | b;
+bool block_status(cudaStream_t s) {
+  const bool a = new_errors(g_block_err, s), b = norm_error(s);
+  return a || b;
 }
 
 void set_block_wait_bound_ns(uint64_t ns) {

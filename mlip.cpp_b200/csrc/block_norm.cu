@@ -288,7 +288,7 @@ struct Feed {
     const uint32_t bar = tc::smem_u32(bars + stage);
     if (ok && !tc::mbar_try_wait(bar, phase) && !tc::wait_within(bar, phase)) {
       ok = false;
-      atomicExch(a.err ? a.err : &g_norm_err, 1);
+      raise_error(a.err, g_norm_err);
       // rows issued and not waited for: this one and the ring's next
       if (t == 0 && !stalled())
         for (int i = 0; i < ring.stages && at + i * step < a.M; ++i) {
@@ -759,7 +759,7 @@ NormArgs args_of(const ResidualNorm &a) {
 
 using namespace blk;
 
-int blk::norm_error(cudaStream_t s) { return take_error(g_norm_err, s); }
+bool blk::norm_error(cudaStream_t s) { return new_errors(g_norm_err, s); }
 void blk::norm_wait_bound(uint64_t ns) { CUDA_CHECK(cudaMemcpyToSymbol(tc::g_wait_ns, &ns, sizeof(ns))); }
 
 void inject_norm_stall() { g_norm_stall.store(true); }

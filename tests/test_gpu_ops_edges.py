@@ -291,3 +291,41 @@ def test_forward_mode_is_refused():
             call(x, w)
     for call in calls:
         call(x, w)
+
+
+def test_every_expired_wait_is_reported_once():
+    """Waits given up between, beside and after checks, on two streams: each
+    check tells whether there were any since the last one."""
+    L = mb.lib()
+    r = torch.randn(40, 256, device="cuda")
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+
+    def expire(stream):
+        with torch.cuda.stream(stream):
+            assert L.mlipcpp_b200_inject_norm_stall() == mb.OK
+            ops.residual_norm(r)
+        stream.synchronize()
+
+    def failed(stream):
+        with torch.cuda.stream(stream):
+            try:
+                ops.check_status()
+            except mb.MLIPError as e:
+                assert e.code == mb.COMPUTATION
+                return True
+        return False
+
+    assert L.mlipcpp_b200_set_wait_bound_ns(1_000_000) == mb.OK
+    try:
+        for a in streams:
+            for b in streams:
+                assert not failed(b)
+                expire(a)
+                assert failed(b) and not failed(a) and not failed(b)
+                expire(a)
+                expire(b)
+                assert failed(a) and not failed(b)
+    finally:
+        assert L.mlipcpp_b200_set_wait_bound_ns(0) == mb.OK
+    assert not failed(streams[0])
