@@ -95,3 +95,44 @@ def test_spellings_of_the_plain_form(model_file):
         path = model_file("tiny", transformer_type=names[0], activation=names[1], normalization=names[2])
         with pytest.raises(mb.MLIPError, match="not supported"):
             mb.Predictor(path)
+
+
+@pytest.mark.parametrize("grid", [(1, 1, 2), (2, 2, 2)])
+def test_domains(model_file, grid):
+    """A cell divided over ranks (emulated on one GPU) equals the whole one."""
+    from mlipcpp_b200 import domain as dd
+    path, s = model_file("pet-mad-s-gated", 5), wl.si_diamond(4, seed=61)
+    full = mb.Predictor(path).predict(s.positions, s.numbers, s.cell, s.pbc, compute_stress=True)
+    e, f, virial, _ = dd.run_emulated(lambda: mb.Predictor(path), s, grid)
+    assert abs(e - full.energy) / s.n_atoms <= 1e-5
+    assert np.abs(f - full.forces).max() <= 1e-4
+    assert np.abs(np.asarray(virial) / abs(np.linalg.det(np.asarray(s.cell, np.float64))) - full.stress).max() <= 1e-4
+
+
+@pytest.mark.parametrize("name", ["tiny-gated", "pet-mad-s-gated"])
+def test_non_conservative_heads(model_file, name):
+    path, s = model_file(name, 8, nc=True), wl.si_diamond(2, seed=62)
+    ref = pet_oracle.load_oracle(path, torch.float64).predict([s], compute_forces=False, compute_nc=True)[0]
+    got = mb.Predictor(path).predict_with_options(s.positions, s.numbers, s.cell, s.pbc, mb.PredictOptions(True, True, True))
+    check(got, ref, s.n_atoms)
+
+
+def test_packed_batch_and_kept_lists(model_file):
+    """The packed call equals the batched one, and a kept neighbour list a
+    fresh one."""
+    from mlipcpp_b200 import sharding as sh
+    path = model_file("pet-mad-s-gated", 12)
+    p, mols = mb.Predictor(path), wl.molecules(20, seed=13)
+    b = sh.PackedBatch.pack(mols)
+    r = p.predict_packed(b.positions, b.numbers, b.n_atoms)
+    for k, w in enumerate(p.predict_batch(mols)):
+        assert r.energies[k] == np.float32(w.energy)
+        np.testing.assert_array_equal(r.forces[b.first[k]:b.first[k + 1]], w.forces)
+    s, kept = wl.si_diamond(2, seed=3), mb.Predictor(path)
+    kept.set_neighbor_skin(0.6)
+    rng = np.random.default_rng(5)
+    for _ in range(3):
+        pos = s.positions + rng.uniform(-0.1, 0.1, s.positions.shape).astype(np.float32)
+        a, f = kept.predict(pos, s.numbers, s.cell), p.predict(pos, s.numbers, s.cell)
+        assert abs(a.energy - f.energy) / s.n_atoms <= 5e-6
+        assert np.abs(a.forces - f.forces).max() <= 5e-5
