@@ -258,9 +258,11 @@ __global__ void __launch_bounds__(256) k_few_rows(const FewRows a, int wpr) {
   finish<T, DUAL>(a, lane, n, v, w);
 }
 
+// (K: as in the tiled products, the truncations of one of the eight warps' sums,
+// 2^-23 for each 16 terms, must not pass half a rounding of the result)
 bool few_mma(const FewRows &a) {
-  return a.dt != DT_F32 && a.K % 8 == 0 && rows16(a.x, a.ldx, a.dt) && rows16(a.w0, a.ldw0, a.dt) &&
-         (!a.w1 || rows16(a.w1, a.ldw1, a.dt));
+  return a.dt != DT_F32 && a.K % 8 == 0 && a.K <= (a.dt == DT_F16 ? 262144 : 2097152) && rows16(a.x, a.ldx, a.dt) &&
+         rows16(a.w0, a.ldw0, a.dt) && (!a.w1 || rows16(a.w1, a.ldw1, a.dt));
 }
 
 template <typename T, int MR, bool DUAL>

@@ -329,3 +329,15 @@ def test_every_expired_wait_is_reported_once():
     finally:
         assert L.mlipcpp_b200_set_wait_bound_ns(0) == mb.OK
     assert not failed(streams[0])
+
+
+@pytest.mark.parametrize("m", [1, 8, 16])
+def test_long_f16_rows(m):
+    """The same of a few rows with 2^22 inputs."""
+    k, n = 1 << 22, 40
+    f16 = torch.float16
+    a, b, scale = 1 + 37 / 1024, 1 + 101 / 1024, 2.0 ** -16
+    x, w = torch.full((m, k), a, dtype=f16, device="cuda"), torch.full((n, k), b, dtype=f16, device="cuda")
+    y = ops.linear(x, w, scale=scale)
+    ref, u = k * a * b * scale, unit(f16)
+    assert (y.double() - ref).abs().max().item() <= 1.5 * u * (1 + u) * ref
