@@ -229,8 +229,8 @@ mlipcpp_error_t mlipcpp_b200_domain_stats(mlipcpp_b200_domain_t domain, double s
  * may run at the same time need one each.  Work is ordered on `stream` (NULL:
  * the legacy default stream); nothing is allocated and nothing waited for, so
  * calls can be captured into a graph.  Errors found before the launch are
- * returned; mlipcpp_b200_ops_status reports a tensor-core pipeline whose
- * bounded wait ran out since. */
+ * returned; mlipcpp_b200_ops_status reports a pipeline whose bounded wait
+ * ran out since. */
 typedef enum {
   MLIPCPP_B200_DTYPE_F32 = 0,
   MLIPCPP_B200_DTYPE_F16 = 1,

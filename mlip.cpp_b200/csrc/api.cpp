@@ -1287,12 +1287,15 @@ mlipcpp_error_t mlipcpp_b200_ops_status(void *stream) {
   }
   try {
     if (pet::block_status(static_cast<cudaStream_t>(stream))) {
-      set_error("A tensor-core pipeline of an operator timed out; its outputs are incomplete");
+      set_error("A pipeline of an operator gave up a wait; its outputs are incomplete");
       return MLIPCPP_ERROR_COMPUTATION;
     }
   } catch (const pet::Error &e) {
     set_error(e.what());
     return static_cast<mlipcpp_error_t>(e.code);
+  } catch (const std::exception &e) {
+    set_error(e.what());
+    return MLIPCPP_ERROR_COMPUTATION;
   }
   clear_error();
   return MLIPCPP_OK;
