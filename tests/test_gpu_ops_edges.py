@@ -341,3 +341,13 @@ def test_long_f16_rows(m):
     y = ops.linear(x, w, scale=scale)
     ref, u = k * a * b * scale, unit(f16)
     assert (y.double() - ref).abs().max().item() <= 1.5 * u * (1 + u) * ref
+
+
+def test_long_f16_tokens():
+    """Both weights' gradients over more tokens than one accumulator takes,
+    over more tiles than there are SMs."""
+    g, f16 = gen(34), torch.float16
+    m, k, f = 40000, 1024, 3000
+    x, dh = rand(g, m, k, dtype=f16), rand(g, m, f, dtype=f16, std=2.0 ** -6)
+    wg, wv = rand(g, f, k, dtype=f16, std=k ** -0.5), rand(g, f, k, dtype=f16, std=k ** -0.5)
+    check_gated(x, wg, wv, None, None, "gelu_tanh", dh)
