@@ -249,10 +249,10 @@ struct Ring {
 
 // One group's ring: `take` waits for the next row's inputs.  A thread whose
 // wait runs out records the error and waits no more: the results are void.  The
-// one that issues the copies then waits, with the default bound, for those on
-// their way, and issues no further ones: no CTA ends while something is written
-// to its shared memory, and no barrier is armed again in an unfinished phase
-// (the others run into their own bounds, once each).
+// one that issues the copies issues no further ones, so that no barrier is armed
+// again in an unfinished phase (the others run into their own bounds, once each),
+// and waits at its end, with the default bound, for those on their way: no CTA
+// ends while something is written to its shared memory.
 template <int TPR>
 struct Feed {
   const NormArgs &a;
@@ -261,7 +261,7 @@ struct Feed {
   char *base;
   int64_t row, step;
   int t, stage, phase;
-  bool ok;
+  int lost;  // 1 + rows since the wait that ran out, or 0
   __device__ __forceinline__ void issue(int s, int64_t at) {
     const void *src[kInputs] = {a.r, a.y, a.ds, a.dout, a.ldg ? a.gate : nullptr};
     const int64_t ld[kInputs] = {a.ldr, a.ldy, a.ldds, a.lddo, a.ldg};
@@ -283,27 +283,31 @@ struct Feed {
     if (t == 0 && !stalled())
       for (int s = 0; s < ring.stages && row + s * step < a.M; ++s) issue(s, row + s * step);
   }
-  // inputs of row `at`
-  __device__ __forceinline__ const char *take(int64_t at) {
+  __device__ __forceinline__ const char *take() {
     const uint32_t bar = tc::smem_u32(bars + stage);
-    if (ok && !tc::mbar_try_wait(bar, phase) && !tc::wait_within(bar, phase)) {
-      ok = false;
+    if (!lost && !tc::mbar_try_wait(bar, phase) && !tc::wait_within(bar, phase)) {
+      lost = 1;
       raise_error(a.err, g_norm_err);
-      // rows issued and not waited for: this one and the ring's next
-      if (t == 0 && !stalled())
-        for (int i = 0; i < ring.stages && at + i * step < a.M; ++i) {
-          const int s = stage + i < ring.stages ? stage + i : stage + i - ring.stages;
-          tc::wait_bounded(tc::smem_u32(bars + s), phase ^ (s < stage ? 1 : 0));
-        }
     }
     return base + static_cast<size_t>(stage) * ring.inputs * ring.row_bytes;
   }
   // every thread of the group has read the stage (after a group barrier)
   __device__ __forceinline__ void give(int64_t at) {
-    if (t == 0 && ok && at + ring.stages * step < a.M) issue(stage, at + ring.stages * step);
+    if (t == 0 && !lost && at + ring.stages * step < a.M) issue(stage, at + ring.stages * step);
+    lost += lost != 0;
     if (++stage == ring.stages) {
       stage = 0;
       phase ^= 1;
+    }
+  }
+  // after the last row: the row of the wait that ran out and the ring's next
+  // ones, as far as there were rows, had been issued
+  __device__ __forceinline__ void end() {
+    if (!lost || t != 0 || stalled()) return;
+    const int n = ring.stages, rows = lost - 1, first = phase * n + stage - rows % (2 * n) + 2 * n;
+    for (int i = 0; i < min(n, rows); ++i) {
+      const int at = (first + i) % (2 * n);
+      tc::wait_bounded(tc::smem_u32(bars + at % n), at / n);
     }
   }
 };
@@ -374,7 +378,7 @@ struct Vectors {
   int64_t row = static_cast<int64_t>(blockIdx.x) * NG + group;                                             \
   Sum<TPR> sum{slots[group], group, 0};                                                                    \
   Vectors<R, T, RING> vec{a};                                                                              \
-  Feed<TPR> feed{a, ring, bars[group], nullptr, row, step, t, 0, 0, true};                                 \
+  Feed<TPR> feed{a, ring, bars[group], nullptr, row, step, t, 0, 0, 0};                                    \
   if (RING) {                                                                                              \
     if (threadIdx.x == 0) {                                                                                \
       for (int g = 0; g < NG; ++g)                                                                         \
@@ -399,7 +403,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_norm_fwd(const NormArgs a, co
   for (; row < a.M; row += step) {
     float2 x[P];
     const char *in = nullptr;
-    if (RING) in = feed.take(row);
+    if (RING) in = feed.take();
     if (RING) R::load(in, 0, t, d, x);
     else R::load(a.r, row * a.ldr, t, d, x);
 #pragma unroll
@@ -433,6 +437,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_norm_fwd(const NormArgs a, co
     vec.plus_b(t, x);
     if (a.out) R::store(a.out, row * a.ldo, t, d, x);
   }
+  if (RING) feed.end();
 }
 
 // HB: a bias or its gradient is there (its sums take E registers each).
@@ -455,7 +460,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 2 : 1) k_norm_bwd(const NormAr
     float2 n[P], u[P], g[P], f[P];
     const char *in[kInputs] = {};
     if (RING) {
-      const char *p = feed.take(row);
+      const char *p = feed.take();
       const void *there[kInputs] = {a.r, a.y, a.ds, a.dout, each ? a.gate : nullptr};
 #pragma unroll
       for (int k = 0; k < kInputs; ++k) {
@@ -566,6 +571,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 2 : 1) k_norm_bwd(const NormAr
       R::store(a.dy, row * a.lddy, t, d, g);
     }
   }
+  if (RING) feed.end();
   // this CTA's sums, each [CTA][d], the groups' added in order
   if (!a.part) return;
 #pragma unroll
