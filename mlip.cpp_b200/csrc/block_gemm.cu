@@ -1306,7 +1306,9 @@ void run(const Product &g, Workspace &ws, cudaStream_t s) {
   p.tiles_m = static_cast<int>((g.M + bm - 1) / bm);
   p.tiles_n = static_cast<int>(tiles / p.tiles_m / p.batch);
   // few tiles and a long contraction: divided over the SMs, where that saves
-  // more k tiles (about 0.35 us each) than the second kernel costs (6 us)
+  // 20 k tiles or more (0.2 us each of 128 x 128 in f16, more of wider tiles and
+  // of f32) against the 6 us of the second kernel.  128 x 128 outputs in f16:
+  // 16, 24, 32 and 64 k tiles in 8.3, 11.7, 9.9 and 11.2 us
   const int at_once = tile.pair ? sms / 2 : sms;
   int splits = 1;
   if (tiles * 2 <= at_once && p.kt >= 16) {

@@ -25,9 +25,11 @@
 // Outputs leave L2 before anything else (__stcs): the inputs of later rows are
 // still to be read there.  16,383 x 4096 f16 forward: 101 us a call, without 106.
 //
-// Measured: 16,383 x 4096 f16 forward in 93 us (5.8 TB/s), 8192 x 4096 bf16
-// backward in 98 us (4.1 TB/s: four reductions a row and only two CTAs an SM,
-// since a row's values and its column sums take 110 registers a thread).
+// Measured: 16,383 x 4096 f16 forward in 98 us (5.5 TB/s), 8192 x 4096 bf16
+// backward in 101 us (4.0 TB/s: four reductions a row and only two CTAs an SM,
+// since a row's values and its column sums take 110 registers a thread).  Rows
+// that are not 16-byte multiples, an element at a time and with spills, take 2.4
+// and 3.1 times as long (4095 columns).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>

@@ -933,8 +933,6 @@ void PETModel::forward_backward(bool grad) {
     head_bwd(L.node, a.zn1[l], a.zn2[l], nullptr, 0, N1, dst);
     if (E1 > 0) head_bwd(L.edge, a.ze1[l], a.ze2[l], a.fc, Nl_[l], E1, dst);
   };
-  // dxin: the block input's gradient in fp32; in chain mode it goes instead
-  // to *sdxin in split form when that is given
   // Pre-norm block: the stream's gradient dy goes around each part and through
   // its norm.  The feed-forward part's input is recomputed from the stream.
   auto block_pre_bwd = [&](int b, const float *dy, float *dxin) {
@@ -968,6 +966,8 @@ void PETModel::forward_backward(bool grad) {
     n.dresidual = {dxin, d};
     residual_norm_bwd(n, ws, s);
   };
+  // dxin: the block input's gradient in fp32; in chain mode it goes instead
+  // to *sdxin in split form when that is given
   auto block_bwd = [&](int b, const float *dy, float *dxin, const Split16View *sdxin = nullptr) {
     if (h.prenorm) {
       block_pre_bwd(b, dy, dxin);

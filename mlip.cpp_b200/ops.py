@@ -7,8 +7,9 @@
 They are the feed-forward half of a pre-norm block: ``residual_norm`` adds a
 sublayer's output to the stream and normalises it for the next sublayer,
 ``gated_linear`` and ``linear`` are that sublayer.  The library's PET models
-with gated feed-forward layers run on the same kernels; here they take any
-tensors, e.g. to build and train a model around it.
+with gated feed-forward layers run the first two of these on the same kernels
+(in float32); here they take any tensors, e.g. to build and train a model
+around it.
 
 Types: float32, float16 and bfloat16, one per call.  Leading dimensions are
 flattened to rows (there may be none); a tensor whose rows are not contiguous
@@ -182,7 +183,8 @@ class _GatedLinear(torch.autograd.Function):
 def gated_linear(x, w_gate, w_value, b_gate=None, b_value=None, activation="silu"):
     """act(x w_gate^T + b_gate) * (x w_value^T + b_value): x [..., K], weights
     [F, K], biases [F] -> [..., F].  Both projections, the activation and the
-    product are one kernel."""
+    product are one kernel; operands that are split (float32) or packed (rows
+    that are not 16-byte aligned) and a divided contraction take another each."""
     if ((x.requires_grad or w_gate.requires_grad or w_value.requires_grad or _wants(b_gate) or _wants(b_value))
             and torch.is_grad_enabled()):
         return _GatedLinear.apply(x, w_gate, w_value, b_gate, b_value, activation)
@@ -240,7 +242,7 @@ class _Linear(torch.autograd.Function):
 
 def linear(x, w, bias=None, activation="identity", residual=None, scale=1.0):
     """residual + scale act(x w^T + bias): x [..., K], w [N, K], bias [N],
-    residual [..., N] -> [..., N], in one kernel."""
+    residual [..., N] -> [..., N], in the kernels of gated_linear."""
     if ((x.requires_grad or w.requires_grad or _wants(bias) or _wants(residual)) and torch.is_grad_enabled()):
         return _Linear.apply(x, w, bias, activation, residual, scale)
     keep: list = []
