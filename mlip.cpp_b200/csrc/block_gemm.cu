@@ -11,8 +11,9 @@
 // backward pass needs a transposed copy.
 //
 //  * 16-bit: one kind::f16 product, fp32 accumulation in tensor memory over
-//    the whole contraction (divided where its truncations could show, see run); BN = 256 (one 128 x 256 tile, two accumulators)
-//    or 128 (four accumulators) when 256-wide tiles would leave SMs idle.
+//    the whole contraction (divided where its truncations could show, see
+//    run); BN = 256 (one 128 x 256 tile, two accumulators) or 128 (four
+//    accumulators) when 256-wide tiles would leave SMs idle.
 //  * f32: A = 2^-s (hi + lo) and B = 2^-t (hi + lo) with one scale per row (the
 //    output's row or column) and 128 contraction elements (one for all of a
 //    model's weight, split when it was loaded) in the way of split16.cuh;
@@ -1319,7 +1320,8 @@ void run(const Product &g, Workspace &ws, cudaStream_t s) {
   // 2^-23 of the sum (f32 joins in registers instead).  Beyond this many all of
   // them together could pass half a rounding of the result: divided further.
   if (!f32) {
-    const int most = (g.dt == DT_F16 ? 32768 : 262144) / BK;  // 2^11 steps of 2^-23 against 2^-11 / 2, 2^14 against 2^-8 / 2
+    // (2^11 steps of 2^-23 against 2^-11 / 2 in f16, 2^14 against 2^-8 / 2 in bf16)
+    const int most = (g.dt == DT_F16 ? 32768 : 262144) / BK;
     splits = std::max(splits, (p.kt + most - 1) / most);
   }
   p.kt_split = (p.kt + splits - 1) / splits;

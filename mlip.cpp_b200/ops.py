@@ -16,8 +16,8 @@ flattened to rows (there may be none); a tensor whose rows are not contiguous
 is copied first.  Everything runs on the tensors' device and its current
 stream, without waiting; the working memory comes from torch's allocator.
 Where an input requires grad, the forwards record themselves for autograd
-(first derivatives, reverse mode; forward-mode duals are refused); the ``*_backward`` functions are the same gradients
-called directly.  An autograd backward is captured into a CUDA graph only
+(first derivatives, reverse mode; forward-mode duals are refused); the
+``*_backward`` functions are the same gradients called directly.  An autograd backward is captured into a CUDA graph only
 when nothing recorded earlier with the same parameters is still held (torch
 ties a parameter's accumulation to the stream of its first use); the
 ``*_backward`` functions have no such condition.
@@ -290,7 +290,8 @@ def _norm_inputs(residual, y, weight, bias, post_weight, post_bias, gate, scale,
         pg, lg = _take(gate, residual, (d,) if channel else shape, d, keep, "gate")
         if channel:
             lg = 0
-    return d, (dt, *kinds, residual.numel() // d, d, _number(scale, "scale"), _number(eps, "eps"), pr, py, pw, pb, ppw, ppb, pg, lr, ly, lg)
+    return d, (dt, *kinds, residual.numel() // d, d, _number(scale, "scale"), _number(eps, "eps"), pr, py, pw, pb,
+               ppw, ppb, pg, lr, ly, lg)
 
 
 class _ResidualNorm(torch.autograd.Function):
