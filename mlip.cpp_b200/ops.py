@@ -17,10 +17,10 @@ is copied first.  Everything runs on the tensors' device and its current
 stream, without waiting; the working memory comes from torch's allocator.
 Where an input requires grad, the forwards record themselves for autograd
 (first derivatives, reverse mode; forward-mode duals are refused); the
-``*_backward`` functions are the same gradients called directly.  An autograd backward is captured into a CUDA graph only
-when nothing recorded earlier with the same parameters is still held (torch
-ties a parameter's accumulation to the stream of its first use); the
-``*_backward`` functions have no such condition.
+``*_backward`` functions are the same gradients called directly.  An autograd
+backward is captured into a CUDA graph only when nothing recorded earlier with
+the same parameters is still held (torch ties a parameter's accumulation to the
+stream of its first use); the ``*_backward`` functions have no such condition.
 
 The kernels are those of the C API (include/mlipcpp_b200.h), which states
 precision and limits; a refused call raises MLIPError.
